@@ -13,7 +13,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from .graph import Graph, as_padded, is_vec4, ld_of, new_padded, rowmajor
+from .graph import Graph, Segments, as_padded, is_vec4, ld_of, new_padded, pad4, rowmajor, segments_of
 from .noise import current_noise
 
 _ws_cache: "dict[tuple, torch.Tensor]" = {}
@@ -2426,3 +2426,234 @@ def gather_i64(src: torch.Tensor, idx: torch.Tensor) -> torch.Tensor:
     out = torch.empty_like(flat)
     _lib.call("hgv_gather_i64", src.data_ptr(), flat.data_ptr(), flat.numel(), out.data_ptr(), _lib.stream())
     return out.view(idx.shape)
+
+
+# --------------------------------------------------------------------------------------
+# activation checkpoints in 8 bits
+# --------------------------------------------------------------------------------------
+def _on_device(t: torch.Tensor):
+    """Context in which the current device is the tensor's (the library launches on the current device's stream)."""
+    return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+def _check_matrix(name: str, t, device=None, columns: Optional[int] = None):
+    if not isinstance(t, torch.Tensor) or t.dim() != 2 or t.dtype != torch.float32:
+        raise _lib.HgvError(f"{name} must be a 2-D float32 tensor, got "
+                            f"{(t.dtype, tuple(t.shape)) if isinstance(t, torch.Tensor) else type(t).__name__}")
+    _lib.require_cuda(t)
+    if device is not None and t.device != device:
+        raise _lib.HgvError(f"{name} is on {t.device}, expected {device}")
+    if columns is not None and t.size(1) != columns:
+        raise _lib.HgvError(f"{name} has {t.size(1)} columns, expected {columns}")
+
+
+def _check_vector(name: str, t, size: int, device):
+    if t is None:
+        return None
+    if t.dim() != 1 or t.numel() != size or t.dtype != torch.float32 or t.device != device:
+        raise _lib.HgvError(f"{name} must be a float32 vector of {size} on {device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    return t.contiguous()
+
+
+class Packed8:
+    """A matrix kept as 8-bit integers with one power of two per row and block of 32 columns (see :func:`pack8`):
+    ``q`` int8 ``[N, ldq]``, ``scale`` uint8 ``[N, ceil(C / 32)]``, ``shape`` ``(N, C)``; 1.03 bytes per element."""
+    __slots__ = ("q", "scale", "shape")
+
+    def __init__(self, q: torch.Tensor, scale: torch.Tensor, shape):
+        self.q, self.scale, self.shape = q, scale, tuple(shape)
+
+    def unpack(self) -> torch.Tensor:
+        """The values that stand for the matrix, as fp32 (a block that held an infinity or NaN reads back as NaN)."""
+        n, c = self.shape
+        out = new_padded(n, c, self.q.device, zero_pad=False)
+        if n:
+            with _on_device(self.q):
+                _lib.call("hgv_unpack8", self.q.data_ptr(), self.q.stride(0), self.scale.data_ptr(), n, c, out.data_ptr(), out.stride(0),
+                          _lib.stream())
+        return out
+
+    def nbytes(self) -> int:
+        return self.q.numel() + self.scale.numel()
+
+    def __repr__(self):
+        return f"Packed8({self.shape[0]} x {self.shape[1]}, {self.q.device})"
+
+
+def pack8(x: torch.Tensor) -> Packed8:
+    """``x`` in 8 bits: block by block (32 columns of one row) the integers ``q = round(x / 2^e)``, ties to even, with the
+    smallest e for which none leaves [-127, 127].  Every value is off by at most half a step ``2^e``, and a step is at most
+    1/63 of the block's largest magnitude (steps below 2^-126 do not occur, nor above 2^121: beyond 127.5 * 2^121 values are
+    cut).  Not differentiable by itself: :func:`linear8` and
+    :func:`group_norm_act` keep their inputs this way for their backward passes."""
+    x = plain(x).detach()
+    _check_matrix("x", x)
+    if x.size(1) < 1:
+        raise _lib.HgvError("pack8: x has no columns")
+    x = rowmajor(x)
+    n, c = x.shape
+    q = torch.empty(n, (c + 15) // 16 * 16, dtype=torch.int8, device=x.device)
+    scale = torch.empty(n, (c + 31) // 32, dtype=torch.uint8, device=x.device)
+    if n:
+        with _on_device(x):
+            _lib.call("hgv_pack8", x.data_ptr(), ld_of(x), n, c, q.data_ptr(), q.stride(0), scale.data_ptr(), _lib.stream())
+    return Packed8(q, scale, (n, c))
+
+
+def _own_rows(t: torch.Tensor) -> torch.Tensor:
+    """``as_padded``, but a column slice of a wider matrix is copied where its rows' last 16 bytes hold foreign columns."""
+    p = as_padded(t)
+    if p is t and t.size(1) % 4 and ld_of(t) > pad4(t.size(1)):
+        p = new_padded(t.size(0), t.size(1), t.device)
+        p.copy_(t)
+    return p
+
+
+class _Linear8(torch.autograd.Function):
+    """y = x W^T + b that keeps x in 8 bits; the weight gradient is formed from the kept values."""
+
+    @staticmethod
+    def forward(ctx, x, w, bias):
+        x = _own_rows(x)
+        need = ctx.needs_input_grad
+        fwd, ctx.image = _images((w, None, False), (w, None, True) if need[0] else None)
+        y = _gemm_nt(x, fwd, None, bias, w.size(0))
+        ctx.packed = None
+        if need[1]:
+            p = pack8(x)
+            ctx.packed = p.shape
+            ctx.save_for_backward(w, p.q, p.scale)
+        else:
+            ctx.save_for_backward(w)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        need = ctx.needs_input_grad
+        w = ctx.saved_tensors[0]
+        gx = gw = gb = None
+        with _on_device(g):
+            g = _own_rows(g)
+            if need[1]:
+                gw, gb = _weight_grad8(g, Packed8(*ctx.saved_tensors[1:], ctx.packed), need[2])
+            elif need[2]:
+                gb = g.sum(0)
+            if need[0]:
+                gx = _gemm_nt(g, ctx.image, None, None, w.size(1))
+        return gx, gw, gb
+
+
+def _weight_grad8(g: torch.Tensor, x8: Packed8, want_bias: bool):
+    """(g^T v  [N, K], column sums of g or None), v the values of ``x8``."""
+    return _gemm_tn(g, x8.unpack(), want_bias)
+
+
+def linear8(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``x @ w.T + bias`` with fp32 results, as :func:`dual_linear`, that keeps ``x`` in 8 bits (:func:`pack8`) for the
+    backward pass: a quarter of the memory.  The gradients with respect to ``x`` and ``bias`` are those of the exact
+    product; the weight gradient is ``g.T @ v`` with ``v`` the 8-bit values of ``x``.  Gradients cannot be differentiated
+    again."""
+    x = plain(x)
+    _check_matrix("x", x)
+    _check_matrix("w", w, x.device, x.size(1))
+    if not 1 <= w.size(0) <= MAX_GEMM_N or not 1 <= w.size(1) <= MAX_GEMM_N:
+        raise _lib.HgvError(f"projection widths above {MAX_GEMM_N} are not supported (got {tuple(w.shape)})")
+    bias = _check_vector("bias", bias, w.size(0), x.device)
+    if x.size(0) == 0:
+        return torch.nn.functional.linear(x, w, bias)           # no rows: an empty matrix, zero gradients
+    with _on_device(x):
+        return _Linear8.apply(x, w, bias)
+
+
+# --------------------------------------------------------------------------------------
+# group norm with an activation, per graph
+# --------------------------------------------------------------------------------------
+_ACTS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3}
+
+
+class _GroupNormAct(torch.autograd.Function):
+    """act(group_norm(x) * w + b) with statistics per (graph, group); the backward pass recomputes the normalised values
+    from x, or from its 8-bit form."""
+
+    @staticmethod
+    def forward(ctx, x, w, b, seg: Segments, groups, act, eps, keep8):
+        x = rowmajor(x)
+        n, c = x.shape
+        lib = _lib.load()
+        out = new_padded(n, c, x.device, zero_pad=False)
+        mean = torch.empty(seg.num_graphs, groups, dtype=torch.float64, device=x.device)
+        rstd = torch.empty(seg.num_graphs, groups, dtype=torch.float32, device=x.device)
+        small, rows, batches, n_batches, chunks = seg._norm_plan(lib.hgv_group_norm_small_rows(c, groups), 4 * ld_of(x))
+        listed = len(seg._sorted)
+        nws = lib.hgv_group_norm_ws(chunks, seg.num_graphs, listed, small, c, groups, 0)
+        ws = torch.empty(nws, dtype=torch.uint8, device=x.device)
+        _lib.call("hgv_group_norm_fwd", x.data_ptr(), ld_of(x), c, groups, act, float(eps), _lib.ptr(w), _lib.ptr(b), seg._ptr.data_ptr(),
+                  seg._order.data_ptr(), seg._chunks.data_ptr(), seg._first.data_ptr(), seg.num_graphs, listed, small, rows, n_batches,
+                  batches, chunks, out.data_ptr(), out.stride(0), mean.data_ptr(), rstd.data_ptr(), ws.data_ptr(), nws, _lib.stream())
+        ctx.seg, ctx.cfg = seg, (groups, act)
+        ctx.packed = None
+        if keep8 and any(ctx.needs_input_grad[:3]):
+            p = pack8(x)
+            ctx.packed = p.shape
+            ctx.save_for_backward(w, b, mean, rstd, p.q, p.scale)
+        else:
+            ctx.save_for_backward(w, b, mean, rstd, x)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        seg, (groups, act) = ctx.seg, ctx.cfg
+        w, b, mean, rstd = ctx.saved_tensors[:4]
+        x, q, scale = (None, *ctx.saved_tensors[4:]) if ctx.packed else (ctx.saved_tensors[4], None, None)
+        need = ctx.needs_input_grad
+        with _on_device(g):
+            g = rowmajor(g)
+            n, c = g.shape
+            lib = _lib.load()
+            gx = new_padded(n, c, g.device, zero_pad=False) if need[0] else None
+            gw = torch.empty(c, dtype=torch.float32, device=g.device) if need[1] else None
+            gb = torch.empty(c, dtype=torch.float32, device=g.device) if need[2] else None
+            row_bytes = 4 * ld_of(g) + (4 * ld_of(x) if x is not None else q.stride(0))
+            small, rows, batches, n_batches, chunks = seg._norm_plan(lib.hgv_group_norm_small_rows(c, groups), row_bytes)
+            listed = len(seg._sorted)
+            nws = lib.hgv_group_norm_ws(chunks, seg.num_graphs, listed, small, c, groups, 1)
+            ws = torch.empty(nws, dtype=torch.uint8, device=g.device)
+            _lib.call("hgv_group_norm_bwd", g.data_ptr(), ld_of(g), _lib.ptr(x), ld_of(x) if x is not None else 0, _lib.ptr(q),
+                      q.stride(0) if q is not None else 0, _lib.ptr(scale), c, groups, act, _lib.ptr(w), _lib.ptr(b), seg._ptr.data_ptr(),
+                      seg._order.data_ptr(), seg._chunks.data_ptr(), seg._first.data_ptr(), seg.num_graphs, listed, small, rows,
+                      n_batches, batches, chunks, mean.data_ptr(), rstd.data_ptr(), _lib.ptr(gx), gx.stride(0) if gx is not None else 0,
+                      _lib.ptr(gw), _lib.ptr(gb), ws.data_ptr(), nws, _lib.stream())
+        return gx, gw, gb, None, None, None, None, None
+
+
+def group_norm_act(x: torch.Tensor, segments, groups: int, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
+                   act: str = "silu", eps: float = 1e-5, keep8: bool = False) -> torch.Tensor:
+    """``act(group_norm(x) * weight + bias)`` over the rows of each graph: ``x`` ``[N, C]`` fp32, the C columns in ``groups``
+    equal groups of neighbours, mean and biased variance per (graph, group).  ``segments``: a
+    :class:`~hgvae_amd.graph.Segments`, or a ``batch`` vector (then one host synchronisation per call).  ``act``: "none",
+    "relu", "silu" or "gelu" (erf).  ``groups=1`` normalises a graph as a whole, ``groups=C`` every column of it by itself.
+
+    The backward pass recomputes what it needs from ``x``; with ``keep8`` from the 8-bit form of it (:func:`pack8`, a quarter
+    of the memory): statistics are those of the exact x, normalised values those of the kept one.  Gradients cannot be
+    differentiated again."""
+    x = plain(x)
+    _check_matrix("x", x)
+    if act not in _ACTS:
+        raise _lib.HgvError(f"unknown activation {act!r} (one of {', '.join(_ACTS)})")
+    groups = int(groups)
+    if groups < 1 or x.size(1) < 1 or x.size(1) % groups:
+        raise _lib.HgvError(f"{x.size(1)} columns cannot be split into {groups} groups")
+    if not eps >= 0.0:
+        raise _lib.HgvError(f"eps must be >= 0, got {eps}")
+    weight = _check_vector("weight", weight, x.size(1), x.device)
+    bias = _check_vector("bias", bias, x.size(1), x.device)
+    with _on_device(x):
+        seg = segments_of(segments, x.size(0))
+        if seg.device != x.device:
+            raise _lib.HgvError(f"segments are on {seg.device}, x is on {x.device}")
+        if x.size(0) == 0:                                      # an empty matrix whose gradients are zeros
+            y = x * 1.0 if weight is None else x * weight
+            return y if bias is None else y + bias
+        return _GroupNormAct.apply(x, weight, bias, seg, groups, _ACTS[act], eps, bool(keep8))

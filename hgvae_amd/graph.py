@@ -7,9 +7,11 @@ later layer, both encode passes and the backward pass reuse it.
 """
 from __future__ import annotations
 
+import bisect
 import weakref
-from typing import Optional
+from typing import Optional, Sequence
 
+import numpy as np
 import torch
 
 from . import _lib
@@ -246,3 +248,123 @@ def graph_of(edge_index, num_nodes: Optional[int] = None) -> Graph:
     ref = weakref.ref(edge_index, lambda _r, k=key: _cache.pop(k, None))
     _cache[key] = (ref, edge_index._version, num_nodes, g)
     return g
+
+
+class Segments:
+    """Which rows of a batched matrix belong to which graph: the plan that the per-graph operators
+    (:func:`~hgvae_amd.functional.group_norm_act`, :func:`~hgvae_amd.functional.graph_attention`) take.
+
+    Rows of a graph are consecutive and graphs follow one another, as ``Batch.from_data_list`` lays them out; a graph may
+    have no rows.  Building one uploads a few arrays (and, from a device tensor, reads the sizes back: one host
+    synchronisation); a plan serves every call, stream and captured graph afterwards, so a loop keeps it next to its batch.
+    """
+    MAX_ROWS = 2 ** 31 - 1
+
+    def __init__(self, sizes: Sequence[int], device):
+        sizes = np.asarray(list(sizes) if not isinstance(sizes, np.ndarray) else sizes)
+        if sizes.ndim != 1 or (sizes.size and sizes.dtype.kind not in "iu"):
+            raise _lib.HgvError("Segments: sizes must be a sequence of integers")
+        sizes = sizes.astype(np.int64)
+        if sizes.size and (int(sizes.min()) < 0 or int(sizes.max()) > self.MAX_ROWS or int(sizes.sum()) > self.MAX_ROWS):
+            raise _lib.HgvError("Segments: sizes must be >= 0 and sum to less than 2^31 rows")
+        self.device = torch.device(device)
+        if self.device.type != "cuda":
+            raise _lib.HgvError("hgvae_amd operators run on the GPU only (Segments needs a cuda device)")
+        if self.device.index is None:
+            self.device = torch.device("cuda", torch.cuda.current_device())
+        self.sizes = [int(s) for s in sizes]
+        self.num_graphs, self.num_rows = len(self.sizes), int(sizes.sum())
+        ptr = np.zeros(self.num_graphs + 1, dtype=np.int64)
+        np.cumsum(sizes, out=ptr[1:])
+        # graphs that have rows, smallest first (stable): operators split this list at a size of their own
+        order = np.argsort(sizes, kind="stable")
+        order = order[int((sizes == 0).sum()):]
+        self._sorted = sizes[order].tolist()
+        # row chunks of the sum / apply passes: about 2 048 of them in all, 32 to 512 rows each, at most 512 per graph
+        rows = min(max(-(-self.num_rows // 2048), 32), 512)
+        per = np.maximum(rows, -(-sizes[order] // 512))
+        counts = -(-sizes[order] // per)
+        self._first_chunk = np.zeros(order.size + 1, dtype=np.int64)
+        np.cumsum(counts, out=self._first_chunk[1:])
+        total = int(self._first_chunk[-1])
+        which = np.repeat(np.arange(order.size), counts)
+        start = ptr[order][which] + (np.arange(total) - self._first_chunk[which]) * per[which]
+        chunks = np.zeros((total, 4), dtype=np.int64)
+        chunks[:, 0], chunks[:, 1] = order[which], start
+        chunks[:, 2] = np.minimum(start + per[which], ptr[order + 1][which])
+        parts = [chunks.ravel(), ptr, order, self._first_chunk]
+        host = np.concatenate(parts).astype(np.int32)
+        self._buf = torch.from_numpy(host).to(self.device)          # copied before the call returns: any stream may read it
+        at = np.cumsum([0] + [p.size for p in parts])
+        self._chunks, self._ptr, self._order, self._first = (self._buf[at[i]:at[i + 1]] for i in range(4))
+        self._norm_plans: "dict[tuple, tuple]" = {}
+
+    @classmethod
+    def from_sizes(cls, sizes: Sequence[int], device="cuda") -> "Segments":
+        """From the number of rows of each graph, in order."""
+        return cls(sizes, device)
+
+    @classmethod
+    def from_ptr(cls, ptr: torch.Tensor, device=None) -> "Segments":
+        """From the first row of each graph and the end (``Batch.ptr``)."""
+        if ptr.dim() != 1 or ptr.numel() < 1 or ptr.dtype not in (torch.int32, torch.int64):
+            raise _lib.HgvError("Segments: ptr must be a 1-D integer tensor with at least one entry")
+        host = ptr.detach().cpu().numpy().astype(np.int64)
+        if host[0] != 0:
+            raise _lib.HgvError("Segments: ptr must start at 0")
+        return cls(np.diff(host), ptr.device if device is None else device)
+
+    @classmethod
+    def from_batch(cls, batch: torch.Tensor, num_graphs: Optional[int] = None) -> "Segments":
+        """From the graph number of each row (``Batch.batch``), which must not decrease."""
+        if batch.dim() != 1 or batch.dtype not in (torch.int32, torch.int64):
+            raise _lib.HgvError("Segments: batch must be a 1-D integer tensor")
+        host = batch.detach().cpu().numpy().astype(np.int64)
+        if host.size and (host[0] < 0 or (np.diff(host) < 0).any()):
+            raise _lib.HgvError("Segments: the rows of a graph must be consecutive and graphs in order")
+        count = int(host[-1]) + 1 if host.size else 0
+        if num_graphs is not None:
+            if int(num_graphs) < count:
+                raise _lib.HgvError(f"Segments: batch names graph {count - 1} of {num_graphs}")
+            count = int(num_graphs)
+        return cls(np.bincount(host, minlength=count) if host.size else np.zeros(count, dtype=np.int64), batch.device)
+
+    def _norm_plan(self, small_rows: int, row_bytes: int):
+        """(graphs that one workgroup reads at once, rows of the largest of them, batches of the others as a host array of
+        (first graph, first chunk) pairs, their number, chunks of the largest batch).  A batch is what the memory-side
+        cache holds between the two passes over it."""
+        key = (small_rows, row_bytes)
+        plan = self._norm_plans.get(key)
+        if plan is None:
+            n_small = bisect.bisect_right(self._sorted, small_rows)
+            limit, cur, marks, most = 96 << 20, 0, [], 0
+            for k in range(n_small, len(self._sorted)):
+                size = self._sorted[k] * row_bytes
+                if not marks or cur + size > limit:
+                    marks.append(k)
+                    cur = 0
+                cur += size
+            marks.append(len(self._sorted))
+            pairs = []
+            for i, k in enumerate(marks):
+                pairs += [k, int(self._first_chunk[k])]
+                if i:
+                    most = max(most, pairs[-1] - pairs[-3])
+            import ctypes
+            plan = (n_small, self._sorted[n_small - 1] if n_small else 0, (ctypes.c_int64 * len(pairs))(*pairs), len(marks) - 1, most)
+            self._norm_plans[key] = plan
+        return plan
+
+    def __repr__(self):
+        return f"Segments({self.num_graphs} graphs, {self.num_rows} rows, {self.device})"
+
+
+def segments_of(segments, num_rows: int) -> Segments:
+    """A :class:`Segments`, or one built for this call from a ``batch`` vector (one host synchronisation)."""
+    if not isinstance(segments, Segments):
+        if not isinstance(segments, torch.Tensor):
+            raise _lib.HgvError("expected Segments or a batch vector")
+        segments = Segments.from_batch(segments)
+    if segments.num_rows != num_rows:
+        raise _lib.HgvError(f"the matrix has {num_rows} rows but the graphs have {segments.num_rows}")
+    return segments

@@ -564,6 +564,38 @@ size_t hgv_grad_norm_ws(void);
 int hgv_grad_norm_clip(const float* g, int64_t n, float max_norm, float* norm_out, float* scale_out, void* ws,
                        size_t ws_bytes, hgv_stream_t stream);
 
+/* ---- activation checkpoints in 8 bits (no reference counterpart: autograd there keeps the fp32 input of every layer,
+ *      gvae/gvae_skipcon.py:105-118) ----------------------------------------------------------------------------------
+ * A block is 32 columns of one row (the last one of a row may be narrower).  With amax its largest magnitude:
+ *   e = floor(log2 amax) - 6, plus 1 where amax >= 127.5 * 2^e, held in [-126, 121];   q = rne(x * 2^-e) cut to +-127;   value = q * 2^e
+ * q [N, ldq] int8, ldq a multiple of 16 in [C, 32 * ceil(C/32)], 16-byte aligned, bytes behind column C zero;
+ * scale [N, ceil(C/32)] uint8 = e + 127, or 255 for a block that holds an infinity or NaN (it reads back as NaN). */
+int hgv_pack8(const float* x, int64_t ldx, int64_t N, int C, int8_t* q, int64_t ldq, uint8_t* scale, hgv_stream_t stream);
+int hgv_unpack8(const int8_t* q, int64_t ldq, const uint8_t* scale, int64_t N, int C, float* out, int64_t ldo, hgv_stream_t stream);
+
+/* ---- group norm with an activation over the rows of each graph, channels last (no reference counterpart: its levels
+ *      normalise over the whole batch, nn.BatchNorm1d at gvae/gvae_skipcon.py:63) --------------------------------------
+ * For graph b and group j of C / groups columns: mean, biased variance over rows x columns, rstd = 1 / sqrt(var + eps);
+ *   out = act((x - mean) * rstd * w + b),  act: 0 none, 1 relu, 2 x * sigmoid(x), 3 gelu (erf).   w, b [C] may be NULL (1, 0).
+ * Graphs: ptr [num_graphs + 1] first rows; order [listed] the graphs that have rows, by size; chunks [*][4] (graph, row, end
+ * row, unused) of the listed graphs in that order; first_chunk [listed + 1].  The first n_small graphs of the list (none
+ * above small_rows <= hgv_group_norm_small_rows(C, groups) rows) are read once; the others are taken in n_batches batches:
+ * batches (a HOST array) holds n_batches + 1 pairs (graph of the list, its first chunk), none with more than batch_chunks chunks.
+ * mean [num_graphs, groups] fp64 and rstd [num_graphs, groups] are written by the forward and read by the backward pass
+ * (entries of graphs without rows are left as they were).
+ * Backward: from x, or (q != NULL) from its 8-bit form; gx, gw [C], gb [C] are written where not NULL. */
+int hgv_group_norm_small_rows(int C, int groups);
+size_t hgv_group_norm_ws(int64_t batch_chunks, int num_graphs, int listed, int n_small, int C, int groups, int backward);
+int hgv_group_norm_fwd(const float* x, int64_t ldx, int C, int groups, int act, float eps, const float* w, const float* b,
+                       const int32_t* ptr, const int32_t* order, const int32_t* chunks, const int32_t* first_chunk, int num_graphs,
+                       int listed, int n_small, int small_rows, int n_batches, const int64_t* batches, int64_t batch_chunks, float* out,
+                       int64_t ldo, double* mean, float* rstd, void* ws, size_t ws_bytes, hgv_stream_t stream);
+int hgv_group_norm_bwd(const float* g, int64_t ldg, const float* x, int64_t ldx, const int8_t* q, int64_t ldq, const uint8_t* scale,
+                       int C, int groups, int act, const float* w, const float* b, const int32_t* ptr, const int32_t* order,
+                       const int32_t* chunks, const int32_t* first_chunk, int num_graphs, int listed, int n_small, int small_rows,
+                       int n_batches, const int64_t* batches, int64_t batch_chunks, const double* mean, const float* rstd, float* gx,
+                       int64_t ldgx, float* gw, float* gb, void* ws, size_t ws_bytes, hgv_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
