@@ -1,0 +1,709 @@
+// Attention among the nodes of each graph: softmax(scale * q k^T) v, forward and backward.
+//
+// Rows of a graph are consecutive; head h of q reads head h / (H / Hk) of k and v.  Arithmetic: fp32 results from the fp16 matrix
+// cores.  Every operand is multiplied by a power of two per (graph, key head) that brings its longest row to a norm below 2^15,
+// and split into two fp16 pieces (22 significant bits, an absolute floor 2^-39 below the largest row); a product is the three
+// piece products hi*hi + hi*lo + lo*hi with fp32 accumulation.  Probabilities are formed in fp32 and split the same way after a
+// multiplication by 2^8 ... 2^15, the gradient of the logits after one that the norms bound (|dP_ij| <= |do_i| |v_j|).
+//
+// Forward: one pass over the keys with the running maximum and sum of the softmax.  The logits are formed transposed
+// (S^T = K Q^T), so a lane owns one query: the maximum and the sum are a lane's own business up to two exchanges, and the
+// probabilities leave the product in the layout in which the next one (O^T = V^T P^T) takes them; V comes from LDS through the
+// transposing loads.  Kept for the backward pass: the output and one number per row and head (lse, base 2; +inf for a row without
+// keys).  Backward: probabilities are recomputed, once by key tiles (dk, dv) and once by query tiles (dq): no atomics, the same
+// bits every time.  A masked key's rows of k and v are taken as zeros, whatever they hold.
+#include "common.h"
+
+namespace {
+
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int TQ = 0, TK = 1, TV = 2, TG = 3;                   // tensors: q, k, v, gradient of the output
+constexpr int NO_EXP = -(1 << 20);                              // "no finite non-zero row"
+
+struct AtArgs {
+    const float* src[4]; int64_t row_stride[4], head_stride[4];     // q, k, v, do
+    int64_t N; int H, Hk, R, D;
+    float scale;
+    const uint8_t* mask;                                        // [N] keys that take part, or null
+    const int32_t* ptr;
+    const int4* tiles;                                          // prepass tiles of 64 rows: (graph, row, first tile, tiles of the graph)
+    int n_tiles;
+    const int4* blocks;                                         // tiles of 128 rows: (graph, row, -, -), largest graphs first
+    int n_blocks;
+    int* part;                                                  // [tile][4][Hk] exponents of the longest row
+    int* exps;                                                  // [B][Hk][4]
+    _Float16* img[4];                                           // [heads][N][hi DP | lo DP]
+    float* out;                                                 // [N, H, D]
+    float* lse;                                                 // [H, N]
+    float* delta;                                               // [H, N] sum_d do * o, scaled (backward)
+    float* dq; float* dk; float* dv;                            // [N, H or Hk, D]
+};
+
+// ---- operands into scaled fp16 pieces ------------------------------------------------------------------------------------
+// Sixteen lanes take one (row, head) vector.  First pass: the exponent e with |row| < 2^e, its maximum over the tile per key head.
+__global__ __launch_bounds__(256) void k_at_norms(const AtArgs a) {
+    __shared__ int best[256];
+    const int ten = blockIdx.y;
+    const int4 tile = a.tiles[blockIdx.x];
+    const int rows = min(64, (int)(a.ptr[tile.x + 1] - tile.y));
+    const int heads = (ten == TQ || ten == TG) ? a.H : a.Hk, per = heads / a.Hk;
+    for (int h0 = 0; h0 < a.Hk; h0 += 256) {                    // key heads in slabs of 256
+        const int hk_n = min(256, a.Hk - h0);
+        for (int i = threadIdx.x; i < hk_n; i += 256) best[i] = NO_EXP;
+        __syncthreads();
+        const int sub = threadIdx.x & 15;
+        for (int v = threadIdx.x >> 4; v < rows * hk_n * per; v += 16) {
+            const int r = v / (hk_n * per), h = h0 * per + v - r * hk_n * per;
+            const int64_t n = tile.y + r;
+            if (a.mask && (ten == TK || ten == TV) && !a.mask[n]) continue;
+            const float* p = a.src[ten] + n * a.row_stride[ten] + h * a.head_stride[ten];
+            double s = 0.0;
+            for (int d = sub; d < a.D; d += 16) s = fma((double)p[d], (double)p[d], s);
+#pragma unroll
+            for (int o = 1; o < 16; o <<= 1) s += __shfl_xor(s, o, 64);
+            if (sub == 0 && s > 0.0 && s < 1e300) {             // rows that hold an infinity or NaN do not count
+                const int e2 = (int)((__double_as_longlong(s) >> 52) & 2047) - 1023;
+                atomicMax(&best[h / per - h0], (e2 >> 1) + 1);
+            }
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < hk_n; i += 256) a.part[((int64_t)blockIdx.x * 4 + ten) * a.Hk + h0 + i] = best[i];
+        __syncthreads();
+    }
+}
+
+// Second pass: one workgroup per (tile, tensor, key head).
+template <int DP>
+__global__ __launch_bounds__(256) void k_at_split(const AtArgs a) {
+    constexpr int E = DP / 16;
+    __shared__ int se[2];
+    const int ten = blockIdx.y, hk = blockIdx.z;
+    const int4 tile = a.tiles[blockIdx.x];
+    if (threadIdx.x < 64) {
+        int e = NO_EXP, ev = NO_EXP;
+        for (int i = threadIdx.x; i < tile.w; i += 64) {
+            e = max(e, a.part[((int64_t)(tile.z + i) * 4 + ten) * a.Hk + hk]);
+            if (ten == TG) ev = max(ev, a.part[((int64_t)(tile.z + i) * 4 + TV) * a.Hk + hk]);
+        }
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) {
+            e = max(e, __shfl_xor(e, o, 64));
+            ev = max(ev, __shfl_xor(ev, o, 64));
+        }
+        if (threadIdx.x == 0) {
+            se[0] = e == NO_EXP ? 0 : e;
+            se[1] = ev == NO_EXP ? 0 : ev;
+        }
+    }
+    __syncthreads();
+    const int e = se[0], ev = se[1];
+    if (threadIdx.x == 0 && (int)blockIdx.x == tile.z) a.exps[((int64_t)tile.x * a.Hk + hk) * 4 + ten] = e;
+    const int rows = min(64, (int)(a.ptr[tile.x + 1] - tile.y));
+    const int per = (ten == TQ || ten == TG) ? a.R : 1, sub = threadIdx.x & 15;
+    for (int v = threadIdx.x >> 4; v < rows * per; v += 16) {
+        const int r = v / per, h = hk * per + v - r * per;
+        const int64_t n = tile.y + r;
+        const bool live = !(a.mask && (ten == TK || ten == TV) && !a.mask[n]);
+        const float* p = a.src[ten] + n * a.row_stride[ten] + h * a.head_stride[ten];
+        const float* o = ten == TG ? a.out + (n * a.H + h) * a.D : nullptr;
+        _Float16 hi[E], lo[E];
+        float dot = 0.f;
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            const int d = sub * E + i;
+            const float x = live && d < a.D ? p[d] : 0.f;
+            const float y = ldexpf(x, 15 - e);
+            if (ten == TG && d < a.D) dot = fmaf(y, o[d], dot);
+            hi[i] = (_Float16)y;
+            lo[i] = (_Float16)(y - (float)hi[i]);
+        }
+        _Float16* dst = a.img[ten] + ((int64_t)h * a.N + n) * (2 * DP) + sub * E;
+#pragma unroll
+        for (int i = 0; i < E; i += 2) {
+            *(f16x2*)(dst + i) = f16x2{hi[i], hi[i + 1]};
+            *(f16x2*)(dst + DP + i) = f16x2{lo[i], lo[i + 1]};
+        }
+        if (ten == TG) {
+#pragma unroll
+            for (int w = 1; w < 16; w <<= 1) dot += __shfl_xor(dot, w, 64);
+            if (sub == 0) a.delta[(int64_t)h * a.N + n] = ldexpf(dot, -16 - ev);
+        }
+    }
+}
+
+// ---- pieces shared by the three products -----------------------------------------------------------------------------------
+// LDS tile of 64 rows: row = [hi DP | lo DP] fp16 + 16 bytes, which puts the same 16-byte chunk of 16 consecutive rows into all
+// 64 banks.
+template <int DP> constexpr int row_bytes() { return 4 * DP + 16; }
+
+template <int DP>
+struct Stage {                                                  // a thread's share of a 64-row tile on its way to LDS
+    static constexpr int CH = DP / 16;                          // 16-byte chunks per thread
+    uint4 v[CH];
+    __device__ __forceinline__ void load(const _Float16* tile, int rows) {          // tile: first row in the image
+        const uint4* p = (const uint4*)tile;
+#pragma unroll
+        for (int i = 0; i < CH; ++i) {
+            const int f = threadIdx.x + 256 * i, r = f / (DP / 4);
+            v[i] = r < rows ? p[f] : make_uint4(0, 0, 0, 0);
+        }
+    }
+    __device__ __forceinline__ void store(unsigned char* lds) const {
+#pragma unroll
+        for (int i = 0; i < CH; ++i) {
+            const int f = threadIdx.x + 256 * i, r = f / (DP / 4), c = f - r * (DP / 4);
+            *(uint4*)(lds + r * row_bytes<DP>() + c * 16) = v[i];
+        }
+    }
+};
+
+struct Frag { f16x8 hi, lo; };
+
+// rows r0 + (lane & 15), columns 32 c + 8 (lane >> 4) ..: a row-operand fragment
+template <int DP>
+__device__ __forceinline__ Frag row_frag(const unsigned char* lds, int r0, int c, int lane) {
+    const unsigned char* p = lds + (r0 + (lane & 15)) * row_bytes<DP>() + c * 64 + (lane >> 4) * 16;
+    Frag f;
+    f.hi = *(const f16x8*)p;
+    f.lo = *(const f16x8*)(p + 2 * DP);
+    return f;
+}
+
+__device__ __forceinline__ f16x8 tr_read(const unsigned char* p, int next) {
+    typedef __attribute__((address_space(3))) s16x4 lds_v;
+    union { struct { s16x4 a, b; } s; f16x8 v; } u;
+    u.s.a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v*)p);
+    u.s.b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v*)(p + next));
+    return u.v;
+}
+// the transposed tile: fragment row d = 16 db + (lane & 15); its eight values are tile rows r0 + 4g + 0..3 and r0 + 16 + 4g + 0..3
+// (g = lane >> 4), the order in which split_frag lays out a product's rows
+template <int DP>
+__device__ __forceinline__ Frag col_frag(const unsigned char* lds, int r0, int db, int lane) {
+    const int g = lane >> 4, i = lane & 15;
+    const unsigned char* p = lds + (r0 + 4 * g + (i >> 2)) * row_bytes<DP>() + db * 32 + (i & 3) * 8;
+    Frag f;
+    f.hi = tr_read(p, 16 * row_bytes<DP>());
+    f.lo = tr_read(p + 2 * DP, 16 * row_bytes<DP>());
+    return f;
+}
+
+__device__ __forceinline__ Frag split_frag(const f32x4& x, const f32x4& y) {
+    Frag f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        f.hi[i] = (_Float16)x[i];
+        f.lo[i] = (_Float16)(x[i] - (float)f.hi[i]);
+        f.hi[4 + i] = (_Float16)y[i];
+        f.lo[4 + i] = (_Float16)(y[i] - (float)f.hi[4 + i]);
+    }
+    return f;
+}
+
+__device__ __forceinline__ f32x4 mma3(const Frag& a, const Frag& b, f32x4 c) {
+    c = __builtin_amdgcn_mfma_f32_16x16x32_f16(a.hi, b.lo, c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_16x16x32_f16(a.lo, b.hi, c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a.hi, b.hi, c, 0, 0, 0);
+}
+
+// fragment of a wave's own rows, straight from the image: column operand, column = row n + (lane & 15)
+template <int DP>
+__device__ __forceinline__ Frag own_frag(const _Float16* img, int64_t row, int c, int lane) {
+    const _Float16* p = img + row * (2 * DP) + c * 32 + (lane >> 4) * 8;
+    Frag f;
+    f.hi = *(const f16x8*)p;
+    f.lo = *(const f16x8*)(p + DP);
+    return f;
+}
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+__device__ __forceinline__ float fold_scale(float scale, int e) {           // scale * log2(e) * 2^e
+    // never zero: a zero would turn a masked logit (-inf) into NaN, and products this small are zeros either way
+    return fmaxf((float)ldexp((double)scale * 1.4426950408889634, e), 1.2e-38f);
+}
+
+__device__ __forceinline__ float* row_out(float* base, int64_t n, int heads, int h, int D) { return base + (n * heads + h) * D; }
+
+// four consecutive columns d .. d + 3 of an output row
+__device__ __forceinline__ void store4(float* p, int d, int D, f32x4 v) {
+    if (d + 3 < D && (D & 3) == 0) *(f32x4*)(p + d) = v;
+    else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (d + i < D) p[d + i] = v[i];
+    }
+}
+
+constexpr float P_BITS = 8.f;                                   // probabilities start at 2^8 and may grow to 2^15 before a rescale
+constexpr float P_GROW = 7.f;
+
+// ---- forward -----------------------------------------------------------------------------------------------------------------
+// A workgroup owns 128 queries of one head (a wave 32), walks the keys of the graph in tiles of 64.
+template <int DP>
+__global__ __launch_bounds__(256) void k_at_fwd(const AtArgs a) {
+    constexpr int KC = DP / 32, DB = DP / 16;
+    __shared__ __align__(16) unsigned char ldsK[64 * row_bytes<DP>()];
+    __shared__ __align__(16) unsigned char ldsV[64 * row_bytes<DP>()];
+    __shared__ __align__(16) float bias[64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
+    const int blk = blockIdx.x / a.H, h = blockIdx.x - blk * a.H, hk = h / a.R;
+    const int4 t = a.blocks[blk];
+    const int64_t k0 = a.ptr[t.x], k1 = a.ptr[t.x + 1];
+    const int64_t q0 = (int64_t)t.y + 32 * wave;
+    const int* ex = a.exps + ((int64_t)t.x * a.Hk + hk) * 4;
+    const float c = fold_scale(a.scale, ex[TQ] + ex[TK] - 30);
+    Frag q[2][KC];
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int k = 0; k < KC; ++k) q[b][k] = own_frag<DP>(a.img[TQ] + (int64_t)h * a.N * (2 * DP), min(q0 + 16 * b + (lane & 15), k1 - 1), k, lane);
+    f32x4 acc[DB][2];
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};     // m: the exponent that is subtracted, base 2
+#pragma unroll
+    for (int d = 0; d < DB; ++d) acc[d][0] = acc[d][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const _Float16* ki = a.img[TK] + ((int64_t)hk * a.N + k0) * (2 * DP);
+    const _Float16* vi = a.img[TV] + ((int64_t)hk * a.N + k0) * (2 * DP);
+    const int n = (int)(k1 - k0);
+    Stage<DP> sk, sv;
+    sk.load(ki, min(64, n));
+    sv.load(vi, min(64, n));
+    float nb = threadIdx.x < 64 && (int)threadIdx.x < n && (!a.mask || a.mask[k0 + threadIdx.x]) ? 0.f : -INFINITY;
+    for (int kt = 0; kt < n; kt += 64) {
+        __syncthreads();
+        sk.store(ldsK);
+        sv.store(ldsV);
+        if (threadIdx.x < 64) bias[threadIdx.x] = nb;
+        __syncthreads();
+        const int next = kt + 64;
+        if (next < n) {
+            sk.load(ki + (int64_t)next * (2 * DP), min(64, n - next));
+            sv.load(vi + (int64_t)next * (2 * DP), min(64, n - next));
+            const int j = next + (int)threadIdx.x;
+            nb = threadIdx.x < 64 && j < n && (!a.mask || a.mask[k0 + j]) ? 0.f : -INFINITY;
+        }
+        const bool biased = a.mask != nullptr || kt + 64 > n;
+        f32x4 s[4][2];
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            s[b][0] = s[b][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int k = 0; k < KC; ++k) {
+                const Frag f = row_frag<DP>(ldsK, 16 * b, k, lane);
+                s[b][0] = mma3(f, q[0][k], s[b][0]);
+                s[b][1] = mma3(f, q[1][k], s[b][1]);
+            }
+            if (biased) {
+                const f32x4 o = *(const f32x4*)(bias + 16 * b + 4 * g);
+                s[b][0] += o;
+                s[b][1] += o;
+            }
+        }
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            float top = fmaxf(fmaxf(s[0][b][0], s[0][b][1]), fmaxf(s[0][b][2], s[0][b][3]));
+#pragma unroll
+            for (int i = 1; i < 4; ++i) top = fmaxf(top, fmaxf(fmaxf(s[i][b][0], s[i][b][1]), fmaxf(s[i][b][2], s[i][b][3])));
+            top = fmaxf(top, __shfl_xor(top, 16, 64));
+            top = fmaxf(top, __shfl_xor(top, 32, 64)) * c;
+            // rescale only when a probability would leave its range
+            if (__any(top > m[b] + P_GROW || (m[b] == -INFINITY && top > -INFINITY))) {
+                const float mn = fmaxf(m[b], top);
+                const float f = m[b] == -INFINITY ? 0.f : exp2_fast(m[b] - mn);
+                m[b] = mn;
+                l[b] *= f;
+#pragma unroll
+                for (int d = 0; d < DB; ++d) acc[d][b] *= f;
+            }
+            const float off = m[b] == -INFINITY ? 0.f : P_BITS - m[b];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float p = exp2_fast(fmaf(s[i][b][j], c, off));
+                    s[i][b][j] = p;
+                    l[b] += p;
+                }
+        }
+#pragma unroll
+        for (int kc = 0; kc < 2; ++kc) {
+            const Frag p0 = split_frag(s[2 * kc][0], s[2 * kc + 1][0]), p1 = split_frag(s[2 * kc][1], s[2 * kc + 1][1]);
+#pragma unroll
+            for (int d = 0; d < DB; ++d) {
+                const Frag f = col_frag<DP>(ldsV, 32 * kc, d, lane);
+                acc[d][0] = mma3(f, p0, acc[d][0]);
+                acc[d][1] = mma3(f, p1, acc[d][1]);
+            }
+        }
+    }
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+        l[b] += __shfl_xor(l[b], 16, 64);
+        l[b] += __shfl_xor(l[b], 32, 64);
+        const int64_t row = q0 + 16 * b + (lane & 15);
+        if (row >= k1) continue;
+        const bool none = l[b] == 0.f;
+        const float f = none ? 0.f : ldexpf(1.f / l[b], ex[TV] - 15);
+        float* o = row_out(a.out, row, a.H, h, a.D);
+#pragma unroll
+        for (int d = 0; d < DB; ++d) store4(o, 16 * d + 4 * g, a.D, none ? f32x4{0.f, 0.f, 0.f, 0.f} : acc[d][b] * f);
+        if (g == 0 && a.lse) a.lse[(int64_t)h * a.N + row] = none ? INFINITY : m[b] - P_BITS + log2f(l[b]);
+    }
+}
+
+// ---- backward: dk and dv ---------------------------------------------------------------------------------------------------
+// A workgroup owns 64 * KB keys of one key head (a wave 16 * KB), walks the queries of the graph, head by head, in tiles of 64 rows.
+template <int DP, int KB>
+__global__ __launch_bounds__(256) void k_at_dkv(const AtArgs a) {
+    constexpr int KC = DP / 32, DB = DP / 16;
+    __shared__ __align__(16) unsigned char ldsQ[64 * row_bytes<DP>()];
+    __shared__ __align__(16) unsigned char ldsG[64 * row_bytes<DP>()];
+    __shared__ __align__(16) float ldsL[64];
+    __shared__ __align__(16) float ldsD[64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
+    constexpr int SPLIT = 2 / KB;                               // workgroups per 128-row block
+    const int unit = blockIdx.x / a.Hk, hk = blockIdx.x - unit * a.Hk;
+    const int4 t = a.blocks[unit / SPLIT];
+    const int64_t g0 = a.ptr[t.x], g1 = a.ptr[t.x + 1];
+    const int64_t first = (int64_t)t.y + (unit % SPLIT) * 64;
+    if (first >= g1) return;
+    const int64_t key0 = first + 16 * KB * wave;
+    const int* ex = a.exps + ((int64_t)t.x * a.Hk + hk) * 4;
+    const float c = fold_scale(a.scale, ex[TQ] + ex[TK] - 30);
+    Frag kf[KB][KC], vf[KB][KC];
+#pragma unroll
+    for (int b = 0; b < KB; ++b)
+#pragma unroll
+        for (int k = 0; k < KC; ++k) {
+            const int64_t row = min(key0 + 16 * b + (lane & 15), g1 - 1);
+            kf[b][k] = own_frag<DP>(a.img[TK] + (int64_t)hk * a.N * (2 * DP), row, k, lane);
+            vf[b][k] = own_frag<DP>(a.img[TV] + (int64_t)hk * a.N * (2 * DP), row, k, lane);
+        }
+    f32x4 dk[DB][KB], dv[DB][KB];
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int b = 0; b < KB; ++b) dk[d][b] = dv[d][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const int n = (int)(g1 - g0), tiles = (n + 63) / 64, steps = tiles * a.R;
+    Stage<DP> sq, sg;
+    float nl = INFINITY, nd = 0.f;
+    auto fetch = [&](int step) __attribute__((always_inline)) {
+        const int hh = hk * a.R + step / tiles, r0 = (step % tiles) * 64, rows = min(64, n - r0);
+        const int64_t at = (int64_t)hh * a.N + g0 + r0;
+        sq.load(a.img[TQ] + at * (2 * DP), rows);
+        sg.load(a.img[TG] + at * (2 * DP), rows);
+        nl = INFINITY; nd = 0.f;
+        if ((int)threadIdx.x < rows) {
+            nl = a.lse[at + threadIdx.x];
+            nd = a.delta[at + threadIdx.x];
+        }
+    };
+    fetch(0);
+    for (int step = 0; step < steps; ++step) {
+        __syncthreads();
+        sq.store(ldsQ);
+        sg.store(ldsG);
+        if (threadIdx.x < 64) {
+            ldsL[threadIdx.x] = 15.f - nl;
+            ldsD[threadIdx.x] = nd;
+        }
+        __syncthreads();
+        if (step + 1 < steps) fetch(step + 1);
+#pragma unroll
+        for (int qc = 0; qc < 2; ++qc) {                        // 32 queries at a time
+            Frag pf[KB], df[KB];
+            {
+                f32x4 p[2][KB], s[2][KB];
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                    const int r0 = 32 * qc + 16 * b;
+#pragma unroll
+                    for (int j = 0; j < KB; ++j) p[b][j] = s[b][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int k = 0; k < KC; ++k) {
+                        const Frag f = row_frag<DP>(ldsQ, r0, k, lane);
+#pragma unroll
+                        for (int j = 0; j < KB; ++j) p[b][j] = mma3(f, kf[j][k], p[b][j]);
+                    }
+#pragma unroll
+                    for (int k = 0; k < KC; ++k) {
+                        const Frag f = row_frag<DP>(ldsG, r0, k, lane);
+#pragma unroll
+                        for (int j = 0; j < KB; ++j) s[b][j] = mma3(f, vf[j][k], s[b][j]);
+                    }
+                    const f32x4 ls = *(const f32x4*)(ldsL + r0 + 4 * g), de = *(const f32x4*)(ldsD + r0 + 4 * g);
+#pragma unroll
+                    for (int j = 0; j < KB; ++j)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            p[b][j][i] = exp2_fast(fmaf(p[b][j][i], c, ls[i]));
+                            s[b][j][i] = p[b][j][i] * fmaf(s[b][j][i], 0x1p-31f, -de[i]);
+                        }
+                }
+#pragma unroll
+                for (int j = 0; j < KB; ++j) {
+                    pf[j] = split_frag(p[0][j], p[1][j]);
+                    df[j] = split_frag(s[0][j], s[1][j]);
+                }
+            }
+#pragma unroll
+            for (int d = 0; d < DB; ++d) {
+                const Frag f = col_frag<DP>(ldsG, 32 * qc, d, lane);
+#pragma unroll
+                for (int j = 0; j < KB; ++j) dv[d][j] = mma3(f, pf[j], dv[d][j]);
+            }
+#pragma unroll
+            for (int d = 0; d < DB; ++d) {
+                const Frag f = col_frag<DP>(ldsQ, 32 * qc, d, lane);
+#pragma unroll
+                for (int j = 0; j < KB; ++j) dk[d][j] = mma3(f, df[j], dk[d][j]);
+            }
+        }
+    }
+#pragma unroll
+    for (int b = 0; b < KB; ++b) {
+        const int64_t row = key0 + 16 * b + (lane & 15);
+        if (row >= g1) continue;
+        const bool live = !a.mask || a.mask[row];
+        float* pk = row_out(a.dk, row, a.Hk, hk, a.D);
+        float* pv = row_out(a.dv, row, a.Hk, hk, a.D);
+        const int ek = ex[TG] + ex[TV] + ex[TQ] - 29, ev = ex[TG] - 30;
+#pragma unroll
+        for (int d = 0; d < DB; ++d) {
+            f32x4 x, y;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                x[i] = live ? ldexpf(dk[d][b][i] * a.scale, ek) : 0.f;
+                y[i] = live ? ldexpf(dv[d][b][i], ev) : 0.f;
+            }
+            store4(pk, 16 * d + 4 * g, a.D, x);
+            store4(pv, 16 * d + 4 * g, a.D, y);
+        }
+    }
+}
+
+// ---- backward: dq -----------------------------------------------------------------------------------------------------------
+template <int DP, int QB>
+__global__ __launch_bounds__(256) void k_at_dq(const AtArgs a) {
+    constexpr int KC = DP / 32, DB = DP / 16;
+    __shared__ __align__(16) unsigned char ldsK[64 * row_bytes<DP>()];
+    __shared__ __align__(16) unsigned char ldsV[64 * row_bytes<DP>()];
+    __shared__ __align__(16) float bias[64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
+    constexpr int SPLIT = 2 / QB;
+    const int unit = blockIdx.x / a.H, h = blockIdx.x - unit * a.H, hk = h / a.R;
+    const int4 t = a.blocks[unit / SPLIT];
+    const int64_t k0 = a.ptr[t.x], k1 = a.ptr[t.x + 1];
+    const int64_t first = (int64_t)t.y + (unit % SPLIT) * 64;
+    if (first >= k1) return;
+    const int64_t q0 = first + 16 * QB * wave;
+    const int* ex = a.exps + ((int64_t)t.x * a.Hk + hk) * 4;
+    const float c = fold_scale(a.scale, ex[TQ] + ex[TK] - 30);
+    Frag q[QB][KC], go[QB][KC];
+    float ls[QB], de[QB];
+#pragma unroll
+    for (int b = 0; b < QB; ++b) {
+        const int64_t row = min(q0 + 16 * b + (lane & 15), k1 - 1);
+#pragma unroll
+        for (int k = 0; k < KC; ++k) {
+            q[b][k] = own_frag<DP>(a.img[TQ] + (int64_t)h * a.N * (2 * DP), row, k, lane);
+            go[b][k] = own_frag<DP>(a.img[TG] + (int64_t)h * a.N * (2 * DP), row, k, lane);
+        }
+        ls[b] = 15.f - a.lse[(int64_t)h * a.N + row];
+        de[b] = a.delta[(int64_t)h * a.N + row];
+    }
+    f32x4 acc[DB][QB];
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int b = 0; b < QB; ++b) acc[d][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const _Float16* ki = a.img[TK] + ((int64_t)hk * a.N + k0) * (2 * DP);
+    const _Float16* vi = a.img[TV] + ((int64_t)hk * a.N + k0) * (2 * DP);
+    const int n = (int)(k1 - k0);
+    Stage<DP> sk, sv;
+    sk.load(ki, min(64, n));
+    sv.load(vi, min(64, n));
+    float nb = threadIdx.x < 64 && (int)threadIdx.x < n && (!a.mask || a.mask[k0 + threadIdx.x]) ? 0.f : -INFINITY;
+    for (int kt = 0; kt < n; kt += 64) {
+        __syncthreads();
+        sk.store(ldsK);
+        sv.store(ldsV);
+        if (threadIdx.x < 64) bias[threadIdx.x] = nb;
+        __syncthreads();
+        const int next = kt + 64;
+        if (next < n) {
+            sk.load(ki + (int64_t)next * (2 * DP), min(64, n - next));
+            sv.load(vi + (int64_t)next * (2 * DP), min(64, n - next));
+            const int j = next + (int)threadIdx.x;
+            nb = threadIdx.x < 64 && j < n && (!a.mask || a.mask[k0 + j]) ? 0.f : -INFINITY;
+        }
+        const bool biased = a.mask != nullptr || kt + 64 > n;
+#pragma unroll
+        for (int kc = 0; kc < 2; ++kc) {
+            Frag df[QB];
+            {
+                f32x4 p[2][QB], s[2][QB];
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                    const int r0 = 32 * kc + 16 * b;
+#pragma unroll
+                    for (int j = 0; j < QB; ++j) p[b][j] = s[b][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int k = 0; k < KC; ++k) {
+                        const Frag f = row_frag<DP>(ldsK, r0, k, lane);
+#pragma unroll
+                        for (int j = 0; j < QB; ++j) p[b][j] = mma3(f, q[j][k], p[b][j]);
+                    }
+#pragma unroll
+                    for (int k = 0; k < KC; ++k) {
+                        const Frag f = row_frag<DP>(ldsV, r0, k, lane);
+#pragma unroll
+                        for (int j = 0; j < QB; ++j) s[b][j] = mma3(f, go[j][k], s[b][j]);
+                    }
+                    if (biased) {
+                        const f32x4 o = *(const f32x4*)(bias + r0 + 4 * g);
+#pragma unroll
+                        for (int j = 0; j < QB; ++j) p[b][j] += o;
+                    }
+#pragma unroll
+                    for (int j = 0; j < QB; ++j)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float e = exp2_fast(fmaf(p[b][j][i], c, ls[j]));
+                            s[b][j][i] = e * fmaf(s[b][j][i], 0x1p-31f, -de[j]);
+                        }
+                }
+#pragma unroll
+                for (int j = 0; j < QB; ++j) df[j] = split_frag(s[0][j], s[1][j]);
+            }
+#pragma unroll
+            for (int d = 0; d < DB; ++d) {
+                const Frag f = col_frag<DP>(ldsK, 32 * kc, d, lane);
+#pragma unroll
+                for (int j = 0; j < QB; ++j) acc[d][j] = mma3(f, df[j], acc[d][j]);
+            }
+        }
+    }
+#pragma unroll
+    for (int b = 0; b < QB; ++b) {
+        const int64_t row = q0 + 16 * b + (lane & 15);
+        if (row >= k1) continue;
+        float* o = row_out(a.dq, row, a.H, h, a.D);
+        const int e = ex[TG] + ex[TV] + ex[TK] - 29;
+#pragma unroll
+        for (int d = 0; d < DB; ++d) {
+            f32x4 x;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = ldexpf(acc[d][b][i] * a.scale, e);
+            store4(o, 16 * d + 4 * g, a.D, x);
+        }
+    }
+}
+
+// ---- host side ----------------------------------------------------------------------------------------------------------------
+int at_dp(int D) { return (D + 31) / 32 * 32; }
+
+struct AtSizes { size_t part, exps, img[4], delta, total; };
+AtSizes at_sizes(int64_t N, int H, int Hk, int D, int64_t n_tiles, int64_t graphs, bool backward) {
+    AtSizes s;
+    const size_t row = (size_t)at_dp(D) * 4;
+    s.part = hgv_align256((size_t)n_tiles * 4 * Hk * sizeof(int));
+    s.exps = hgv_align256((size_t)graphs * Hk * 4 * sizeof(int));
+    s.img[TQ] = hgv_align256((size_t)N * H * row);
+    s.img[TK] = s.img[TV] = hgv_align256((size_t)N * Hk * row);
+    s.img[TG] = backward ? s.img[TQ] : 0;
+    s.delta = backward ? hgv_align256((size_t)N * H * sizeof(float)) : 0;
+    s.total = s.part + s.exps + s.img[0] + s.img[1] + s.img[2] + s.img[3] + s.delta;
+    return s;
+}
+
+template <int DP>
+int at_launch(const AtArgs& a, bool backward, hipStream_t stream) {
+    const int tensors = backward ? 4 : 3;
+    hipLaunchKernelGGL(k_at_norms, dim3((unsigned)a.n_tiles, (unsigned)tensors), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL(k_at_split<DP>, dim3((unsigned)a.n_tiles, (unsigned)tensors, (unsigned)a.Hk), dim3(256), 0, stream, a);
+    if (!backward) {
+        hipLaunchKernelGGL(k_at_fwd<DP>, dim3((unsigned)((int64_t)a.n_blocks * a.H)), dim3(256), 0, stream, a);
+    } else {
+        // wide heads: 16 keys / queries per wave, so that the accumulators of 32 do not push the operands out of the registers
+        constexpr int KB = DP <= 64 ? 2 : 1;
+        if (a.dk) hipLaunchKernelGGL((k_at_dkv<DP, KB>), dim3((unsigned)((int64_t)a.n_blocks * a.Hk * (2 / KB))), dim3(256), 0, stream, a);
+        if (a.dq) hipLaunchKernelGGL((k_at_dq<DP, KB>), dim3((unsigned)((int64_t)a.n_blocks * a.H * (2 / KB))), dim3(256), 0, stream, a);
+    }
+    HGV_CHECK_LAUNCH(backward ? "graph_attention_bwd" : "graph_attention_fwd");
+    return HGV_OK;
+}
+
+int at_dispatch(const AtArgs& a, bool backward, hipStream_t stream) {
+    switch (at_dp(a.D)) {
+        case 32: return at_launch<32>(a, backward, stream);
+        case 64: return at_launch<64>(a, backward, stream);
+        case 96: return at_launch<96>(a, backward, stream);
+        default: return at_launch<128>(a, backward, stream);
+    }
+}
+
+int at_fill(AtArgs& a, const char* what, int64_t N, int num_graphs, int H, int Hk, int D, float scale, const uint8_t* mask, const int32_t* ptr,
+            const int32_t* tiles, int n_tiles, const int32_t* blocks, int n_blocks, void* ws, size_t ws_bytes, bool backward) {
+    HGV_REQUIRE(N > 0 && N <= 0x7fffffff && num_graphs > 0 && H > 0 && Hk > 0 && H % Hk == 0 && D > 0, HGV_EINVAL, "%s: bad sizes", what);
+    HGV_REQUIRE(D <= 128 && H <= 65535, HGV_EUNSUPPORTED, "%s: heads of %d columns (at most 128), %d of them", what, D, H);
+    HGV_REQUIRE(scale > 0.f && scale < INFINITY, HGV_EINVAL, "%s: the scale must be positive and finite", what);
+    HGV_REQUIRE(ptr && tiles && blocks && n_tiles > 0 && n_blocks > 0, HGV_EINVAL, "%s: null plan", what);
+    HGV_REQUIRE((int64_t)n_blocks * H * 2 <= 0x7fffffff, HGV_EUNSUPPORTED, "%s: too many tiles", what);
+    const AtSizes s = at_sizes(N, H, Hk, D, n_tiles, num_graphs, backward);
+    HGV_REQUIRE(ws && ws_bytes >= s.total && hgv_aligned(ws, 256), HGV_EWORKSPACE, "%s: workspace too small or misaligned", what);
+    a.N = N; a.H = H; a.Hk = Hk; a.R = H / Hk; a.D = D; a.scale = scale; a.mask = mask; a.ptr = ptr;
+    a.tiles = (const int4*)tiles; a.n_tiles = n_tiles; a.blocks = (const int4*)blocks; a.n_blocks = n_blocks;
+    char* p = (char*)ws;
+    a.part = (int*)p; p += s.part;
+    a.exps = (int*)p; p += s.exps;
+    for (int i = 0; i < 4; ++i) { a.img[i] = (_Float16*)p; p += s.img[i]; }
+    a.delta = (float*)p;
+    return HGV_OK;
+}
+
+}  // namespace
+
+extern "C" size_t hgv_graph_attention_ws(int64_t N, int num_graphs, int H, int Hk, int D, int64_t n_tiles, int backward) {
+    if (N <= 0 || num_graphs <= 0 || H <= 0 || Hk <= 0 || D <= 0 || n_tiles <= 0) return 0;
+    return at_sizes(N, H, Hk, D, n_tiles, num_graphs, backward != 0).total;
+}
+
+extern "C" int hgv_graph_attention_fwd(const float* q, int64_t q_row, int64_t q_head, const float* k, int64_t k_row, int64_t k_head,
+                                       const float* v, int64_t v_row, int64_t v_head, int64_t N, int num_graphs, int H, int Hk, int D,
+                                       float scale, const uint8_t* mask, const int32_t* ptr, const int32_t* tiles, int n_tiles,
+                                       const int32_t* blocks, int n_blocks, float* out, float* lse, void* ws, size_t ws_bytes,
+                                       hipStream_t stream) {
+    AtArgs a = {};
+    const int rc = at_fill(a, "graph_attention_fwd", N, num_graphs, H, Hk, D, scale, mask, ptr, tiles, n_tiles, blocks, n_blocks, ws, ws_bytes, false);
+    if (rc) return rc;
+    HGV_REQUIRE(q && k && v && out && (D % 4 || hgv_aligned(out, 16)), HGV_EINVAL, "graph_attention_fwd: null or misaligned buffer");
+    a.src[TQ] = q; a.row_stride[TQ] = q_row; a.head_stride[TQ] = q_head;
+    a.src[TK] = k; a.row_stride[TK] = k_row; a.head_stride[TK] = k_head;
+    a.src[TV] = v; a.row_stride[TV] = v_row; a.head_stride[TV] = v_head;
+    a.out = out; a.lse = lse;
+    return at_dispatch(a, false, stream);
+}
+
+extern "C" int hgv_graph_attention_bwd(const float* q, int64_t q_row, int64_t q_head, const float* k, int64_t k_row, int64_t k_head,
+                                       const float* v, int64_t v_row, int64_t v_head, const float* g, int64_t g_row, int64_t g_head,
+                                       const float* out, const float* lse, int64_t N, int num_graphs, int H, int Hk, int D, float scale,
+                                       const uint8_t* mask, const int32_t* ptr, const int32_t* tiles, int n_tiles, const int32_t* blocks,
+                                       int n_blocks, float* dq, float* dk, float* dv, void* ws, size_t ws_bytes, hipStream_t stream) {
+    AtArgs a = {};
+    const int rc = at_fill(a, "graph_attention_bwd", N, num_graphs, H, Hk, D, scale, mask, ptr, tiles, n_tiles, blocks, n_blocks, ws, ws_bytes, true);
+    if (rc) return rc;
+    HGV_REQUIRE(q && k && v && g && out && lse && (dq || dk) && !dk == !dv, HGV_EINVAL, "graph_attention_bwd: null buffer (dk and dv come together)");
+    HGV_REQUIRE(D % 4 || (hgv_aligned(dq, 16) && hgv_aligned(dk, 16) && hgv_aligned(dv, 16)), HGV_EINVAL, "graph_attention_bwd: misaligned buffer");
+    a.src[TQ] = q; a.row_stride[TQ] = q_row; a.head_stride[TQ] = q_head;
+    a.src[TK] = k; a.row_stride[TK] = k_row; a.head_stride[TK] = k_head;
+    a.src[TV] = v; a.row_stride[TV] = v_row; a.head_stride[TV] = v_head;
+    a.src[TG] = g; a.row_stride[TG] = g_row; a.head_stride[TG] = g_head;
+    a.out = (float*)out; a.lse = (float*)lse; a.dq = dq; a.dk = dk; a.dv = dv;
+    return at_dispatch(a, true, stream);
+}

@@ -2657,3 +2657,100 @@ def group_norm_act(x: torch.Tensor, segments, groups: int, weight: Optional[torc
             y = x * 1.0 if weight is None else x * weight
             return y if bias is None else y + bias
         return _GroupNormAct.apply(x, weight, bias, seg, groups, _ACTS[act], eps, bool(keep8))
+
+
+# --------------------------------------------------------------------------------------
+# attention among the nodes of a graph
+# --------------------------------------------------------------------------------------
+MAX_HEAD = 128
+
+
+def _unit_rows(t: torch.Tensor) -> torch.Tensor:
+    return t if t.size(2) == 1 or t.stride(2) == 1 else t.contiguous()
+
+
+def _strided(t: torch.Tensor):
+    return t.data_ptr(), t.stride(0), t.stride(1)
+
+
+class _GraphAttention(torch.autograd.Function):
+    """softmax(scale q k^T) v within each graph; keeps the output and one number per row and head, and recomputes the
+    probabilities in the backward pass."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, seg: Segments, mask, scale):
+        q, k, v = _unit_rows(q), _unit_rows(k), _unit_rows(v)
+        n, h, d = q.shape
+        hk = k.size(1)
+        out = torch.empty(n, h, d, dtype=torch.float32, device=q.device)
+        train = any(ctx.needs_input_grad[:3])
+        lse = torch.empty(h, n, dtype=torch.float32, device=q.device) if train else None
+        nws = _lib.load().hgv_graph_attention_ws(n, seg.num_graphs, h, hk, d, seg._n_tiles, 0)
+        ws = torch.empty(nws, dtype=torch.uint8, device=q.device)
+        _lib.call("hgv_graph_attention_fwd", *_strided(q), *_strided(k), *_strided(v), n, seg.num_graphs, h, hk, d, scale, _lib.ptr(mask),
+                  seg._ptr.data_ptr(), seg._tiles.data_ptr(), seg._n_tiles, seg._blocks.data_ptr(), seg._n_blocks, out.data_ptr(),
+                  _lib.ptr(lse), ws.data_ptr(), nws, _lib.stream())
+        ctx.seg, ctx.scale = seg, scale
+        if train:
+            ctx.save_for_backward(q, k, v, out, lse, mask)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        q, k, v, out, lse, mask = ctx.saved_tensors
+        seg, need = ctx.seg, ctx.needs_input_grad
+        n, h, d = q.shape
+        hk = k.size(1)
+        with _on_device(g):
+            g = _unit_rows(g)
+            dq = torch.empty(n, h, d, dtype=torch.float32, device=q.device) if need[0] else None
+            dk, dv = (torch.empty(n, hk, d, dtype=torch.float32, device=q.device) if need[1] or need[2] else None for _ in range(2))
+            nws = _lib.load().hgv_graph_attention_ws(n, seg.num_graphs, h, hk, d, seg._n_tiles, 1)
+            ws = torch.empty(nws, dtype=torch.uint8, device=q.device)
+            _lib.call("hgv_graph_attention_bwd", *_strided(q), *_strided(k), *_strided(v), *_strided(g), out.data_ptr(), lse.data_ptr(), n,
+                      seg.num_graphs, h, hk, d, ctx.scale, _lib.ptr(mask), seg._ptr.data_ptr(), seg._tiles.data_ptr(), seg._n_tiles,
+                      seg._blocks.data_ptr(), seg._n_blocks, _lib.ptr(dq), _lib.ptr(dk), _lib.ptr(dv), ws.data_ptr(), nws, _lib.stream())
+        return dq, dk if need[1] else None, dv if need[2] else None, None, None, None
+
+
+def graph_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, segments, mask: Optional[torch.Tensor] = None,
+                    scale: Optional[float] = None) -> torch.Tensor:
+    """Attention of every node to the nodes of its own graph: ``softmax(scale * q k^T) v`` per graph and head, fp32.
+
+    ``q`` ``[N, H, D]``, ``k`` and ``v`` ``[N, Hk, D]`` with H a multiple of Hk (query heads h * H / Hk ... share key head h)
+    and D up to 128; slices of a wider projection are taken as they are where the last axis has unit stride.
+    ``segments``: a :class:`~hgvae_amd.graph.Segments`, or a ``batch`` vector (then one host synchronisation per call).
+    ``mask`` ``[N]`` bool: nodes that take part as keys; a graph without any gives zeros, and what a masked row of ``k`` or
+    ``v`` holds does not matter.  ``scale`` (positive) defaults to ``D ** -0.5``.  Returns ``[N, H, D]``.
+
+    The backward pass recomputes the probabilities from the output and one number per row and head; its results do not
+    depend on the order in which workgroups run.  Gradients cannot be differentiated again."""
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        if not isinstance(t, torch.Tensor) or t.dim() != 3 or t.dtype != torch.float32:
+            raise _lib.HgvError(f"{name} must be a float32 [N, heads, columns] tensor, got "
+                                f"{(t.dtype, tuple(t.shape)) if isinstance(t, torch.Tensor) else type(t).__name__}")
+        _lib.require_cuda(t)
+        if t.device != q.device:
+            raise _lib.HgvError(f"{name} is on {t.device}, q is on {q.device}")
+    n, h, d = q.shape
+    if k.shape != v.shape or k.size(0) != n or k.size(2) != d or h < 1 or k.size(1) < 1 or h % k.size(1):
+        raise _lib.HgvError(f"q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not belong together")
+    if not 1 <= d <= MAX_HEAD:
+        raise _lib.HgvError(f"heads of {d} columns are not supported (1 to {MAX_HEAD})")
+    if h > 65535:
+        raise _lib.HgvError(f"{h} heads are not supported")
+    scale = d ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale < float("inf"):
+        raise _lib.HgvError(f"scale must be positive and finite, got {scale}")
+    if mask is not None:
+        if not isinstance(mask, torch.Tensor) or mask.dtype != torch.bool or mask.shape != (n,) or mask.device != q.device:
+            raise _lib.HgvError(f"mask must be a bool vector of {n} on {q.device}")
+        mask = mask.contiguous().view(torch.uint8)
+    with _on_device(q):
+        seg = segments_of(segments, n)
+        if seg.device != q.device:
+            raise _lib.HgvError(f"segments are on {seg.device}, q is on {q.device}")
+        if n == 0:
+            return q * 1.0 + (k.sum() + v.sum()) * 0.0          # an empty result whose gradients are zeros
+        return _GraphAttention.apply(q, k, v, seg, mask, scale)

@@ -292,12 +292,28 @@ class Segments:
         chunks = np.zeros((total, 4), dtype=np.int64)
         chunks[:, 0], chunks[:, 1] = order[which], start
         chunks[:, 2] = np.minimum(start + per[which], ptr[order + 1][which])
-        parts = [chunks.ravel(), ptr, order, self._first_chunk]
+        # attention: tiles of 64 rows in row order, each with the first tile of its graph and their number, and blocks of 128
+        # rows, those of the largest graphs first
+        tiles, blocks = self._tiles_of(sizes, ptr, np.flatnonzero(sizes), 64), self._tiles_of(sizes, ptr, order[::-1], 128)
+        self._n_tiles, self._n_blocks = len(tiles), len(blocks)
+        parts = [chunks.ravel(), tiles.ravel(), blocks.ravel(), ptr, order, self._first_chunk]
         host = np.concatenate(parts).astype(np.int32)
         self._buf = torch.from_numpy(host).to(self.device)          # copied before the call returns: any stream may read it
         at = np.cumsum([0] + [p.size for p in parts])
-        self._chunks, self._ptr, self._order, self._first = (self._buf[at[i]:at[i + 1]] for i in range(4))
+        self._chunks, self._tiles, self._blocks, self._ptr, self._order, self._first = (self._buf[at[i]:at[i + 1]] for i in range(6))
         self._norm_plans: "dict[tuple, tuple]" = {}
+
+    @staticmethod
+    def _tiles_of(sizes, ptr, graphs, rows: int) -> np.ndarray:
+        """(graph, first row, first tile of the graph, tiles of the graph) of every tile of ``rows`` rows, graph by graph."""
+        counts = -(-sizes[graphs] // rows)
+        first = np.cumsum(counts) - counts
+        total = int(counts.sum())
+        which = np.repeat(np.arange(len(graphs)), counts)
+        out = np.empty((total, 4), dtype=np.int64)
+        out[:, 0], out[:, 2], out[:, 3] = graphs[which], first[which], counts[which]
+        out[:, 1] = ptr[graphs][which] + (np.arange(total) - first[which]) * rows
+        return out
 
     @classmethod
     def from_sizes(cls, sizes: Sequence[int], device="cuda") -> "Segments":

@@ -122,6 +122,65 @@ class GATConv(nn.Module):
                 "(gvae/gvae_skipcon_attention.py:74,96)")
 
 
+class GroupNormAct(nn.Module):
+    """Group norm with an activation over the rows of each graph (:func:`~hgvae_amd.functional.group_norm_act`):
+    ``forward(x, segments)``.  ``keep8`` keeps the input of the level in 8 bits for the backward pass."""
+
+    def __init__(self, channels: int, groups: int, act: str = "silu", eps: float = 1e-5, affine: bool = True, keep8: bool = False):
+        super().__init__()
+        if groups < 1 or channels < 1 or channels % groups:
+            raise ValueError(f"{channels} channels cannot be split into {groups} groups")
+        self.channels, self.groups, self.act, self.eps, self.keep8 = channels, groups, act, eps, keep8
+        self.weight = nn.Parameter(torch.ones(channels)) if affine else None
+        self.bias = nn.Parameter(torch.zeros(channels)) if affine else None
+
+    def forward(self, x: torch.Tensor, segments) -> torch.Tensor:
+        return Fn.group_norm_act(x, segments, self.groups, self.weight, self.bias, act=self.act, eps=self.eps, keep8=self.keep8)
+
+    def extra_repr(self):
+        return f"{self.channels}, groups={self.groups}, act={self.act}, keep8={self.keep8}"
+
+
+class Linear8(nn.Linear):
+    """``nn.Linear`` that keeps its input in 8 bits for the weight gradient (:func:`~hgvae_amd.functional.linear8`)."""
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        return Fn.linear8(x, self.weight, self.bias)
+
+
+class GraphAttention(nn.Module):
+    """Multi-head attention among the nodes of each graph: projections to ``heads`` queries and ``kv_heads`` keys and
+    values, :func:`~hgvae_amd.functional.graph_attention`, output projection.  ``forward(x, segments, mask=None)``.  With
+    ``keep8`` the projections keep their input in 8 bits for the backward pass."""
+
+    def __init__(self, channels: int, heads: int = 1, kv_heads: int = None, head_dim: int = None, keep8: bool = False):
+        super().__init__()
+        kv_heads = heads if kv_heads is None else kv_heads
+        if head_dim is None:
+            if heads < 1 or channels % heads:
+                raise ValueError(f"{channels} channels cannot be split into {heads} heads")
+            head_dim = channels // heads
+        if heads < 1 or kv_heads < 1 or heads % kv_heads:
+            raise ValueError(f"{heads} heads cannot share {kv_heads} key heads")
+        self.channels, self.heads, self.kv_heads, self.head_dim, self.keep8 = channels, heads, kv_heads, head_dim, keep8
+        self.lin_q = nn.Linear(channels, heads * head_dim, bias=False)
+        self.lin_k = nn.Linear(channels, kv_heads * head_dim, bias=False)
+        self.lin_v = nn.Linear(channels, kv_heads * head_dim, bias=False)
+        self.lin_out = nn.Linear(heads * head_dim, channels)
+        for lin in (self.lin_q, self.lin_k, self.lin_v, self.lin_out):
+            _kaiming_linear_(lin)
+
+    def forward(self, x: torch.Tensor, segments, mask=None) -> torch.Tensor:
+        project = Fn.linear8 if self.keep8 else (lambda x, w, b=None: Fn.dual_linear(x, w, bias=b))
+        n, d = x.size(0), self.head_dim
+        q, k, v = (project(x, lin.weight).unflatten(1, (-1, d)) for lin in (self.lin_q, self.lin_k, self.lin_v))
+        out = Fn.graph_attention(q, k, v, segments, mask=mask)
+        return project(out.reshape(n, self.heads * d), self.lin_out.weight, self.lin_out.bias)
+
+    def extra_repr(self):
+        return f"{self.channels}, heads={self.heads}, kv_heads={self.kv_heads}, head_dim={self.head_dim}, keep8={self.keep8}"
+
+
 class SelectTopK(nn.Module):
     """The scalar selector PyG >= 2.4 keeps inside SAGPooling (checkpoint key ``select.weight``, shape [1, 1],
     U(-1, 1) at init): score = tanh(s * w / ||w||)."""

@@ -596,6 +596,28 @@ int hgv_group_norm_bwd(const float* g, int64_t ldg, const float* x, int64_t ldx,
                        int n_batches, const int64_t* batches, int64_t batch_chunks, const double* mean, const float* rstd, float* gx,
                        int64_t ldgx, float* gw, float* gb, void* ws, size_t ws_bytes, hgv_stream_t stream);
 
+/* ---- attention among the nodes of each graph (no reference counterpart: its attention runs along edges, GATConv at
+ *      gvae/gvae_skipcon_attention.py:68) -----------------------------------------------------------------------------
+ * q, out, dq [N, H, D]; k, v, dk, dv [N, Hk, D], H a multiple of Hk, D <= 128; head h of q reads head h / (H / Hk).  q, k, v and
+ * g have unit stride along D and any row and head strides (elements); out and the gradients are contiguous (16-byte aligned
+ * where D is a multiple of 4).  For row i of a graph over its keys j (mask[j] != 0, or all where mask is NULL):
+ *   p = softmax_j(scale * q_i . k_j),  out_i = sum_j p_j v_j;   a graph without keys gives zeros, and zero gradients.
+ * A masked row of k or v may hold anything; its dk and dv are zeros.  scale > 0.
+ * Graphs: ptr [num_graphs + 1]; tiles [n_tiles][4] (graph, first row, first tile of the graph, tiles of the graph) of 64 rows;
+ * blocks [n_blocks][4] (graph, first row, -, -) of 128 rows, in the order in which they are to run.
+ * lse [H, N] (base 2, of the scaled logits; +inf for a row without keys) may be NULL in the forward pass; the backward pass
+ * reads it and out.  dq, or dk and dv together, may be NULL. */
+size_t hgv_graph_attention_ws(int64_t N, int num_graphs, int H, int Hk, int D, int64_t n_tiles, int backward);
+int hgv_graph_attention_fwd(const float* q, int64_t q_row, int64_t q_head, const float* k, int64_t k_row, int64_t k_head, const float* v,
+                            int64_t v_row, int64_t v_head, int64_t N, int num_graphs, int H, int Hk, int D, float scale,
+                            const uint8_t* mask, const int32_t* ptr, const int32_t* tiles, int n_tiles, const int32_t* blocks,
+                            int n_blocks, float* out, float* lse, void* ws, size_t ws_bytes, hgv_stream_t stream);
+int hgv_graph_attention_bwd(const float* q, int64_t q_row, int64_t q_head, const float* k, int64_t k_row, int64_t k_head, const float* v,
+                            int64_t v_row, int64_t v_head, const float* g, int64_t g_row, int64_t g_head, const float* out,
+                            const float* lse, int64_t N, int num_graphs, int H, int Hk, int D, float scale, const uint8_t* mask,
+                            const int32_t* ptr, const int32_t* tiles, int n_tiles, const int32_t* blocks, int n_blocks, float* dq,
+                            float* dk, float* dv, void* ws, size_t ws_bytes, hgv_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
