@@ -193,16 +193,25 @@ __device__ __forceinline__ Frag col_frag(const unsigned char* lds, int r0, int d
     return f;
 }
 
+// Two pieces of values in registers.  The large piece is cut (v_cvt_pkrtz, two values at once) rather than rounded: what is
+// left then goes into the small piece whatever happened to x before.  (A plain conversion may be merged with the multiplication
+// in front of it, which rounds once instead of twice, and the difference was then taken from the other result: one value in some
+// thousands lost its small piece.)  The small piece is rounded to nearest: 2^-22 of x, without a drift.
+__device__ __forceinline__ void split2(float x, float y, f16x2& hi, f16x2& lo) {
+    union { __fp16 __attribute__((ext_vector_type(2))) a; f16x2 b; } u;
+    u.a = __builtin_amdgcn_cvt_pkrtz(x, y);
+    hi = u.b;
+    const float rx = fmaf((float)hi[0], -1.f, x), ry = fmaf((float)hi[1], -1.f, y);
+    lo = f16x2{(_Float16)rx, (_Float16)ry};
+}
+
 __device__ __forceinline__ Frag split_frag(const f32x4& x, const f32x4& y) {
-    Frag f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        f.hi[i] = (_Float16)x[i];
-        f.lo[i] = (_Float16)(x[i] - (float)f.hi[i]);
-        f.hi[4 + i] = (_Float16)y[i];
-        f.lo[4 + i] = (_Float16)(y[i] - (float)f.hi[4 + i]);
-    }
-    return f;
+    union { Frag f; struct { f16x2 hi[4], lo[4]; } p; } u;
+    split2(x[0], x[1], u.p.hi[0], u.p.lo[0]);
+    split2(x[2], x[3], u.p.hi[1], u.p.lo[1]);
+    split2(y[0], y[1], u.p.hi[2], u.p.lo[2]);
+    split2(y[2], y[3], u.p.hi[3], u.p.lo[3]);
+    return u.f;
 }
 
 __device__ __forceinline__ f32x4 mma3(const Frag& a, const Frag& b, f32x4 c) {

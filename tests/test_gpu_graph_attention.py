@@ -100,7 +100,7 @@ def run(q, k, v, seg, g, mask=None, scale=None):
 
 SHAPES = [([1], 1, 1, 1), ([1, 1, 1], 2, 1, 5), ([2, 0, 3], 1, 1, 32), ([64], 2, 2, 64), ([65, 63], 4, 2, 23), ([138] * 3, 4, 4, 64),
           ([127, 128, 129, 1], 3, 1, 96), ([300], 2, 1, 128), ([454, 7], 6, 2, 23), ([200], 1, 1, 127), ([90, 300], 2, 2, 33), ([1000], 1, 1, 64),
-          ([17] * 20, 2, 2, 16), ([700], 3, 3, 97)]
+          ([17] * 20, 2, 2, 16), ([700], 3, 3, 97), ([8] * 600, 1, 1, 16)]
 
 
 @pytest.mark.parametrize("sizes,h,hk,d", SHAPES, ids=[f"{len(s)}x{max(s)}-{h}-{hk}-{d}" for s, h, hk, d in SHAPES])
