@@ -255,7 +255,7 @@ constexpr float P_GROW = 7.f;
 // ---- forward -----------------------------------------------------------------------------------------------------------------
 // A workgroup owns 128 queries of one head (a wave 32), walks the keys of the graph in tiles of 64.
 template <int DP>
-__global__ __launch_bounds__(256) void k_at_fwd(const AtArgs a) {
+__global__ __launch_bounds__(256, 2) void k_at_fwd(const AtArgs a) {
     constexpr int KC = DP / 32, DB = DP / 16;
     __shared__ __align__(16) unsigned char ldsK[64 * row_bytes<DP>()];
     __shared__ __align__(16) unsigned char ldsV[64 * row_bytes<DP>()];
@@ -368,7 +368,7 @@ __global__ __launch_bounds__(256) void k_at_fwd(const AtArgs a) {
 // ---- backward: dk and dv ---------------------------------------------------------------------------------------------------
 // A workgroup owns 64 * KB keys of one key head (a wave 16 * KB), walks the queries of the graph, head by head, in tiles of 64 rows.
 template <int DP, int KB>
-__global__ __launch_bounds__(256) void k_at_dkv(const AtArgs a) {
+__global__ __launch_bounds__(256, 2) void k_at_dkv(const AtArgs a) {
     constexpr int KC = DP / 32, DB = DP / 16;
     __shared__ __align__(16) unsigned char ldsQ[64 * row_bytes<DP>()];
     __shared__ __align__(16) unsigned char ldsG[64 * row_bytes<DP>()];
@@ -498,7 +498,7 @@ __global__ __launch_bounds__(256) void k_at_dkv(const AtArgs a) {
 
 // ---- backward: dq -----------------------------------------------------------------------------------------------------------
 template <int DP, int QB>
-__global__ __launch_bounds__(256) void k_at_dq(const AtArgs a) {
+__global__ __launch_bounds__(256, 2) void k_at_dq(const AtArgs a) {
     constexpr int KC = DP / 32, DB = DP / 16;
     __shared__ __align__(16) unsigned char ldsK[64 * row_bytes<DP>()];
     __shared__ __align__(16) unsigned char ldsV[64 * row_bytes<DP>()];
