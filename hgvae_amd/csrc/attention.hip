@@ -21,6 +21,7 @@ typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int TQ = 0, TK = 1, TV = 2, TG = 3;                   // tensors: q, k, v, gradient of the output
 constexpr int NO_EXP = -(1 << 20);                              // "no finite non-zero row"
@@ -33,8 +34,10 @@ struct AtArgs {
     const int32_t* ptr;
     const int4* tiles;                                          // prepass tiles of 64 rows: (graph, row, first tile, tiles of the graph)
     int n_tiles;
-    const int4* blocks;                                         // tiles of 128 rows: (graph, row, -, -), largest graphs first
-    int n_blocks;
+    const int4* blocks;                                         // of a launch: tiles of 64 or 128 rows, largest graphs first
+    const int4* block_list[2]; int n_blocks[2];                 // all of them: (graph, row, -, -) of 64 rows, of 128 rows
+    float neg;                                                  // -1, unknown to the compiler: keeps x - (float)half one instruction (v_fma_mix_f32)
+
     int* part;                                                  // [tile][4][Hk] exponents of the longest row
     int* exps;                                                  // [B][Hk][4]
     _Float16* img[4];                                           // [heads][N][hi DP | lo DP]
@@ -137,59 +140,67 @@ __global__ __launch_bounds__(256) void k_at_split(const AtArgs a) {
 }
 
 // ---- pieces shared by the three products -----------------------------------------------------------------------------------
-// LDS tile of 64 rows: row = [hi DP | lo DP] fp16 + 16 bytes, which puts the same 16-byte chunk of 16 consecutive rows into all
-// 64 banks.
-template <int DP> constexpr int row_bytes() { return 4 * DP + 16; }
+// Products run on v_mfma_f32_16x16x32_f16 (with real operands it delivers 1.9 PFLOP/s on this card, the 32x32x16 form 1.5: power, not
+// issue, is what limits them): a row operand has lane l hold row l & 15, columns 8 (l >> 4) .. + 7 of a 32-wide slice; a column
+// operand the same with columns for rows; the result has lane l hold column l & 15, rows 4 (l >> 4) + 0..3.
+//
+// LDS tile: a line is [hi DP | lo DP] fp16 + 16 bytes, and of 16 rows the first eight take the even lines: then neither 16 rows of
+// one 16-byte chunk (row operands) nor 8 rows of two chunks (transposing loads, 32 lanes at a time) meet in one of the 64 banks.
+template <int DP> constexpr int line_bytes() { return 4 * DP + 16; }
+__device__ __forceinline__ int line_of(int row) { return (row & ~15) | ((row & 7) << 1) | ((row >> 3) & 1); }
 
-template <int DP>
-struct Stage {                                                  // a thread's share of a 64-row tile on its way to LDS
-    static constexpr int CH = DP / 16;                          // 16-byte chunks per thread
+// A thread's share of a tile of 64 rows on its way to LDS (threads: NT); rows from `rows` on are zeros.
+template <int DP, int NT>
+struct Stage {
+    static constexpr int CH = 64 * (DP / 4) / NT;               // 16-byte chunks per thread
     uint4 v[CH];
     __device__ __forceinline__ void load(const _Float16* tile, int rows) {          // tile: first row in the image
         const uint4* p = (const uint4*)tile;
 #pragma unroll
         for (int i = 0; i < CH; ++i) {
-            const int f = threadIdx.x + 256 * i, r = f / (DP / 4);
+            const int f = threadIdx.x + NT * i, r = f / (DP / 4);
             v[i] = r < rows ? p[f] : make_uint4(0, 0, 0, 0);
         }
     }
     __device__ __forceinline__ void store(unsigned char* lds) const {
 #pragma unroll
         for (int i = 0; i < CH; ++i) {
-            const int f = threadIdx.x + 256 * i, r = f / (DP / 4), c = f - r * (DP / 4);
-            *(uint4*)(lds + r * row_bytes<DP>() + c * 16) = v[i];
+            const int f = threadIdx.x + NT * i, r = f / (DP / 4), c = f - r * (DP / 4);
+            *(uint4*)(lds + line_of(r) * line_bytes<DP>() + c * 16) = v[i];
         }
     }
 };
 
 struct Frag { f16x8 hi, lo; };
 
-// rows r0 + (lane & 15), columns 32 c + 8 (lane >> 4) ..: a row-operand fragment
+// rows r0 + (lane & 15) (r0 a multiple of 16), columns 32 c + 8 (lane >> 4) ..
 template <int DP>
 __device__ __forceinline__ Frag row_frag(const unsigned char* lds, int r0, int c, int lane) {
-    const unsigned char* p = lds + (r0 + (lane & 15)) * row_bytes<DP>() + c * 64 + (lane >> 4) * 16;
+    const unsigned char* p = lds + line_of(lane & 15) * line_bytes<DP>() + (lane >> 4) * 16 + r0 * line_bytes<DP>() + c * 64;
     Frag f;
     f.hi = *(const f16x8*)p;
     f.lo = *(const f16x8*)(p + 2 * DP);
     return f;
 }
 
-__device__ __forceinline__ f16x8 tr_read(const unsigned char* p, int next) {
+__device__ __forceinline__ s16x4 tr_read(const unsigned char* p) {
     typedef __attribute__((address_space(3))) s16x4 lds_v;
-    union { struct { s16x4 a, b; } s; f16x8 v; } u;
-    u.s.a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v*)p);
-    u.s.b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v*)(p + next));
-    return u.v;
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v*)p);
 }
-// the transposed tile: fragment row d = 16 db + (lane & 15); its eight values are tile rows r0 + 4g + 0..3 and r0 + 16 + 4g + 0..3
-// (g = lane >> 4), the order in which split_frag lays out a product's rows
+// the transposed tile as a row operand: row d = 16 db + (lane & 15); its eight values are tile rows r0 + 4 g + 0..3 and
+// r0 + 16 + 4 g + 0..3 (g = lane >> 4): the rows that a lane holds of two results, in the order of split_frag
 template <int DP>
 __device__ __forceinline__ Frag col_frag(const unsigned char* lds, int r0, int db, int lane) {
-    const int g = lane >> 4, i = lane & 15;
-    const unsigned char* p = lds + (r0 + 4 * g + (i >> 2)) * row_bytes<DP>() + db * 32 + (i & 3) * 8;
+    const int i = lane & 15;
+    const unsigned char* hi = lds + line_of(4 * (lane >> 4) + (i >> 2)) * line_bytes<DP>() + (i & 3) * 8 + r0 * line_bytes<DP>() + db * 32;
+    const unsigned char* lo = hi + 2 * DP;
+    union { struct { s16x4 a, b; } s; f16x8 v; } u, w;
+    u.s.a = tr_read(hi);
+    u.s.b = tr_read(hi + 16 * line_bytes<DP>());
+    w.s.a = tr_read(lo);
+    w.s.b = tr_read(lo + 16 * line_bytes<DP>());
     Frag f;
-    f.hi = tr_read(p, 16 * row_bytes<DP>());
-    f.lo = tr_read(p + 2 * DP, 16 * row_bytes<DP>());
+    f.hi = u.v; f.lo = w.v;
     return f;
 }
 
@@ -197,20 +208,20 @@ __device__ __forceinline__ Frag col_frag(const unsigned char* lds, int r0, int d
 // left then goes into the small piece whatever happened to x before.  (A plain conversion may be merged with the multiplication
 // in front of it, which rounds once instead of twice, and the difference was then taken from the other result: one value in some
 // thousands lost its small piece.)  The small piece is rounded to nearest: 2^-22 of x, without a drift.
-__device__ __forceinline__ void split2(float x, float y, f16x2& hi, f16x2& lo) {
+__device__ __forceinline__ void split2(float x, float y, f16x2& hi, f16x2& lo, float neg) {
     union { __fp16 __attribute__((ext_vector_type(2))) a; f16x2 b; } u;
     u.a = __builtin_amdgcn_cvt_pkrtz(x, y);
     hi = u.b;
-    const float rx = fmaf((float)hi[0], -1.f, x), ry = fmaf((float)hi[1], -1.f, y);
+    const float rx = fmaf((float)hi[0], neg, x), ry = fmaf((float)hi[1], neg, y);
     lo = f16x2{(_Float16)rx, (_Float16)ry};
 }
 
-__device__ __forceinline__ Frag split_frag(const f32x4& x, const f32x4& y) {
+__device__ __forceinline__ Frag split_frag(const f32x4& x, const f32x4& y, float neg) {
     union { Frag f; struct { f16x2 hi[4], lo[4]; } p; } u;
-    split2(x[0], x[1], u.p.hi[0], u.p.lo[0]);
-    split2(x[2], x[3], u.p.hi[1], u.p.lo[1]);
-    split2(y[0], y[1], u.p.hi[2], u.p.lo[2]);
-    split2(y[2], y[3], u.p.hi[3], u.p.lo[3]);
+    split2(x[0], x[1], u.p.hi[0], u.p.lo[0], neg);
+    split2(x[2], x[3], u.p.hi[1], u.p.lo[1], neg);
+    split2(y[0], y[1], u.p.hi[2], u.p.lo[2], neg);
+    split2(y[2], y[3], u.p.hi[3], u.p.lo[3], neg);
     return u.f;
 }
 
@@ -253,12 +264,12 @@ constexpr float P_BITS = 8.f;                                   // probabilities
 constexpr float P_GROW = 7.f;
 
 // ---- forward -----------------------------------------------------------------------------------------------------------------
-// A workgroup owns 128 queries of one head (a wave 32), walks the keys of the graph in tiles of 64.
-template <int DP>
-__global__ __launch_bounds__(256, 2) void k_at_fwd(const AtArgs a) {
+// A workgroup owns 32 * NW queries of one head (a wave 32), walks the keys of the graph in tiles of 64.
+template <int DP, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void k_at_fwd(const AtArgs a) {
     constexpr int KC = DP / 32, DB = DP / 16;
-    __shared__ __align__(16) unsigned char ldsK[64 * row_bytes<DP>()];
-    __shared__ __align__(16) unsigned char ldsV[64 * row_bytes<DP>()];
+    __shared__ __align__(16) unsigned char ldsK[64 * line_bytes<DP>()];
+    __shared__ __align__(16) unsigned char ldsV[64 * line_bytes<DP>()];
     __shared__ __align__(16) float bias[64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
     const int blk = blockIdx.x / a.H, h = blockIdx.x - blk * a.H, hk = h / a.R;
@@ -279,7 +290,7 @@ __global__ __launch_bounds__(256, 2) void k_at_fwd(const AtArgs a) {
     const _Float16* ki = a.img[TK] + ((int64_t)hk * a.N + k0) * (2 * DP);
     const _Float16* vi = a.img[TV] + ((int64_t)hk * a.N + k0) * (2 * DP);
     const int n = (int)(k1 - k0);
-    Stage<DP> sk, sv;
+    Stage<DP, 64 * NW> sk, sv;
     sk.load(ki, min(64, n));
     sv.load(vi, min(64, n));
     float nb = threadIdx.x < 64 && (int)threadIdx.x < n && (!a.mask || a.mask[k0 + threadIdx.x]) ? 0.f : -INFINITY;
@@ -315,9 +326,9 @@ __global__ __launch_bounds__(256, 2) void k_at_fwd(const AtArgs a) {
         }
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
-            float top = fmaxf(fmaxf(s[0][b][0], s[0][b][1]), fmaxf(s[0][b][2], s[0][b][3]));
+            float top = s[0][b][0];
 #pragma unroll
-            for (int i = 1; i < 4; ++i) top = fmaxf(top, fmaxf(fmaxf(s[i][b][0], s[i][b][1]), fmaxf(s[i][b][2], s[i][b][3])));
+            for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i >> 2][b][i & 3]);
             top = fmaxf(top, __shfl_xor(top, 16, 64));
             top = fmaxf(top, __shfl_xor(top, 32, 64)) * c;
             // rescale only when a probability would leave its range
@@ -330,18 +341,20 @@ __global__ __launch_bounds__(256, 2) void k_at_fwd(const AtArgs a) {
                 for (int d = 0; d < DB; ++d) acc[d][b] *= f;
             }
             const float off = m[b] == -INFINITY ? 0.f : P_BITS - m[b];
+            float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const float p = exp2_fast(fmaf(s[i][b][j], c, off));
                     s[i][b][j] = p;
-                    l[b] += p;
+                    sum[j] += p;
                 }
+            l[b] += (sum[0] + sum[1]) + (sum[2] + sum[3]);
         }
 #pragma unroll
         for (int kc = 0; kc < 2; ++kc) {
-            const Frag p0 = split_frag(s[2 * kc][0], s[2 * kc + 1][0]), p1 = split_frag(s[2 * kc][1], s[2 * kc + 1][1]);
+            const Frag p0 = split_frag(s[2 * kc][0], s[2 * kc + 1][0], a.neg), p1 = split_frag(s[2 * kc][1], s[2 * kc + 1][1], a.neg);
 #pragma unroll
             for (int d = 0; d < DB; ++d) {
                 const Frag f = col_frag<DP>(ldsV, 32 * kc, d, lane);
@@ -366,22 +379,19 @@ __global__ __launch_bounds__(256, 2) void k_at_fwd(const AtArgs a) {
 }
 
 // ---- backward: dk and dv ---------------------------------------------------------------------------------------------------
-// A workgroup owns 64 * KB keys of one key head (a wave 16 * KB), walks the queries of the graph, head by head, in tiles of 64 rows.
-template <int DP, int KB>
-__global__ __launch_bounds__(256, 2) void k_at_dkv(const AtArgs a) {
+// A workgroup owns 16 * KB * NW keys of one key head (a wave 16 * KB), walks the queries of the graph, head by head, in tiles of 64 rows.
+template <int DP, int KB, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void k_at_dkv(const AtArgs a) {
     constexpr int KC = DP / 32, DB = DP / 16;
-    __shared__ __align__(16) unsigned char ldsQ[64 * row_bytes<DP>()];
-    __shared__ __align__(16) unsigned char ldsG[64 * row_bytes<DP>()];
+    __shared__ __align__(16) unsigned char ldsQ[64 * line_bytes<DP>()];
+    __shared__ __align__(16) unsigned char ldsG[64 * line_bytes<DP>()];
     __shared__ __align__(16) float ldsL[64];
     __shared__ __align__(16) float ldsD[64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
-    constexpr int SPLIT = 2 / KB;                               // workgroups per 128-row block
-    const int unit = blockIdx.x / a.Hk, hk = blockIdx.x - unit * a.Hk;
-    const int4 t = a.blocks[unit / SPLIT];
+    const int blk = blockIdx.x / a.Hk, hk = blockIdx.x - blk * a.Hk;
+    const int4 t = a.blocks[blk];
     const int64_t g0 = a.ptr[t.x], g1 = a.ptr[t.x + 1];
-    const int64_t first = (int64_t)t.y + (unit % SPLIT) * 64;
-    if (first >= g1) return;
-    const int64_t key0 = first + 16 * KB * wave;
+    const int64_t key0 = (int64_t)t.y + 16 * KB * wave;
     const int* ex = a.exps + ((int64_t)t.x * a.Hk + hk) * 4;
     const float c = fold_scale(a.scale, ex[TQ] + ex[TK] - 30);
     Frag kf[KB][KC], vf[KB][KC];
@@ -399,7 +409,7 @@ __global__ __launch_bounds__(256, 2) void k_at_dkv(const AtArgs a) {
 #pragma unroll
         for (int b = 0; b < KB; ++b) dk[d][b] = dv[d][b] = f32x4{0.f, 0.f, 0.f, 0.f};
     const int n = (int)(g1 - g0), tiles = (n + 63) / 64, steps = tiles * a.R;
-    Stage<DP> sq, sg;
+    Stage<DP, 64 * NW> sq, sg;
     float nl = INFINITY, nd = 0.f;
     auto fetch = [&](int step) __attribute__((always_inline)) {
         const int hh = hk * a.R + step / tiles, r0 = (step % tiles) * 64, rows = min(64, n - r0);
@@ -456,8 +466,8 @@ __global__ __launch_bounds__(256, 2) void k_at_dkv(const AtArgs a) {
                 }
 #pragma unroll
                 for (int j = 0; j < KB; ++j) {
-                    pf[j] = split_frag(p[0][j], p[1][j]);
-                    df[j] = split_frag(s[0][j], s[1][j]);
+                    pf[j] = split_frag(p[0][j], p[1][j], a.neg);
+                    df[j] = split_frag(s[0][j], s[1][j], a.neg);
                 }
             }
 #pragma unroll
@@ -497,20 +507,17 @@ __global__ __launch_bounds__(256, 2) void k_at_dkv(const AtArgs a) {
 }
 
 // ---- backward: dq -----------------------------------------------------------------------------------------------------------
-template <int DP, int QB>
-__global__ __launch_bounds__(256, 2) void k_at_dq(const AtArgs a) {
+template <int DP, int QB, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void k_at_dq(const AtArgs a) {
     constexpr int KC = DP / 32, DB = DP / 16;
-    __shared__ __align__(16) unsigned char ldsK[64 * row_bytes<DP>()];
-    __shared__ __align__(16) unsigned char ldsV[64 * row_bytes<DP>()];
+    __shared__ __align__(16) unsigned char ldsK[64 * line_bytes<DP>()];
+    __shared__ __align__(16) unsigned char ldsV[64 * line_bytes<DP>()];
     __shared__ __align__(16) float bias[64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
-    constexpr int SPLIT = 2 / QB;
-    const int unit = blockIdx.x / a.H, h = blockIdx.x - unit * a.H, hk = h / a.R;
-    const int4 t = a.blocks[unit / SPLIT];
+    const int blk = blockIdx.x / a.H, h = blockIdx.x - blk * a.H, hk = h / a.R;
+    const int4 t = a.blocks[blk];
     const int64_t k0 = a.ptr[t.x], k1 = a.ptr[t.x + 1];
-    const int64_t first = (int64_t)t.y + (unit % SPLIT) * 64;
-    if (first >= k1) return;
-    const int64_t q0 = first + 16 * QB * wave;
+    const int64_t q0 = (int64_t)t.y + 16 * QB * wave;
     const int* ex = a.exps + ((int64_t)t.x * a.Hk + hk) * 4;
     const float c = fold_scale(a.scale, ex[TQ] + ex[TK] - 30);
     Frag q[QB][KC], go[QB][KC];
@@ -534,7 +541,7 @@ __global__ __launch_bounds__(256, 2) void k_at_dq(const AtArgs a) {
     const _Float16* ki = a.img[TK] + ((int64_t)hk * a.N + k0) * (2 * DP);
     const _Float16* vi = a.img[TV] + ((int64_t)hk * a.N + k0) * (2 * DP);
     const int n = (int)(k1 - k0);
-    Stage<DP> sk, sv;
+    Stage<DP, 64 * NW> sk, sv;
     sk.load(ki, min(64, n));
     sv.load(vi, min(64, n));
     float nb = threadIdx.x < 64 && (int)threadIdx.x < n && (!a.mask || a.mask[k0 + threadIdx.x]) ? 0.f : -INFINITY;
@@ -588,7 +595,7 @@ __global__ __launch_bounds__(256, 2) void k_at_dq(const AtArgs a) {
                         }
                 }
 #pragma unroll
-                for (int j = 0; j < QB; ++j) df[j] = split_frag(s[0][j], s[1][j]);
+                for (int j = 0; j < QB; ++j) df[j] = split_frag(s[0][j], s[1][j], a.neg);
             }
 #pragma unroll
             for (int d = 0; d < DB; ++d) {
@@ -631,18 +638,35 @@ AtSizes at_sizes(int64_t N, int H, int Hk, int D, int64_t n_tiles, int64_t graph
     return s;
 }
 
+template <typename F>
+void at_rows(AtArgs& a, int heads, F launch) {
+    // blocks of 128 rows where that gives a workgroup to each of the 256 compute units, else of 64
+    const int i = (int64_t)a.n_blocks[1] * heads >= 256 ? 1 : 0;
+    a.blocks = a.block_list[i];
+    launch(i, dim3((unsigned)((int64_t)a.n_blocks[i] * heads)));
+}
+
 template <int DP>
-int at_launch(const AtArgs& a, bool backward, hipStream_t stream) {
+int at_launch(AtArgs a, bool backward, hipStream_t stream) {
     const int tensors = backward ? 4 : 3;
     hipLaunchKernelGGL(k_at_norms, dim3((unsigned)a.n_tiles, (unsigned)tensors), dim3(256), 0, stream, a);
     hipLaunchKernelGGL(k_at_split<DP>, dim3((unsigned)a.n_tiles, (unsigned)tensors, (unsigned)a.Hk), dim3(256), 0, stream, a);
     if (!backward) {
-        hipLaunchKernelGGL(k_at_fwd<DP>, dim3((unsigned)((int64_t)a.n_blocks * a.H)), dim3(256), 0, stream, a);
+        at_rows(a, a.H, [&](int i, dim3 grid) {
+            if (i) hipLaunchKernelGGL((k_at_fwd<DP, 4>), grid, dim3(256), 0, stream, a);
+            else hipLaunchKernelGGL((k_at_fwd<DP, 2>), grid, dim3(128), 0, stream, a);
+        });
     } else {
         // wide heads: 16 keys / queries per wave, so that the accumulators of 32 do not push the operands out of the registers
         constexpr int KB = DP <= 64 ? 2 : 1;
-        if (a.dk) hipLaunchKernelGGL((k_at_dkv<DP, KB>), dim3((unsigned)((int64_t)a.n_blocks * a.Hk * (2 / KB))), dim3(256), 0, stream, a);
-        if (a.dq) hipLaunchKernelGGL((k_at_dq<DP, KB>), dim3((unsigned)((int64_t)a.n_blocks * a.H * (2 / KB))), dim3(256), 0, stream, a);
+        if (a.dk) at_rows(a, a.Hk, [&](int i, dim3 grid) {
+            if (i) hipLaunchKernelGGL((k_at_dkv<DP, KB, 8 / KB>), grid, dim3(512 / KB), 0, stream, a);
+            else hipLaunchKernelGGL((k_at_dkv<DP, KB, 4 / KB>), grid, dim3(256 / KB), 0, stream, a);
+        });
+        if (a.dq) at_rows(a, a.H, [&](int i, dim3 grid) {
+            if (i) hipLaunchKernelGGL((k_at_dq<DP, KB, 8 / KB>), grid, dim3(512 / KB), 0, stream, a);
+            else hipLaunchKernelGGL((k_at_dq<DP, KB, 4 / KB>), grid, dim3(256 / KB), 0, stream, a);
+        });
     }
     HGV_CHECK_LAUNCH(backward ? "graph_attention_bwd" : "graph_attention_fwd");
     return HGV_OK;
@@ -658,16 +682,19 @@ int at_dispatch(const AtArgs& a, bool backward, hipStream_t stream) {
 }
 
 int at_fill(AtArgs& a, const char* what, int64_t N, int num_graphs, int H, int Hk, int D, float scale, const uint8_t* mask, const int32_t* ptr,
-            const int32_t* tiles, int n_tiles, const int32_t* blocks, int n_blocks, void* ws, size_t ws_bytes, bool backward) {
+            const int32_t* tiles, int n_tiles, const int32_t* blocks, int n64, int n128, void* ws, size_t ws_bytes, bool backward) {
     HGV_REQUIRE(N > 0 && N <= 0x7fffffff && num_graphs > 0 && H > 0 && Hk > 0 && H % Hk == 0 && D > 0, HGV_EINVAL, "%s: bad sizes", what);
     HGV_REQUIRE(D <= 128 && H <= 65535, HGV_EUNSUPPORTED, "%s: heads of %d columns (at most 128), %d of them", what, D, H);
     HGV_REQUIRE(scale > 0.f && scale < INFINITY, HGV_EINVAL, "%s: the scale must be positive and finite", what);
-    HGV_REQUIRE(ptr && tiles && blocks && n_tiles > 0 && n_blocks > 0, HGV_EINVAL, "%s: null plan", what);
-    HGV_REQUIRE((int64_t)n_blocks * H * 2 <= 0x7fffffff, HGV_EUNSUPPORTED, "%s: too many tiles", what);
+    HGV_REQUIRE(ptr && tiles && blocks && n_tiles > 0 && n64 > 0 && n128 > 0, HGV_EINVAL, "%s: null plan", what);
+    HGV_REQUIRE((int64_t)n64 * H <= 0x3fffffff, HGV_EUNSUPPORTED, "%s: too many tiles", what);
     const AtSizes s = at_sizes(N, H, Hk, D, n_tiles, num_graphs, backward);
     HGV_REQUIRE(ws && ws_bytes >= s.total && hgv_aligned(ws, 256), HGV_EWORKSPACE, "%s: workspace too small or misaligned", what);
+    a.neg = -1.f;
     a.N = N; a.H = H; a.Hk = Hk; a.R = H / Hk; a.D = D; a.scale = scale; a.mask = mask; a.ptr = ptr;
-    a.tiles = (const int4*)tiles; a.n_tiles = n_tiles; a.blocks = (const int4*)blocks; a.n_blocks = n_blocks;
+    a.tiles = (const int4*)tiles; a.n_tiles = n_tiles;
+    a.n_blocks[0] = n64; a.n_blocks[1] = n128;
+    a.block_list[0] = (const int4*)blocks; a.block_list[1] = a.block_list[0] + n64;
     char* p = (char*)ws;
     a.part = (int*)p; p += s.part;
     a.exps = (int*)p; p += s.exps;
@@ -686,10 +713,10 @@ extern "C" size_t hgv_graph_attention_ws(int64_t N, int num_graphs, int H, int H
 extern "C" int hgv_graph_attention_fwd(const float* q, int64_t q_row, int64_t q_head, const float* k, int64_t k_row, int64_t k_head,
                                        const float* v, int64_t v_row, int64_t v_head, int64_t N, int num_graphs, int H, int Hk, int D,
                                        float scale, const uint8_t* mask, const int32_t* ptr, const int32_t* tiles, int n_tiles,
-                                       const int32_t* blocks, int n_blocks, float* out, float* lse, void* ws, size_t ws_bytes,
+                                       const int32_t* blocks, int n64, int n128, float* out, float* lse, void* ws, size_t ws_bytes,
                                        hipStream_t stream) {
     AtArgs a = {};
-    const int rc = at_fill(a, "graph_attention_fwd", N, num_graphs, H, Hk, D, scale, mask, ptr, tiles, n_tiles, blocks, n_blocks, ws, ws_bytes, false);
+    const int rc = at_fill(a, "graph_attention_fwd", N, num_graphs, H, Hk, D, scale, mask, ptr, tiles, n_tiles, blocks, n64, n128, ws, ws_bytes, false);
     if (rc) return rc;
     HGV_REQUIRE(q && k && v && out && (D % 4 || hgv_aligned(out, 16)), HGV_EINVAL, "graph_attention_fwd: null or misaligned buffer");
     a.src[TQ] = q; a.row_stride[TQ] = q_row; a.head_stride[TQ] = q_head;
@@ -703,9 +730,9 @@ extern "C" int hgv_graph_attention_bwd(const float* q, int64_t q_row, int64_t q_
                                        const float* v, int64_t v_row, int64_t v_head, const float* g, int64_t g_row, int64_t g_head,
                                        const float* out, const float* lse, int64_t N, int num_graphs, int H, int Hk, int D, float scale,
                                        const uint8_t* mask, const int32_t* ptr, const int32_t* tiles, int n_tiles, const int32_t* blocks,
-                                       int n_blocks, float* dq, float* dk, float* dv, void* ws, size_t ws_bytes, hipStream_t stream) {
+                                       int n64, int n128, float* dq, float* dk, float* dv, void* ws, size_t ws_bytes, hipStream_t stream) {
     AtArgs a = {};
-    const int rc = at_fill(a, "graph_attention_bwd", N, num_graphs, H, Hk, D, scale, mask, ptr, tiles, n_tiles, blocks, n_blocks, ws, ws_bytes, true);
+    const int rc = at_fill(a, "graph_attention_bwd", N, num_graphs, H, Hk, D, scale, mask, ptr, tiles, n_tiles, blocks, n64, n128, ws, ws_bytes, true);
     if (rc) return rc;
     HGV_REQUIRE(q && k && v && g && out && lse && (dq || dk) && !dk == !dv, HGV_EINVAL, "graph_attention_bwd: null buffer (dk and dv come together)");
     HGV_REQUIRE(D % 4 || (hgv_aligned(dq, 16) && hgv_aligned(dk, 16) && hgv_aligned(dv, 16)), HGV_EINVAL, "graph_attention_bwd: misaligned buffer");

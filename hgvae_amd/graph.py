@@ -292,11 +292,11 @@ class Segments:
         chunks = np.zeros((total, 4), dtype=np.int64)
         chunks[:, 0], chunks[:, 1] = order[which], start
         chunks[:, 2] = np.minimum(start + per[which], ptr[order + 1][which])
-        # attention: tiles of 64 rows in row order, each with the first tile of its graph and their number, and blocks of 128
-        # rows, those of the largest graphs first
-        tiles, blocks = self._tiles_of(sizes, ptr, np.flatnonzero(sizes), 64), self._tiles_of(sizes, ptr, order[::-1], 128)
-        self._n_tiles, self._n_blocks = len(tiles), len(blocks)
-        parts = [chunks.ravel(), tiles.ravel(), blocks.ravel(), ptr, order, self._first_chunk]
+        # attention: tiles of 64 rows in row order, each with the first tile of its graph and their number, and blocks of 64
+        # and of 128 rows, those of the largest graphs first
+        tiles, blocks = self._tiles_of(sizes, ptr, np.flatnonzero(sizes), 64), [self._tiles_of(sizes, ptr, order[::-1], r) for r in (64, 128)]
+        self._n_tiles, self._n_blocks = len(tiles), [len(b) for b in blocks]
+        parts = [chunks.ravel(), tiles.ravel(), np.concatenate(blocks).ravel(), ptr, order, self._first_chunk]
         host = np.concatenate(parts).astype(np.int32)
         self._buf = torch.from_numpy(host).to(self.device)          # copied before the call returns: any stream may read it
         at = np.cumsum([0] + [p.size for p in parts])
