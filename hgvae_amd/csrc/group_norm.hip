@@ -12,8 +12,9 @@
 //
 // Two ways to run:  graphs whose columns of one slab (whole groups, 32 columns or more) fit into the registers of a workgroup
 // are read once (k_gn_small);  larger ones take a pass for the sums over row chunks, a small pass that joins them per graph and
-// a pass that applies them.  The second read of those comes from the 256 MB memory-side cache: the graphs are taken in batches
-// that fit into it.
+// a pass that applies them.  Bound by memory: 3 passes over the matrix forward (2 would be the least), 5 backward (3).  Taking the
+// graphs in batches of 48 ... 192 MB, so that the second read meets the memory-side cache, was measured and is slower (1.78 ... 1.37
+// against 1.23 ms for 1.28 M x 138 forward and backward): the ends of the many short launches cost more than the cache brings.
 #include "pack8.h"
 
 namespace {
@@ -51,7 +52,7 @@ struct GnArgs {
     const int32_t* first_chunk;       // [listed + 1] first chunk of the k-th graph of that order
     float* out; int64_t ldo;          // out or gx
     double* mean; float* rstd;        // [B, groups]
-    double2* part;                    // [chunk of the batch][C] sums over a chunk's rows
+    double2* part;                    // [chunk][C] sums over a chunk's rows, from the first chunk of a larger graph on
     double2* colsum;                  // [rows of colsum][C] column sums (dz * xh, dz): one row per small workgroup, then per large graph
     float2* gsum;                     // [B, groups] mean(a), mean(a * xh)
     int n_small, slab, nslabs, pad;   // pad: columns behind the last one that rows of out have for 16-byte access (zeroed)
@@ -142,14 +143,18 @@ __global__ __launch_bounds__(NT) void k_gn_small(const GnArgs a) {
         float x[R], g[R];
         double s1 = 0.0, s2 = 0.0;
         if (active) {
+            const float* px = Q8 ? nullptr : a.x + (r0 + ty) * a.ldx + col;
+            const float* pg = BWD ? a.g + (r0 + ty) * a.ldg + col : nullptr;
 #pragma unroll
             for (int i = 0; i < R; ++i) {
                 const int r = ty + i * ty_n;
                 x[i] = 0.f;
                 if (r < n) {
-                    x[i] = Q8 ? value8(a, r0 + r, col) : a.x[(r0 + r) * a.ldx + col];
-                    if (BWD) g[i] = a.g[(r0 + r) * a.ldg + col];
+                    x[i] = Q8 ? value8(a, r0 + r, col) : *px;
+                    if (BWD) g[i] = *pg;
                 }
+                if (!Q8) px += ty_n * a.ldx;
+                if (BWD) pg += ty_n * a.ldg;
             }
         }
         Mean2 m; float rs;
@@ -331,10 +336,10 @@ __global__ __launch_bounds__(256) void k_gn_sums(const GnArgs a, const int chunk
 // One workgroup per (large graph, slab of whole groups): adds the sums of the graph's chunks and forms the group's statistics
 // (forward) or the two means of the backward pass and the graph's row of column sums.
 template <bool BWD>
-__global__ __launch_bounds__(1024) void k_gn_join(const GnArgs a, const int k0, const int chunk0, const int colrow0) {
+__global__ __launch_bounds__(1024) void k_gn_join(const GnArgs a, const int chunk0, const int colrow0) {
     __shared__ double2 red[1024];
     __shared__ double2 grp[1024];
-    const int k = k0 + blockIdx.x, graph = a.order[k];
+    const int k = a.n_small + blockIdx.x, graph = a.order[k];
     const int ch0 = a.first_chunk[k] - chunk0, ch1 = a.first_chunk[k + 1] - chunk0;
     const double count = (double)(a.ptr[graph + 1] - a.ptr[graph]) * a.per;
     const int c0 = blockIdx.y * a.slab, sc = min(a.slab, a.C - c0);
@@ -413,7 +418,7 @@ __global__ __launch_bounds__(256) void k_gn_apply(const GnArgs a, const int chun
             m1[i] = t.x; m2[i] = t.y;
         }
     }
-#pragma unroll 2
+#pragma unroll 1
     for (int n = ch.y + l.ty; n < ch.z; n += l.ty_n) {
         float v[VEC], o[VEC];
         load_x<VEC, Q8>(a, n, l.c, v);
@@ -469,7 +474,7 @@ __global__ __launch_bounds__(1024) void k_gn_affine(const double2* __restrict__ 
 }
 
 // ---- host side --------------------------------------------------------------------------------------------------------
-constexpr int SMALL_R = 32;                                     // rows that a thread of k_gn_small holds
+constexpr int SMALL_R = 16;                                     // rows that a thread of k_gn_small holds
 constexpr int SMALL_WGS = 2048;                                 // workgroups of it per slab
 
 int gn_slab(int C, int per) {                                   // whole groups, at least 32 columns
@@ -483,12 +488,14 @@ int gn_small_rows(int C, int per) {
 }
 
 template <int ACT, bool BWD, bool Q8>
-int gn_launch(const GnArgs& a, int listed, int small_rows, int n_batches, const int64_t* batches, float* gw, float* gb, hipStream_t stream) {
+int gn_launch(const GnArgs& a, int listed, int small_rows, int chunk0, int chunk1, float* gw, float* gb, hipStream_t stream) {
     const int small_wgs = min(a.n_small, SMALL_WGS);
     if (a.n_small > 0) {
         const dim3 grid((unsigned)small_wgs, (unsigned)a.nslabs);
         if (a.slab <= 256 && small_rows <= 256 / a.slab * SMALL_R)
             hipLaunchKernelGGL((k_gn_small<256, SMALL_R, ACT, BWD, Q8>), grid, dim3(256), 0, stream, a);
+        else if (a.slab <= 512 && small_rows <= 512 / a.slab * SMALL_R)
+            hipLaunchKernelGGL((k_gn_small<512, SMALL_R, ACT, BWD, Q8>), grid, dim3(512), 0, stream, a);
         else
             hipLaunchKernelGGL((k_gn_small<1024, SMALL_R, ACT, BWD, Q8>), grid, dim3(1024), 0, stream, a);
     }
@@ -496,17 +503,15 @@ int gn_launch(const GnArgs& a, int listed, int small_rows, int n_batches, const 
                      (!BWD || (hgv_aligned(a.g, 16) && a.ldg % 4 == 0 && a.ldg >= (a.C + 3) / 4 * 4)) &&
                      (!a.out || (hgv_aligned(a.out, 16) && a.ldo % 4 == 0 && a.ldo >= (a.C + 3) / 4 * 4));
     const unsigned slabs = (unsigned)hgv_cdiv(a.C, vec ? 1024 : 256);
-    for (int i = 0; i < n_batches; ++i) {
-        const int k0 = (int)batches[2 * i], k1 = (int)batches[2 * i + 2], ch0 = (int)batches[2 * i + 1], ch1 = (int)batches[2 * i + 3];
-        if (k1 <= k0 || ch1 <= ch0) continue;
-        const dim3 grid((unsigned)(ch1 - ch0), slabs);
-        if (vec) hipLaunchKernelGGL((k_gn_sums<4, ACT, BWD, Q8>), grid, dim3(256), 0, stream, a, ch0);
-        else hipLaunchKernelGGL((k_gn_sums<1, ACT, BWD, Q8>), grid, dim3(256), 0, stream, a, ch0);
-        hipLaunchKernelGGL(k_gn_join<BWD>, dim3((unsigned)(k1 - k0), (unsigned)a.nslabs), dim3(1024), 0, stream, a, k0, ch0,
-                           small_wgs + k0 - a.n_small);
+    if (listed > a.n_small) {
+        const dim3 grid((unsigned)(chunk1 - chunk0), slabs);
+        if (vec) hipLaunchKernelGGL((k_gn_sums<4, ACT, BWD, Q8>), grid, dim3(256), 0, stream, a, chunk0);
+        else hipLaunchKernelGGL((k_gn_sums<1, ACT, BWD, Q8>), grid, dim3(256), 0, stream, a, chunk0);
+        hipLaunchKernelGGL(k_gn_join<BWD>, dim3((unsigned)(listed - a.n_small), (unsigned)a.nslabs), dim3(1024), 0, stream, a, chunk0,
+                           small_wgs);
         if (a.out) {
-            if (vec) hipLaunchKernelGGL((k_gn_apply<4, ACT, BWD, Q8>), grid, dim3(256), 0, stream, a, ch0);
-            else hipLaunchKernelGGL((k_gn_apply<1, ACT, BWD, Q8>), grid, dim3(256), 0, stream, a, ch0);
+            if (vec) hipLaunchKernelGGL((k_gn_apply<4, ACT, BWD, Q8>), grid, dim3(256), 0, stream, a, chunk0);
+            else hipLaunchKernelGGL((k_gn_apply<1, ACT, BWD, Q8>), grid, dim3(256), 0, stream, a, chunk0);
         }
     }
     if (BWD && a.colsum)
@@ -516,13 +521,12 @@ int gn_launch(const GnArgs& a, int listed, int small_rows, int n_batches, const 
     return HGV_OK;
 }
 
-int gn_check(const GnArgs& a, int num_graphs, int listed, int n_small, int small_rows, int n_batches, const int64_t* batches, const char* what) {
+int gn_check(const GnArgs& a, int num_graphs, int listed, int n_small, int small_rows, int chunk0, int chunk1, const char* what) {
     HGV_REQUIRE(a.C > 0 && a.groups > 0 && a.C % a.groups == 0, HGV_EINVAL, "%s: %d columns in %d groups", what, a.C, a.groups);
-    HGV_REQUIRE(listed >= 0 && listed <= num_graphs && n_small >= 0 && n_small <= listed && n_batches >= 0, HGV_EINVAL, "%s: bad graph counts", what);
+    HGV_REQUIRE(listed >= 0 && listed <= num_graphs && n_small >= 0 && n_small <= listed && chunk0 >= 0 && chunk1 - chunk0 >= listed - n_small, HGV_EINVAL, "%s: bad graph counts", what);
     HGV_REQUIRE(a.ptr && a.order && a.chunks && a.first_chunk && a.mean && a.rstd, HGV_EINVAL, "%s: null buffer", what);
     HGV_REQUIRE(n_small == 0 || small_rows <= gn_small_rows(a.C, a.per), HGV_EINVAL,
                 "%s: graphs of %d rows do not fit the one-read kernel", what, small_rows);
-    HGV_REQUIRE(n_batches == 0 || batches, HGV_EINVAL, "%s: null batch list", what);
     HGV_REQUIRE(hgv_cdiv(a.C, 256) <= 65535, HGV_EUNSUPPORTED, "%s: too many columns", what);
     return HGV_OK;
 }
@@ -533,8 +537,8 @@ extern "C" int hgv_group_norm_small_rows(int C, int groups) {
     return C > 0 && groups > 0 && C % groups == 0 ? gn_small_rows(C, C / groups) : 0;
 }
 
-extern "C" size_t hgv_group_norm_ws(int64_t batch_chunks, int num_graphs, int listed, int n_small, int C, int groups, int backward) {
-    size_t n = hgv_align256((size_t)batch_chunks * C * sizeof(double2));
+extern "C" size_t hgv_group_norm_ws(int64_t n_chunks, int num_graphs, int listed, int n_small, int C, int groups, int backward) {
+    size_t n = hgv_align256((size_t)n_chunks * C * sizeof(double2));
     if (backward) {
         n += hgv_align256((size_t)(min(n_small, SMALL_WGS) + listed - n_small) * C * sizeof(double2));
         n += hgv_align256((size_t)num_graphs * groups * sizeof(float2));
@@ -544,41 +548,39 @@ extern "C" size_t hgv_group_norm_ws(int64_t batch_chunks, int num_graphs, int li
 
 extern "C" int hgv_group_norm_fwd(const float* x, int64_t ldx, int C, int groups, int act, float eps, const float* w, const float* b,
                                   const int32_t* ptr, const int32_t* order, const int32_t* chunks, const int32_t* first_chunk,
-                                  int num_graphs, int listed, int n_small, int small_rows, int n_batches, const int64_t* batches, int64_t batch_chunks,
+                                  int num_graphs, int listed, int n_small, int small_rows, int chunk0, int chunk1,
                                   float* out, int64_t ldo, double* mean, float* rstd, void* ws, size_t ws_bytes, hipStream_t stream) {
     GnArgs a = {};
     a.x = x; a.ldx = ldx; a.C = C; a.groups = groups; a.per = groups > 0 ? C / groups : 0; a.eps = eps; a.w = w; a.b = b;
     a.ptr = ptr; a.order = order; a.chunks = (const int4*)chunks; a.first_chunk = first_chunk; a.out = out; a.ldo = ldo;
     a.mean = mean; a.rstd = rstd; a.n_small = n_small;
-    const int rc = gn_check(a, num_graphs, listed, n_small, small_rows, n_batches, batches, "group_norm_fwd");
+    const int rc = gn_check(a, num_graphs, listed, n_small, small_rows, chunk0, chunk1, "group_norm_fwd");
     if (rc) return rc;
     HGV_REQUIRE(x && out && ldx >= C && ldo >= C, HGV_EINVAL, "group_norm_fwd: null buffer or bad leading dimension");
-    HGV_REQUIRE(ws_bytes >= hgv_group_norm_ws(batch_chunks, num_graphs, listed, n_small, C, groups, 0) && hgv_aligned(ws, 256), HGV_EWORKSPACE,
+    HGV_REQUIRE(ws_bytes >= hgv_group_norm_ws(chunk1 - chunk0, num_graphs, listed, n_small, C, groups, 0) && hgv_aligned(ws, 256), HGV_EWORKSPACE,
                 "group_norm_fwd: workspace too small or misaligned");
-    for (int i = 0; i < n_batches; ++i)
-        HGV_REQUIRE(batches[2 * i + 3] - batches[2 * i + 1] <= batch_chunks, HGV_EWORKSPACE, "group_norm_fwd: a batch has more chunks than the workspace");
     a.pad = C % 4 && a.out && a.ldo >= (C + 3) / 4 * 4 ? 4 - C % 4 : 0;
     a.slab = gn_slab(C, a.per); a.nslabs = (int)hgv_cdiv(C, a.slab);
     HGV_REQUIRE(a.nslabs <= 65535, HGV_EUNSUPPORTED, "group_norm_fwd: too many columns");
     a.part = (double2*)ws;
     switch (act) {
-        case ACT_NONE: return gn_launch<ACT_NONE, false, false>(a, listed, small_rows, n_batches, batches, nullptr, nullptr, stream);
-        case ACT_RELU: return gn_launch<ACT_RELU, false, false>(a, listed, small_rows, n_batches, batches, nullptr, nullptr, stream);
-        case ACT_SILU: return gn_launch<ACT_SILU, false, false>(a, listed, small_rows, n_batches, batches, nullptr, nullptr, stream);
-        case ACT_GELU: return gn_launch<ACT_GELU, false, false>(a, listed, small_rows, n_batches, batches, nullptr, nullptr, stream);
+        case ACT_NONE: return gn_launch<ACT_NONE, false, false>(a, listed, small_rows, chunk0, chunk1, nullptr, nullptr, stream);
+        case ACT_RELU: return gn_launch<ACT_RELU, false, false>(a, listed, small_rows, chunk0, chunk1, nullptr, nullptr, stream);
+        case ACT_SILU: return gn_launch<ACT_SILU, false, false>(a, listed, small_rows, chunk0, chunk1, nullptr, nullptr, stream);
+        case ACT_GELU: return gn_launch<ACT_GELU, false, false>(a, listed, small_rows, chunk0, chunk1, nullptr, nullptr, stream);
     }
     hgv_set_error("group_norm_fwd: unknown activation %d", act);
     return HGV_EINVAL;
 }
 
 template <bool Q8>
-static int gn_bwd(int act, const GnArgs& a, int listed, int small_rows, int n_batches, const int64_t* batches, float* gw, float* gb,
+static int gn_bwd(int act, const GnArgs& a, int listed, int small_rows, int chunk0, int chunk1, float* gw, float* gb,
                   hipStream_t stream) {
     switch (act) {
-        case ACT_NONE: return gn_launch<ACT_NONE, true, Q8>(a, listed, small_rows, n_batches, batches, gw, gb, stream);
-        case ACT_RELU: return gn_launch<ACT_RELU, true, Q8>(a, listed, small_rows, n_batches, batches, gw, gb, stream);
-        case ACT_SILU: return gn_launch<ACT_SILU, true, Q8>(a, listed, small_rows, n_batches, batches, gw, gb, stream);
-        case ACT_GELU: return gn_launch<ACT_GELU, true, Q8>(a, listed, small_rows, n_batches, batches, gw, gb, stream);
+        case ACT_NONE: return gn_launch<ACT_NONE, true, Q8>(a, listed, small_rows, chunk0, chunk1, gw, gb, stream);
+        case ACT_RELU: return gn_launch<ACT_RELU, true, Q8>(a, listed, small_rows, chunk0, chunk1, gw, gb, stream);
+        case ACT_SILU: return gn_launch<ACT_SILU, true, Q8>(a, listed, small_rows, chunk0, chunk1, gw, gb, stream);
+        case ACT_GELU: return gn_launch<ACT_GELU, true, Q8>(a, listed, small_rows, chunk0, chunk1, gw, gb, stream);
     }
     hgv_set_error("group_norm_bwd: unknown activation %d", act);
     return HGV_EINVAL;
@@ -587,7 +589,7 @@ static int gn_bwd(int act, const GnArgs& a, int listed, int small_rows, int n_ba
 extern "C" int hgv_group_norm_bwd(const float* g, int64_t ldg, const float* x, int64_t ldx, const int8_t* q, int64_t ldq,
                                   const uint8_t* scale, int C, int groups, int act, const float* w, const float* b, const int32_t* ptr,
                                   const int32_t* order, const int32_t* chunks, const int32_t* first_chunk, int num_graphs, int listed,
-                                  int n_small, int small_rows, int n_batches, const int64_t* batches, int64_t batch_chunks, const double* mean,
+                                  int n_small, int small_rows, int chunk0, int chunk1, const double* mean,
                                   const float* rstd, float* gx, int64_t ldgx, float* gw, float* gb, void* ws, size_t ws_bytes,
                                   hipStream_t stream) {
     GnArgs a = {};
@@ -595,24 +597,22 @@ extern "C" int hgv_group_norm_bwd(const float* g, int64_t ldg, const float* x, i
     a.C = C; a.groups = groups; a.per = groups > 0 ? C / groups : 0; a.w = w; a.b = b;
     a.ptr = ptr; a.order = order; a.chunks = (const int4*)chunks; a.first_chunk = first_chunk; a.out = gx; a.ldo = ldgx;
     a.mean = (double*)mean; a.rstd = (float*)rstd; a.n_small = n_small;
-    const int rc = gn_check(a, num_graphs, listed, n_small, small_rows, n_batches, batches, "group_norm_bwd");
+    const int rc = gn_check(a, num_graphs, listed, n_small, small_rows, chunk0, chunk1, "group_norm_bwd");
     if (rc) return rc;
     HGV_REQUIRE(g && ldg >= C && (!gx || ldgx >= C) && (gx || gw || gb), HGV_EINVAL, "group_norm_bwd: null buffer or bad leading dimension");
     HGV_REQUIRE(q ? (scale && ldq >= C && ldq % 16 == 0 && hgv_aligned(q, 16)) : (x && ldx >= C), HGV_EINVAL,
                 "group_norm_bwd: needs x, or its 8-bit form");
-    HGV_REQUIRE(ws_bytes >= hgv_group_norm_ws(batch_chunks, num_graphs, listed, n_small, C, groups, 1) && hgv_aligned(ws, 256), HGV_EWORKSPACE,
+    HGV_REQUIRE(ws_bytes >= hgv_group_norm_ws(chunk1 - chunk0, num_graphs, listed, n_small, C, groups, 1) && hgv_aligned(ws, 256), HGV_EWORKSPACE,
                 "group_norm_bwd: workspace too small or misaligned");
-    for (int i = 0; i < n_batches; ++i)
-        HGV_REQUIRE(batches[2 * i + 3] - batches[2 * i + 1] <= batch_chunks, HGV_EWORKSPACE, "group_norm_bwd: a batch has more chunks than the workspace");
     a.pad = C % 4 && a.out && a.ldo >= (C + 3) / 4 * 4 ? 4 - C % 4 : 0;
     a.slab = gn_slab(C, a.per); a.nslabs = (int)hgv_cdiv(C, a.slab);
     HGV_REQUIRE(a.nslabs <= 65535, HGV_EUNSUPPORTED, "group_norm_bwd: too many columns");
     char* p = (char*)ws;
     a.part = (double2*)p;
-    p += hgv_align256((size_t)batch_chunks * C * sizeof(double2));
+    p += hgv_align256((size_t)(chunk1 - chunk0) * C * sizeof(double2));
     if (gw || gb) a.colsum = (double2*)p;
     p += hgv_align256((size_t)(min(n_small, SMALL_WGS) + listed - n_small) * C * sizeof(double2));
     a.gsum = (float2*)p;
-    return q ? gn_bwd<true>(act, a, listed, small_rows, n_batches, batches, gw, gb, stream)
-             : gn_bwd<false>(act, a, listed, small_rows, n_batches, batches, gw, gb, stream);
+    return q ? gn_bwd<true>(act, a, listed, small_rows, chunk0, chunk1, gw, gb, stream)
+             : gn_bwd<false>(act, a, listed, small_rows, chunk0, chunk1, gw, gb, stream);
 }

@@ -2584,13 +2584,13 @@ class _GroupNormAct(torch.autograd.Function):
         out = new_padded(n, c, x.device, zero_pad=False)
         mean = torch.empty(seg.num_graphs, groups, dtype=torch.float64, device=x.device)
         rstd = torch.empty(seg.num_graphs, groups, dtype=torch.float32, device=x.device)
-        small, rows, batches, n_batches, chunks = seg._norm_plan(lib.hgv_group_norm_small_rows(c, groups), 4 * ld_of(x))
+        small, rows, chunk0, chunk1 = seg._norm_plan(lib.hgv_group_norm_small_rows(c, groups))
         listed = len(seg._sorted)
-        nws = lib.hgv_group_norm_ws(chunks, seg.num_graphs, listed, small, c, groups, 0)
+        nws = lib.hgv_group_norm_ws(chunk1 - chunk0, seg.num_graphs, listed, small, c, groups, 0)
         ws = torch.empty(nws, dtype=torch.uint8, device=x.device)
         _lib.call("hgv_group_norm_fwd", x.data_ptr(), ld_of(x), c, groups, act, float(eps), _lib.ptr(w), _lib.ptr(b), seg._ptr.data_ptr(),
-                  seg._order.data_ptr(), seg._chunks.data_ptr(), seg._first.data_ptr(), seg.num_graphs, listed, small, rows, n_batches,
-                  batches, chunks, out.data_ptr(), out.stride(0), mean.data_ptr(), rstd.data_ptr(), ws.data_ptr(), nws, _lib.stream())
+                  seg._order.data_ptr(), seg._chunks.data_ptr(), seg._first.data_ptr(), seg.num_graphs, listed, small, rows, chunk0,
+                  chunk1, out.data_ptr(), out.stride(0), mean.data_ptr(), rstd.data_ptr(), ws.data_ptr(), nws, _lib.stream())
         ctx.seg, ctx.cfg = seg, (groups, act)
         ctx.packed = None
         if keep8 and any(ctx.needs_input_grad[:3]):
@@ -2615,15 +2615,14 @@ class _GroupNormAct(torch.autograd.Function):
             gx = new_padded(n, c, g.device, zero_pad=False) if need[0] else None
             gw = torch.empty(c, dtype=torch.float32, device=g.device) if need[1] else None
             gb = torch.empty(c, dtype=torch.float32, device=g.device) if need[2] else None
-            row_bytes = 4 * ld_of(g) + (4 * ld_of(x) if x is not None else q.stride(0))
-            small, rows, batches, n_batches, chunks = seg._norm_plan(lib.hgv_group_norm_small_rows(c, groups), row_bytes)
+            small, rows, chunk0, chunk1 = seg._norm_plan(lib.hgv_group_norm_small_rows(c, groups))
             listed = len(seg._sorted)
-            nws = lib.hgv_group_norm_ws(chunks, seg.num_graphs, listed, small, c, groups, 1)
+            nws = lib.hgv_group_norm_ws(chunk1 - chunk0, seg.num_graphs, listed, small, c, groups, 1)
             ws = torch.empty(nws, dtype=torch.uint8, device=g.device)
             _lib.call("hgv_group_norm_bwd", g.data_ptr(), ld_of(g), _lib.ptr(x), ld_of(x) if x is not None else 0, _lib.ptr(q),
                       q.stride(0) if q is not None else 0, _lib.ptr(scale), c, groups, act, _lib.ptr(w), _lib.ptr(b), seg._ptr.data_ptr(),
                       seg._order.data_ptr(), seg._chunks.data_ptr(), seg._first.data_ptr(), seg.num_graphs, listed, small, rows,
-                      n_batches, batches, chunks, mean.data_ptr(), rstd.data_ptr(), _lib.ptr(gx), gx.stride(0) if gx is not None else 0,
+                      chunk0, chunk1, mean.data_ptr(), rstd.data_ptr(), _lib.ptr(gx), gx.stride(0) if gx is not None else 0,
                       _lib.ptr(gw), _lib.ptr(gb), ws.data_ptr(), nws, _lib.stream())
         return gx, gw, gb, None, None, None, None, None
 

@@ -280,15 +280,16 @@ class Segments:
         order = np.argsort(sizes, kind="stable")
         order = order[int((sizes == 0).sum()):]
         self._sorted = sizes[order].tolist()
-        # row chunks of the sum / apply passes: about 2 048 of them in all, 32 to 512 rows each, at most 512 per graph
-        rows = min(max(-(-self.num_rows // 2048), 32), 512)
+        # row chunks of the norm's passes: 64 rows (32 where that leaves fewer than 2 048 of them), at most 512 per graph
+        rows = 64 if self.num_rows >= 64 * 2048 else 32
         per = np.maximum(rows, -(-sizes[order] // 512))
         counts = -(-sizes[order] // per)
-        self._first_chunk = np.zeros(order.size + 1, dtype=np.int64)
-        np.cumsum(counts, out=self._first_chunk[1:])
-        total = int(self._first_chunk[-1])
+        first = np.zeros(order.size + 1, dtype=np.int64)
+        np.cumsum(counts, out=first[1:])
+        total = int(first[-1])
+        self._first_host = first.tolist()
         which = np.repeat(np.arange(order.size), counts)
-        start = ptr[order][which] + (np.arange(total) - self._first_chunk[which]) * per[which]
+        start = ptr[order][which] + (np.arange(total) - first[which]) * per[which]
         chunks = np.zeros((total, 4), dtype=np.int64)
         chunks[:, 0], chunks[:, 1] = order[which], start
         chunks[:, 2] = np.minimum(start + per[which], ptr[order + 1][which])
@@ -296,12 +297,11 @@ class Segments:
         # and of 128 rows, those of the largest graphs first
         tiles, blocks = self._tiles_of(sizes, ptr, np.flatnonzero(sizes), 64), [self._tiles_of(sizes, ptr, order[::-1], r) for r in (64, 128)]
         self._n_tiles, self._n_blocks = len(tiles), [len(b) for b in blocks]
-        parts = [chunks.ravel(), tiles.ravel(), np.concatenate(blocks).ravel(), ptr, order, self._first_chunk]
+        parts = [chunks.ravel(), tiles.ravel(), np.concatenate(blocks).ravel(), ptr, order, first]
         host = np.concatenate(parts).astype(np.int32)
         self._buf = torch.from_numpy(host).to(self.device)          # copied before the call returns: any stream may read it
         at = np.cumsum([0] + [p.size for p in parts])
         self._chunks, self._tiles, self._blocks, self._ptr, self._order, self._first = (self._buf[at[i]:at[i + 1]] for i in range(6))
-        self._norm_plans: "dict[tuple, tuple]" = {}
 
     @staticmethod
     def _tiles_of(sizes, ptr, graphs, rows: int) -> np.ndarray:
@@ -345,31 +345,12 @@ class Segments:
             count = int(num_graphs)
         return cls(np.bincount(host, minlength=count) if host.size else np.zeros(count, dtype=np.int64), batch.device)
 
-    def _norm_plan(self, small_rows: int, row_bytes: int):
-        """(graphs that one workgroup reads at once, rows of the largest of them, batches of the others as a host array of
-        (first graph, first chunk) pairs, their number, chunks of the largest batch).  A batch is what the memory-side
-        cache holds between the two passes over it."""
-        key = (small_rows, row_bytes)
-        plan = self._norm_plans.get(key)
-        if plan is None:
-            n_small = bisect.bisect_right(self._sorted, small_rows)
-            limit, cur, marks, most = 96 << 20, 0, [], 0
-            for k in range(n_small, len(self._sorted)):
-                size = self._sorted[k] * row_bytes
-                if not marks or cur + size > limit:
-                    marks.append(k)
-                    cur = 0
-                cur += size
-            marks.append(len(self._sorted))
-            pairs = []
-            for i, k in enumerate(marks):
-                pairs += [k, int(self._first_chunk[k])]
-                if i:
-                    most = max(most, pairs[-1] - pairs[-3])
-            import ctypes
-            plan = (n_small, self._sorted[n_small - 1] if n_small else 0, (ctypes.c_int64 * len(pairs))(*pairs), len(marks) - 1, most)
-            self._norm_plans[key] = plan
-        return plan
+    def _norm_plan(self, small_rows: int):
+        """(graphs that one workgroup reads at once, rows of the largest of them, first chunk of the others, end of the chunks)."""
+        n = bisect.bisect_right(self._sorted, small_rows)
+        if n < len(self._sorted) and 8 * sum(self._sorted[:n]) < self.num_rows:
+            n = 0                       # a few small graphs beside large ones: not worth a launch of their own
+        return n, self._sorted[n - 1] if n else 0, self._first_host[n], self._first_host[-1]
 
     def __repr__(self):
         return f"Segments({self.num_graphs} graphs, {self.num_rows} rows, {self.device})"

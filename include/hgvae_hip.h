@@ -579,21 +579,19 @@ int hgv_unpack8(const int8_t* q, int64_t ldq, const uint8_t* scale, int64_t N, i
  *   out = act((x - mean) * rstd * w + b),  act: 0 none, 1 relu, 2 x * sigmoid(x), 3 gelu (erf).   w, b [C] may be NULL (1, 0).
  * Graphs: ptr [num_graphs + 1] first rows; order [listed] the graphs that have rows, by size; chunks [*][4] (graph, row, end
  * row, unused) of the listed graphs in that order; first_chunk [listed + 1].  The first n_small graphs of the list (none
- * above small_rows <= hgv_group_norm_small_rows(C, groups) rows) are read once; the others are taken in n_batches batches:
- * batches (a HOST array) holds n_batches + 1 pairs (graph of the list, its first chunk), none with more than batch_chunks chunks.
+ * above small_rows <= hgv_group_norm_small_rows(C, groups) rows) are read once; the others take chunks chunk0 .. chunk1 - 1.
  * mean [num_graphs, groups] fp64 and rstd [num_graphs, groups] are written by the forward and read by the backward pass
  * (entries of graphs without rows are left as they were).
  * Backward: from x, or (q != NULL) from its 8-bit form; gx, gw [C], gb [C] are written where not NULL. */
 int hgv_group_norm_small_rows(int C, int groups);
-size_t hgv_group_norm_ws(int64_t batch_chunks, int num_graphs, int listed, int n_small, int C, int groups, int backward);
+size_t hgv_group_norm_ws(int64_t n_chunks, int num_graphs, int listed, int n_small, int C, int groups, int backward);
 int hgv_group_norm_fwd(const float* x, int64_t ldx, int C, int groups, int act, float eps, const float* w, const float* b,
                        const int32_t* ptr, const int32_t* order, const int32_t* chunks, const int32_t* first_chunk, int num_graphs,
-                       int listed, int n_small, int small_rows, int n_batches, const int64_t* batches, int64_t batch_chunks, float* out,
-                       int64_t ldo, double* mean, float* rstd, void* ws, size_t ws_bytes, hgv_stream_t stream);
+                       int listed, int n_small, int small_rows, int chunk0, int chunk1, float* out, int64_t ldo, double* mean, float* rstd, void* ws, size_t ws_bytes, hgv_stream_t stream);
 int hgv_group_norm_bwd(const float* g, int64_t ldg, const float* x, int64_t ldx, const int8_t* q, int64_t ldq, const uint8_t* scale,
                        int C, int groups, int act, const float* w, const float* b, const int32_t* ptr, const int32_t* order,
                        const int32_t* chunks, const int32_t* first_chunk, int num_graphs, int listed, int n_small, int small_rows,
-                       int n_batches, const int64_t* batches, int64_t batch_chunks, const double* mean, const float* rstd, float* gx,
+                       int chunk0, int chunk1, const double* mean, const float* rstd, float* gx,
                        int64_t ldgx, float* gw, float* gb, void* ws, size_t ws_bytes, hgv_stream_t stream);
 
 /* ---- attention among the nodes of each graph (no reference counterpart: its attention runs along edges, GATConv at
