@@ -151,6 +151,8 @@ SIGNATURES = {
                                           _i32, _i32, _f32, _vp, _vp, _vp, _i32, _vp, _i32, _i32, _vp, _vp, _vp, _vp, _sz, _vp]),
     "hgv_pack8": (C.c_int, [_vp, _i64, _i64, _i32, _vp, _i64, _vp, _vp]),
     "hgv_unpack8": (C.c_int, [_vp, _i64, _vp, _i64, _i32, _vp, _i64, _vp]),
+    "hgv_gemm_tn8_ws": (_sz, [_i64, _i32, _i32]),
+    "hgv_gemm_tn8": (C.c_int, [_vp, _i64, _i32, _vp, _i64, _vp, _i32, _i64, _vp, _i64, _vp, _vp, _sz, _vp]),
     "hgv_group_norm_small_rows": (C.c_int, [_i32, _i32]),
     "hgv_group_norm_ws": (_sz, [_i64, _i32, _i32, _i32, _i32, _i32, _i32]),
     "hgv_group_norm_fwd": (C.c_int, [_vp, _i64, _i32, _i32, _i32, _f32, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32,

@@ -127,3 +127,220 @@ extern "C" int hgv_unpack8(const int8_t* q, int64_t ldq, const uint8_t* scale, i
     HGV_CHECK_LAUNCH("unpack8");
     return HGV_OK;
 }
+
+// ---- weight gradient from the 8-bit form -----------------------------------------------------------------------------------------
+// GW[N, K] = G^T V, V the values of an 8-bit matrix, with the column sums of G as the bias gradient.  V is exact in bf16, so three
+// bf16 pieces of G (8 bits each, cut: together all 24) make the product exact up to its fp32 accumulation: three piece products
+// where two fp32 operands take six.
+//
+// A workgroup of nine waves takes 144 x 144 outputs over every sets-th tile of 32 rows: G is split and V widened on the way into
+// LDS (row-major, 288 bytes per row, which spreads the eight rows of a transposing load over all banks), two buffers, the next
+// tile's loads in flight during the products.  Wave w owns columns 16 w .. of G and all columns of V; the column sums are a product
+// with a tile of ones.  Partial sums are added in fp64 in a fixed order by k_tn8_reduce.
+// 1.28 M rows, 138 x 138: 260 us = 3.4 TB/s (the six-product kernel over the unpacked matrix: 400, and 165 for unpacking).  Matrix
+// cores 30 %, vector units 36 %, LDS 21 % of the time: splitting, LDS and products of a tile follow one another behind one barrier.
+// Measured without effect: two workgroups per unit, two to four tiles in flight, half of the waves splitting behind their products.
+namespace {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int T8_ROWS = 32, T8_W = 144, T8_LINE = 2 * T8_W, T8_PIECE = T8_ROWS * T8_LINE, T8_BUF = 4 * T8_PIECE, T8_LDS = 2 * T8_BUF + T8_ROWS * 32, T8_THREADS = 576;
+constexpr int T8_SET = (81 + 9) * 256;                          // floats of a partial set: 81 tiles, nine tiles of column sums
+
+struct Tn8Args {
+    const float* G; int64_t ldg; int N;
+    const int8_t* q; int64_t ldq; const uint8_t* scale; int nb, K;
+    int64_t M, steps;
+    int ngrps, kgrps, sets;
+    float* partial;                                             // [n group][k group][set][T8_SET]
+};
+
+__device__ __forceinline__ uint2 t8_pack(const uint32_t b[4]) {  // upper halves of four floats
+    return make_uint2(__builtin_amdgcn_perm(b[1], b[0], 0x07060302u), __builtin_amdgcn_perm(b[3], b[2], 0x07060302u));
+}
+
+__device__ __forceinline__ bf16x8 t8_read(const unsigned char* p, int line = T8_LINE) {
+    typedef __attribute__((address_space(3))) s16x4 lds_v;
+    union { struct { s16x4 a, b; } s; bf16x8 v; } u;
+    u.s.a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v*)p);
+    u.s.b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v*)(p + 16 * line));
+    return u.v;
+}
+
+__global__ __launch_bounds__(T8_THREADS, 5) void k_gemm_tn8(const Tn8Args a) {
+    extern __shared__ __align__(16) unsigned char t8_lds[];
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    const int per = a.ngrps * a.kgrps, grp = blockIdx.x % per, set = blockIdx.x / per;
+    const int ng = grp / a.kgrps, kg = grp - ng * a.kgrps;
+    const int n0 = T8_W * ng, k0 = T8_W * kg, n_w = min(T8_W, a.N - n0), k_w = min(T8_W, a.K - k0);
+    const int64_t lo = set, hi = a.steps, by_n = a.sets;
+    const int nt = (n_w + 15) / 16, kt = (k_w + 15) / 16;
+    // this thread's two quads of the tile: the same four columns, 16 rows apart
+    const int row = t / 36, c = 4 * (t - 36 * row);
+    const bool g_live = c < n_w, v_live = c < k_w;
+    // one offset per lane; what depends on the tile is uniform
+    const uint32_t go = (uint32_t)(row * a.ldg + c), qo = (uint32_t)(row * a.ldq + c), so = (uint32_t)(row * a.nb + ((k0 + c) >> 5));
+    float4 g[2];
+    uint32_t w[2];
+    int by[2];
+    auto load = [&](int64_t s) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int64_t n = s * T8_ROWS + 16 * i;
+            const float* gp = a.G + n * a.ldg + n0;
+            const int8_t* qp = a.q + n * a.ldq + k0;
+            const uint8_t* sp = a.scale + n * a.nb;
+            g[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+            w[i] = 0; by[i] = 127;
+            if (n + row < a.M) {
+                if (g_live) g[i] = *(const float4*)(gp + go);
+                if (v_live) {
+                    w[i] = *(const uint32_t*)(qp + qo);
+                    by[i] = sp[so];
+                }
+            }
+        }
+    };
+    auto put = [&](int b) __attribute__((always_inline)) {
+        unsigned char* base = t8_lds + b * T8_BUF + row * T8_LINE + 2 * c;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const float x[4] = {g[i].x, g[i].y, g[i].z, g[i].w};
+            uint32_t p[3][4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                p[0][e] = __float_as_uint(x[e]);
+                const float r = x[e] - __uint_as_float(p[0][e] & 0xffff0000u);          // exact
+                p[1][e] = __float_as_uint(r);
+                p[2][e] = __float_as_uint(r - __uint_as_float(p[1][e] & 0xffff0000u));  // exact, eight bits left
+            }
+            float v[4];
+            p8_values4(w[i], by[i], v);
+            const uint32_t vb[4] = {__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
+            unsigned char* at = base + 16 * i * T8_LINE;
+#pragma unroll
+            for (int j = 0; j < 3; ++j) *(uint2*)(at + j * T8_PIECE) = t8_pack(p[j]);
+            *(uint2*)(at + 3 * T8_PIECE) = t8_pack(vb);
+        }
+    };
+    f32x4 acc[9], accb = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < 9; ++k) acc[k] = f32x4{0.f, 0.f, 0.f, 0.f};
+    // a tile of ones behind the two buffers, for the column sums
+    for (int i = t; i < T8_ROWS * 4; i += T8_THREADS) *(uint2*)(t8_lds + 2 * T8_BUF + i * 8) = make_uint2(0x3f803f80u, 0x3f803f80u);
+    const int i16 = lane & 15;
+    const int at = (4 * (lane >> 4) + (i16 >> 2)) * T8_LINE + (i16 & 3) * 8;
+    if (lo < hi) {
+        load(lo);
+        put(0);
+        if (lo + by_n < hi) load(lo + by_n);
+    }
+    __syncthreads();
+    int b = 0;
+    for (int64_t s = lo; s < hi; s += by_n, b ^= 1) {
+        if (s + by_n < hi) {
+            put(b ^ 1);
+            if (s + 2 * by_n < hi) load(s + 2 * by_n);
+        }
+        if (wave < nt) {
+            const unsigned char* base = t8_lds + b * T8_BUF + at;
+            bf16x8 gf[3];
+#pragma unroll
+            for (int j = 0; j < 3; ++j) gf[j] = t8_read(base + j * T8_PIECE + wave * 32);
+#pragma unroll
+            for (int k = 0; k < 9; ++k)
+                if (k < kt) {
+                    const bf16x8 v = t8_read(base + 3 * T8_PIECE + k * 32);
+#pragma unroll
+                    for (int j = 2; j >= 0; --j) acc[k] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(gf[j], v, acc[k], 0, 0, 0);
+                }
+            if (kg == 0) {
+                const bf16x8 ones = t8_read(t8_lds + 2 * T8_BUF + (4 * (lane >> 4) + (i16 >> 2)) * 32 + (i16 & 3) * 8, 32);
+#pragma unroll
+                for (int j = 2; j >= 0; --j) accb = __builtin_amdgcn_mfma_f32_16x16x32_bf16(gf[j], ones, accb, 0, 0, 0);
+            }
+        }
+        __syncthreads();
+    }
+    if (wave < nt) {
+        float* out = a.partial + ((int64_t)grp * a.sets + set) * T8_SET + lane * 4;
+#pragma unroll
+        for (int k = 0; k < 9; ++k)
+            if (k < kt) *(f32x4*)(out + (wave * 9 + k) * 256) = acc[k];
+        if (kg == 0) *(f32x4*)(out + (81 + wave) * 256) = accb;
+    }
+}
+
+// One workgroup per 64 floats of a tile: 16 threads' worth of sets per float, added in a fixed order.
+__global__ __launch_bounds__(1024) void k_tn8_reduce(const float* __restrict__ partial, const int sets, const int ngrps, const int kgrps, const int N,
+                                                     const int K, float* __restrict__ GW, const int64_t ldgw, float* __restrict__ gbias) {
+    __shared__ double red[1024];
+    const int grp = blockIdx.y, ng = grp / kgrps, kg = grp - ng * kgrps;
+    const int tile = blockIdx.x >> 2, part = blockIdx.x & 3;
+    const bool bias = tile >= 81;
+    const int tn = bias ? tile - 81 : tile / 9, tk = bias ? 0 : tile - 9 * tn;
+    const int n0 = T8_W * ng + 16 * tn, k0 = T8_W * kg + 16 * tk;
+    if (n0 >= N || (bias ? kg != 0 || !gbias : k0 >= K) || 16 * tn >= T8_W) return;      // the whole workgroup
+    const int e = threadIdx.x & 63, j = threadIdx.x >> 6;
+    const float* p = partial + (int64_t)grp * sets * T8_SET + tile * 256 + part * 64 + e;
+    double s = 0.0;
+#pragma unroll 8
+    for (int i = j; i < sets; i += 16) s += (double)p[(int64_t)i * T8_SET];
+    red[threadIdx.x] = s;
+    for (int o = 8; o > 0; o >>= 1) {
+        __syncthreads();
+        if (j < o) red[threadIdx.x] += red[threadIdx.x + 64 * o];
+    }
+    if (j > 0) return;
+    const int f = part * 64 + e, lane = f >> 2;                 // lane and register of the product's result
+    const int n = n0 + 4 * (lane >> 4) + (f & 3), k = k0 + (lane & 15);
+    if (n >= N) return;
+    if (bias) {
+        if ((lane & 15) == 0) gbias[n] = (float)red[e];
+    } else if (k < K) {
+        GW[(int64_t)n * ldgw + k] = (float)red[e];
+    }
+}
+
+int tn8_sets(int64_t M, int per) {
+    const int64_t steps = hgv_cdiv(M, T8_ROWS);
+    // one workgroup per compute unit, at least four tiles each
+    return (int)max((int64_t)1, min((int64_t)max(256 / per, 1), steps / 4));
+}
+
+}  // namespace
+
+extern "C" size_t hgv_gemm_tn8_ws(int64_t M, int N, int K) {
+    if (M <= 0 || N <= 0 || K <= 0) return 0;
+    const int per = (int)(hgv_cdiv(N, T8_W) * hgv_cdiv(K, T8_W));
+    return hgv_align256((size_t)per * tn8_sets(M, per) * T8_SET * sizeof(float));
+}
+
+extern "C" int hgv_gemm_tn8(const float* G, int64_t ldg, int N, const int8_t* q, int64_t ldq, const uint8_t* scale, int K, int64_t M, float* GW,
+                            int64_t ldgw, float* gbias, void* ws, size_t ws_bytes, hipStream_t stream) {
+    HGV_REQUIRE(M > 0 && N > 0 && K > 0, HGV_EINVAL, "gemm_tn8: bad sizes");
+    HGV_REQUIRE(G && q && scale && GW && hgv_aligned(G, 16) && ldg % 4 == 0 && ldg >= (N + 3) / 4 * 4 && ldq >= K && ldq % 16 == 0 &&
+                hgv_aligned(q, 16) && ldgw >= K, HGV_EINVAL, "gemm_tn8: null / misaligned buffer or bad leading dimension");
+    HGV_REQUIRE(N <= 65536 && K <= 65536, HGV_EUNSUPPORTED, "gemm_tn8: widths above 65536");
+    HGV_REQUIRE(ws && ws_bytes >= hgv_gemm_tn8_ws(M, N, K) && hgv_aligned(ws, 256), HGV_EWORKSPACE, "gemm_tn8: workspace too small or misaligned");
+    Tn8Args a = {};
+    a.G = G; a.ldg = ldg; a.N = N; a.q = q; a.ldq = ldq; a.scale = scale; a.nb = (K + 31) / 32; a.K = K; a.M = M;
+    a.steps = hgv_cdiv(M, T8_ROWS); a.ngrps = (int)hgv_cdiv(N, T8_W); a.kgrps = (int)hgv_cdiv(K, T8_W);
+    const int per = a.ngrps * a.kgrps;
+    a.sets = tn8_sets(M, per); a.partial = (float*)ws;
+    HGV_REQUIRE(per <= 65535, HGV_EUNSUPPORTED, "gemm_tn8: widths not supported");
+    static bool raised[64] = {false};
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) dev = 0;
+    if (!raised[dev]) {
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(k_gemm_tn8), hipFuncAttributeMaxDynamicSharedMemorySize, T8_LDS);
+        HGV_REQUIRE(e == hipSuccess, HGV_ELAUNCH, "gemm_tn8: cannot raise the dynamic LDS limit: %s", hipGetErrorString(e));
+        raised[dev] = true;
+    }
+    hipLaunchKernelGGL(k_gemm_tn8, dim3((unsigned)(per * a.sets)), dim3(T8_THREADS), T8_LDS, stream, a);
+    hipLaunchKernelGGL(k_tn8_reduce, dim3(90 * 4, (unsigned)per), dim3(1024), 0, stream, a.partial, a.sets, a.ngrps, a.kgrps, N, K, GW, ldgw, gbias);
+    HGV_CHECK_LAUNCH("gemm_tn8");
+    return HGV_OK;
+}

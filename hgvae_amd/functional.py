@@ -2546,7 +2546,14 @@ class _Linear8(torch.autograd.Function):
 
 def _weight_grad8(g: torch.Tensor, x8: Packed8, want_bias: bool):
     """(g^T v  [N, K], column sums of g or None), v the values of ``x8``."""
-    return _gemm_tn(g, x8.unpack(), want_bias)
+    n, k = g.size(1), x8.shape[1]
+    gw = torch.empty(n, k, dtype=torch.float32, device=g.device)
+    gb = torch.empty(n, dtype=torch.float32, device=g.device) if want_bias else None
+    nws = _lib.load().hgv_gemm_tn8_ws(g.size(0), n, k)
+    ws = torch.empty(nws, dtype=torch.uint8, device=g.device)
+    _lib.call("hgv_gemm_tn8", g.data_ptr(), ld_of(g), n, x8.q.data_ptr(), x8.q.stride(0), x8.scale.data_ptr(), k, g.size(0), gw.data_ptr(), k,
+              _lib.ptr(gb), ws.data_ptr(), nws, _lib.stream())
+    return gw, gb
 
 
 def linear8(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None) -> torch.Tensor:

@@ -572,6 +572,11 @@ int hgv_grad_norm_clip(const float* g, int64_t n, float max_norm, float* norm_ou
  * scale [N, ceil(C/32)] uint8 = e + 127, or 255 for a block that holds an infinity or NaN (it reads back as NaN). */
 int hgv_pack8(const float* x, int64_t ldx, int64_t N, int C, int8_t* q, int64_t ldq, uint8_t* scale, hgv_stream_t stream);
 int hgv_unpack8(const int8_t* q, int64_t ldq, const uint8_t* scale, int64_t N, int C, float* out, int64_t ldo, hgv_stream_t stream);
+/* Weight gradient of a projection whose input was kept in 8 bits: GW[N, K] = G^T V with V [M, K] the values of (q, scale), and
+ * (where not NULL) gbias[N] = column sums of G.  G [M, ldg] 16-byte aligned, ldg a multiple of 4 that covers N rounded up to 4. */
+size_t hgv_gemm_tn8_ws(int64_t M, int N, int K);
+int hgv_gemm_tn8(const float* G, int64_t ldg, int N, const int8_t* q, int64_t ldq, const uint8_t* scale, int K, int64_t M, float* GW,
+                 int64_t ldgw, float* gbias, void* ws, size_t ws_bytes, hgv_stream_t stream);
 
 /* ---- group norm with an activation over the rows of each graph, channels last (no reference counterpart: its levels
  *      normalise over the whole batch, nn.BatchNorm1d at gvae/gvae_skipcon.py:63) --------------------------------------
