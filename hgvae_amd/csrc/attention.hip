@@ -32,12 +32,13 @@ struct AtArgs {
     float scale;
     const uint8_t* mask;                                        // [N] keys that take part, or null
     const int32_t* ptr;
-    const int4* tiles;                                          // prepass tiles of 64 rows: (graph, row, first tile, tiles of the graph)
+    const int4* tiles;                                          // tiles of 64 rows: (graph, row, first tile, tiles of the graph)
     int n_tiles;
     const int4* blocks;                                         // of a launch: tiles of 64 or 128 rows, largest graphs first
     const int4* block_list[2]; int n_blocks[2];                 // all of them: (graph, row, -, -) of 64 rows, of 128 rows
     float neg;                                                  // -1, unknown to the compiler: keeps x - (float)half one instruction (v_fma_mix_f32)
 
+    int max_rows;                                               // of the largest graph
     int* part;                                                  // [tile][4][Hk] exponents of the longest row
     int* exps;                                                  // [B][Hk][4]
     _Float16* img[4];                                           // [heads][N][hi DP | lo DP]
@@ -48,90 +49,129 @@ struct AtArgs {
 };
 
 // ---- operands into scaled fp16 pieces ------------------------------------------------------------------------------------
-// Sixteen lanes take one (row, head) vector.  First pass: the exponent e with |row| < 2^e, its maximum over the tile per key head.
-__global__ __launch_bounds__(256) void k_at_norms(const AtArgs a) {
-    __shared__ int best[256];
-    const int ten = blockIdx.y;
-    const int4 tile = a.tiles[blockIdx.x];
-    const int rows = min(64, (int)(a.ptr[tile.x + 1] - tile.y));
-    const int heads = (ten == TQ || ten == TG) ? a.H : a.Hk, per = heads / a.Hk;
-    for (int h0 = 0; h0 < a.Hk; h0 += 256) {                    // key heads in slabs of 256
-        const int hk_n = min(256, a.Hk - h0);
-        for (int i = threadIdx.x; i < hk_n; i += 256) best[i] = NO_EXP;
-        __syncthreads();
-        const int sub = threadIdx.x & 15;
-        for (int v = threadIdx.x >> 4; v < rows * hk_n * per; v += 16) {
-            const int r = v / (hk_n * per), h = h0 * per + v - r * hk_n * per;
-            const int64_t n = tile.y + r;
-            if (a.mask && (ten == TK || ten == TV) && !a.mask[n]) continue;
-            const float* p = a.src[ten] + n * a.row_stride[ten] + h * a.head_stride[ten];
-            double s = 0.0;
-            for (int d = sub; d < a.D; d += 16) s = fma((double)p[d], (double)p[d], s);
+// Sixteen lanes take one (row, head) vector, a lane DP / 16 neighbouring columns of it.  VEC: 8- or 16-byte loads (D = DP, strides
+// and addresses that allow it).
+template <int DP, bool VEC>
+__device__ __forceinline__ void load_part(const float* p, int sub, int D, bool live, float v[DP / 16]) {
+    constexpr int E = DP / 16;
+    if (VEC) {
+        if (E % 4 == 0) {
 #pragma unroll
-            for (int o = 1; o < 16; o <<= 1) s += __shfl_xor(s, o, 64);
-            if (sub == 0 && s > 0.0 && s < 1e300) {             // rows that hold an infinity or NaN do not count
-                const int e2 = (int)((__double_as_longlong(s) >> 52) & 2047) - 1023;
-                atomicMax(&best[h / per - h0], (e2 >> 1) + 1);
+            for (int i = 0; i < E; i += 4) {
+                const f32x4 t = live ? *(const f32x4*)(p + sub * E + i) : f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[i + j] = t[j];
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < E; i += 2) {
+                const float2 t = live ? *(const float2*)(p + sub * E + i) : make_float2(0.f, 0.f);
+                v[i] = t.x; v[i + 1] = t.y;
             }
         }
-        __syncthreads();
-        for (int i = threadIdx.x; i < hk_n; i += 256) a.part[((int64_t)blockIdx.x * 4 + ten) * a.Hk + h0 + i] = best[i];
-        __syncthreads();
+    } else {
+#pragma unroll
+        for (int i = 0; i < E; ++i) v[i] = live && sub * E + i < D ? p[sub * E + i] : 0.f;
     }
 }
 
-// Second pass: one workgroup per (tile, tensor, key head).
-template <int DP>
-__global__ __launch_bounds__(256) void k_at_split(const AtArgs a) {
-    constexpr int E = DP / 16;
-    __shared__ int se[2];
-    const int ten = blockIdx.y, hk = blockIdx.z;
-    const int4 tile = a.tiles[blockIdx.x];
-    if (threadIdx.x < 64) {
-        int e = NO_EXP, ev = NO_EXP;
-        for (int i = threadIdx.x; i < tile.w; i += 64) {
-            e = max(e, a.part[((int64_t)(tile.z + i) * 4 + ten) * a.Hk + hk]);
-            if (ten == TG) ev = max(ev, a.part[((int64_t)(tile.z + i) * 4 + TV) * a.Hk + hk]);
-        }
+// The exponent e with |row| < 2^e of the longest row among rows n0 .. n0 + rows - 1 of key head hk, over the whole workgroup
+// (NO_EXP: none that is finite and not zero).  red: four ints of LDS, free to be written.
+template <int DP, bool VEC>
+__device__ __forceinline__ int longest_row(const AtArgs& a, int ten, int hk, int64_t n0, int rows, int* red) {
+    const int per = (ten == TQ || ten == TG) ? a.R : 1, sub = threadIdx.x & 15;
+    const bool masked = a.mask && (ten == TK || ten == TV);
+    int best = NO_EXP;
+    for (int i = threadIdx.x >> 4; i < rows * per; i += 16) {
+        const int r = i / per, h = hk * per + i - r * per;
+        const int64_t n = n0 + r;
+        float v[DP / 16];
+        load_part<DP, VEC>(a.src[ten] + n * a.row_stride[ten] + h * a.head_stride[ten], sub, a.D, !(masked && !a.mask[n]), v);
+        double s = 0.0;
 #pragma unroll
-        for (int o = 32; o > 0; o >>= 1) {
-            e = max(e, __shfl_xor(e, o, 64));
-            ev = max(ev, __shfl_xor(ev, o, 64));
-        }
-        if (threadIdx.x == 0) {
-            se[0] = e == NO_EXP ? 0 : e;
-            se[1] = ev == NO_EXP ? 0 : ev;
-        }
+        for (int e = 0; e < DP / 16; ++e) s = fma((double)v[e], (double)v[e], s);
+#pragma unroll
+        for (int o = 1; o < 16; o <<= 1) s += __shfl_xor(s, o, 64);
+        const int e2 = (int)((__double_as_longlong(s) >> 52) & 2047) - 1023;
+        if (s > 0.0 && s < 1e300) best = max(best, (e2 >> 1) + 1);      // rows that hold an infinity or NaN do not count
     }
+#pragma unroll
+    for (int o = 16; o < 64; o <<= 1) best = max(best, __shfl_xor(best, o, 64));
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = best;
     __syncthreads();
-    const int e = se[0], ev = se[1];
-    if (threadIdx.x == 0 && (int)blockIdx.x == tile.z) a.exps[((int64_t)tile.x * a.Hk + hk) * 4 + ten] = e;
+    best = max(max(red[0], red[1]), max(red[2], red[3]));
+    __syncthreads();
+    return best;
+}
+
+// Graphs of more than four tiles: one workgroup per (tile, tensor, key head) leaves the exponent of its tile.
+template <int DP, bool VEC>
+__global__ __launch_bounds__(256) void k_at_norms(const AtArgs a, const int first) {
+    __shared__ int red[4];
+    const int ten = first + blockIdx.y, hk = blockIdx.z;
+    const int4 tile = a.tiles[blockIdx.x];
+    const int best = longest_row<DP, VEC>(a, ten, hk, tile.y, min(64, (int)(a.ptr[tile.x + 1] - tile.y)), red);
+    if (threadIdx.x == 0) a.part[((int64_t)blockIdx.x * 4 + ten) * a.Hk + hk] = best;
+}
+
+// The exponent of a (graph, tensor, key head): from its tiles, or (SELF, graphs of up to four tiles) from the rows themselves, which
+// saves a launch.
+template <int DP, bool VEC, bool SELF>
+__device__ __forceinline__ int graph_exp(const AtArgs& a, int4 tile, int ten, int hk, int* red) {
+    int e = NO_EXP;
+    if (SELF) {
+        e = longest_row<DP, VEC>(a, ten, hk, a.ptr[tile.x], (int)(a.ptr[tile.x + 1] - a.ptr[tile.x]), red);
+    } else {
+        for (int i = threadIdx.x; i < tile.w; i += 256) e = max(e, a.part[((int64_t)(tile.z + i) * 4 + ten) * a.Hk + hk]);
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) e = max(e, __shfl_xor(e, o, 64));
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = e;
+        __syncthreads();
+        e = max(max(red[0], red[1]), max(red[2], red[3]));
+        __syncthreads();
+    }
+    return e == NO_EXP ? 0 : e;
+}
+
+// One workgroup per (tile, tensor, key head).  The gradient's also takes the dot products with the output.
+template <int DP, bool VEC, bool SELF>
+__global__ __launch_bounds__(256) void k_at_split(const AtArgs a, const int first) {
+    constexpr int E = DP / 16;
+    __shared__ int red[4];
+    const int ten = first + blockIdx.y, hk = blockIdx.z;
+    const int4 tile = a.tiles[blockIdx.x];
+    const int e = graph_exp<DP, VEC, SELF>(a, tile, ten, hk, red);
+    const int64_t at = ((int64_t)tile.x * a.Hk + hk) * 4;
+    const int ev = ten != TG ? 0 : first == TG ? a.exps[at + TV] : graph_exp<DP, VEC, SELF>(a, tile, TV, hk, red);
+    if (threadIdx.x == 0 && (int)blockIdx.x == tile.z) a.exps[at + ten] = e;
     const int rows = min(64, (int)(a.ptr[tile.x + 1] - tile.y));
     const int per = (ten == TQ || ten == TG) ? a.R : 1, sub = threadIdx.x & 15;
-    for (int v = threadIdx.x >> 4; v < rows * per; v += 16) {
-        const int r = v / per, h = hk * per + v - r * per;
+    const bool masked = a.mask && (ten == TK || ten == TV);
+    for (int i = threadIdx.x >> 4; i < rows * per; i += 16) {
+        const int r = i / per, h = hk * per + i - r * per;
         const int64_t n = tile.y + r;
-        const bool live = !(a.mask && (ten == TK || ten == TV) && !a.mask[n]);
-        const float* p = a.src[ten] + n * a.row_stride[ten] + h * a.head_stride[ten];
-        const float* o = ten == TG ? a.out + (n * a.H + h) * a.D : nullptr;
-        _Float16 hi[E], lo[E];
-        float dot = 0.f;
+        float v[E];
+        load_part<DP, VEC>(a.src[ten] + n * a.row_stride[ten] + h * a.head_stride[ten], sub, a.D, !(masked && !a.mask[n]), v);
+        f16x2 hi[E / 2], lo[E / 2];
 #pragma unroll
-        for (int i = 0; i < E; ++i) {
-            const int d = sub * E + i;
-            const float x = live && d < a.D ? p[d] : 0.f;
-            const float y = ldexpf(x, 15 - e);
-            if (ten == TG && d < a.D) dot = fmaf(y, o[d], dot);
-            hi[i] = (_Float16)y;
-            lo[i] = (_Float16)(y - (float)hi[i]);
+        for (int j = 0; j < E; ++j) v[j] = ldexpf(v[j], 15 - e);
+#pragma unroll
+        for (int j = 0; j < E; j += 2) {
+            hi[j / 2] = f16x2{(_Float16)v[j], (_Float16)v[j + 1]};
+            lo[j / 2] = f16x2{(_Float16)(v[j] - (float)hi[j / 2][0]), (_Float16)(v[j + 1] - (float)hi[j / 2][1])};
         }
         _Float16* dst = a.img[ten] + ((int64_t)h * a.N + n) * (2 * DP) + sub * E;
 #pragma unroll
-        for (int i = 0; i < E; i += 2) {
-            *(f16x2*)(dst + i) = f16x2{hi[i], hi[i + 1]};
-            *(f16x2*)(dst + DP + i) = f16x2{lo[i], lo[i + 1]};
+        for (int j = 0; j < E / 2; ++j) {
+            *(f16x2*)(dst + 2 * j) = hi[j];
+            *(f16x2*)(dst + DP + 2 * j) = lo[j];
         }
         if (ten == TG) {
+            const float* o = a.out + (n * a.H + h) * a.D;
+            float dot = 0.f;
+#pragma unroll
+            for (int j = 0; j < E; ++j)
+                if (sub * E + j < a.D) dot = fmaf(v[j], o[sub * E + j], dot);
 #pragma unroll
             for (int w = 1; w < 16; w <<= 1) dot += __shfl_xor(dot, w, 64);
             if (sub == 0) a.delta[(int64_t)h * a.N + n] = ldexpf(dot, -16 - ev);
@@ -646,11 +686,25 @@ void at_rows(AtArgs& a, int heads, F launch) {
     launch(i, dim3((unsigned)((int64_t)a.n_blocks[i] * heads)));
 }
 
+// The operands' images: tensors first .. last.
+template <int DP, bool VEC>
+void at_images(const AtArgs& a, int first, int last, hipStream_t stream) {
+    const dim3 grid((unsigned)a.n_tiles, (unsigned)(last - first + 1), (unsigned)a.Hk);
+    if (a.max_rows <= 256) {
+        hipLaunchKernelGGL((k_at_split<DP, VEC, true>), grid, dim3(256), 0, stream, a, first);
+    } else {
+        hipLaunchKernelGGL((k_at_norms<DP, VEC>), grid, dim3(256), 0, stream, a, first);
+        hipLaunchKernelGGL((k_at_split<DP, VEC, false>), grid, dim3(256), 0, stream, a, first);
+    }
+}
+
 template <int DP>
 int at_launch(AtArgs a, bool backward, hipStream_t stream) {
-    const int tensors = backward ? 4 : 3;
-    hipLaunchKernelGGL(k_at_norms, dim3((unsigned)a.n_tiles, (unsigned)tensors), dim3(256), 0, stream, a);
-    hipLaunchKernelGGL(k_at_split<DP>, dim3((unsigned)a.n_tiles, (unsigned)tensors, (unsigned)a.Hk), dim3(256), 0, stream, a);
+    bool vec = a.D == DP;
+    for (int i = 0; i < (backward ? 4 : 3); ++i)
+        vec = vec && hgv_aligned(a.src[i], 16) && a.row_stride[i] % 4 == 0 && a.head_stride[i] % 4 == 0;
+    if (vec) at_images<DP, true>(a, TQ, backward ? TG : TV, stream);
+    else at_images<DP, false>(a, TQ, backward ? TG : TV, stream);
     if (!backward) {
         at_rows(a, a.H, [&](int i, dim3 grid) {
             if (i) hipLaunchKernelGGL((k_at_fwd<DP, 4>), grid, dim3(256), 0, stream, a);
@@ -682,17 +736,17 @@ int at_dispatch(const AtArgs& a, bool backward, hipStream_t stream) {
 }
 
 int at_fill(AtArgs& a, const char* what, int64_t N, int num_graphs, int H, int Hk, int D, float scale, const uint8_t* mask, const int32_t* ptr,
-            const int32_t* tiles, int n_tiles, const int32_t* blocks, int n64, int n128, void* ws, size_t ws_bytes, bool backward) {
+            int max_rows, const int32_t* tiles, int n_tiles, const int32_t* blocks, int n64, int n128, void* ws, size_t ws_bytes, bool backward) {
     HGV_REQUIRE(N > 0 && N <= 0x7fffffff && num_graphs > 0 && H > 0 && Hk > 0 && H % Hk == 0 && D > 0, HGV_EINVAL, "%s: bad sizes", what);
     HGV_REQUIRE(D <= 128 && H <= 65535, HGV_EUNSUPPORTED, "%s: heads of %d columns (at most 128), %d of them", what, D, H);
     HGV_REQUIRE(scale > 0.f && scale < INFINITY, HGV_EINVAL, "%s: the scale must be positive and finite", what);
-    HGV_REQUIRE(ptr && tiles && blocks && n_tiles > 0 && n64 > 0 && n128 > 0, HGV_EINVAL, "%s: null plan", what);
+    HGV_REQUIRE(ptr && tiles && blocks && n_tiles > 0 && n64 > 0 && n128 > 0 && max_rows > 0, HGV_EINVAL, "%s: null plan", what);
     HGV_REQUIRE((int64_t)n64 * H <= 0x3fffffff, HGV_EUNSUPPORTED, "%s: too many tiles", what);
     const AtSizes s = at_sizes(N, H, Hk, D, n_tiles, num_graphs, backward);
     HGV_REQUIRE(ws && ws_bytes >= s.total && hgv_aligned(ws, 256), HGV_EWORKSPACE, "%s: workspace too small or misaligned", what);
     a.neg = -1.f;
     a.N = N; a.H = H; a.Hk = Hk; a.R = H / Hk; a.D = D; a.scale = scale; a.mask = mask; a.ptr = ptr;
-    a.tiles = (const int4*)tiles; a.n_tiles = n_tiles;
+    a.tiles = (const int4*)tiles; a.n_tiles = n_tiles; a.max_rows = max_rows;
     a.n_blocks[0] = n64; a.n_blocks[1] = n128;
     a.block_list[0] = (const int4*)blocks; a.block_list[1] = a.block_list[0] + n64;
     char* p = (char*)ws;
@@ -712,11 +766,11 @@ extern "C" size_t hgv_graph_attention_ws(int64_t N, int num_graphs, int H, int H
 
 extern "C" int hgv_graph_attention_fwd(const float* q, int64_t q_row, int64_t q_head, const float* k, int64_t k_row, int64_t k_head,
                                        const float* v, int64_t v_row, int64_t v_head, int64_t N, int num_graphs, int H, int Hk, int D,
-                                       float scale, const uint8_t* mask, const int32_t* ptr, const int32_t* tiles, int n_tiles,
+                                       float scale, const uint8_t* mask, const int32_t* ptr, int max_rows, const int32_t* tiles, int n_tiles,
                                        const int32_t* blocks, int n64, int n128, float* out, float* lse, void* ws, size_t ws_bytes,
                                        hipStream_t stream) {
     AtArgs a = {};
-    const int rc = at_fill(a, "graph_attention_fwd", N, num_graphs, H, Hk, D, scale, mask, ptr, tiles, n_tiles, blocks, n64, n128, ws, ws_bytes, false);
+    const int rc = at_fill(a, "graph_attention_fwd", N, num_graphs, H, Hk, D, scale, mask, ptr, max_rows, tiles, n_tiles, blocks, n64, n128, ws, ws_bytes, false);
     if (rc) return rc;
     HGV_REQUIRE(q && k && v && out && (D % 4 || hgv_aligned(out, 16)), HGV_EINVAL, "graph_attention_fwd: null or misaligned buffer");
     a.src[TQ] = q; a.row_stride[TQ] = q_row; a.head_stride[TQ] = q_head;
@@ -729,10 +783,10 @@ extern "C" int hgv_graph_attention_fwd(const float* q, int64_t q_row, int64_t q_
 extern "C" int hgv_graph_attention_bwd(const float* q, int64_t q_row, int64_t q_head, const float* k, int64_t k_row, int64_t k_head,
                                        const float* v, int64_t v_row, int64_t v_head, const float* g, int64_t g_row, int64_t g_head,
                                        const float* out, const float* lse, int64_t N, int num_graphs, int H, int Hk, int D, float scale,
-                                       const uint8_t* mask, const int32_t* ptr, const int32_t* tiles, int n_tiles, const int32_t* blocks,
+                                       const uint8_t* mask, const int32_t* ptr, int max_rows, const int32_t* tiles, int n_tiles, const int32_t* blocks,
                                        int n64, int n128, float* dq, float* dk, float* dv, void* ws, size_t ws_bytes, hipStream_t stream) {
     AtArgs a = {};
-    const int rc = at_fill(a, "graph_attention_bwd", N, num_graphs, H, Hk, D, scale, mask, ptr, tiles, n_tiles, blocks, n64, n128, ws, ws_bytes, true);
+    const int rc = at_fill(a, "graph_attention_bwd", N, num_graphs, H, Hk, D, scale, mask, ptr, max_rows, tiles, n_tiles, blocks, n64, n128, ws, ws_bytes, true);
     if (rc) return rc;
     HGV_REQUIRE(q && k && v && g && out && lse && (dq || dk) && !dk == !dv, HGV_EINVAL, "graph_attention_bwd: null buffer (dk and dv come together)");
     HGV_REQUIRE(D % 4 || (hgv_aligned(dq, 16) && hgv_aligned(dk, 16) && hgv_aligned(dv, 16)), HGV_EINVAL, "graph_attention_bwd: misaligned buffer");

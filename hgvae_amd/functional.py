@@ -2694,7 +2694,7 @@ class _GraphAttention(torch.autograd.Function):
         nws = _lib.load().hgv_graph_attention_ws(n, seg.num_graphs, h, hk, d, seg._n_tiles, 0)
         ws = torch.empty(nws, dtype=torch.uint8, device=q.device)
         _lib.call("hgv_graph_attention_fwd", *_strided(q), *_strided(k), *_strided(v), n, seg.num_graphs, h, hk, d, scale, _lib.ptr(mask),
-                  seg._ptr.data_ptr(), seg._tiles.data_ptr(), seg._n_tiles, seg._blocks.data_ptr(), *seg._n_blocks, out.data_ptr(),
+                  seg._ptr.data_ptr(), seg._sorted[-1], seg._tiles.data_ptr(), seg._n_tiles, seg._blocks.data_ptr(), *seg._n_blocks, out.data_ptr(),
                   _lib.ptr(lse), ws.data_ptr(), nws, _lib.stream())
         ctx.seg, ctx.scale = seg, scale
         if train:
@@ -2715,7 +2715,7 @@ class _GraphAttention(torch.autograd.Function):
             nws = _lib.load().hgv_graph_attention_ws(n, seg.num_graphs, h, hk, d, seg._n_tiles, 1)
             ws = torch.empty(nws, dtype=torch.uint8, device=q.device)
             _lib.call("hgv_graph_attention_bwd", *_strided(q), *_strided(k), *_strided(v), *_strided(g), out.data_ptr(), lse.data_ptr(), n,
-                      seg.num_graphs, h, hk, d, ctx.scale, _lib.ptr(mask), seg._ptr.data_ptr(), seg._tiles.data_ptr(), seg._n_tiles,
+                      seg.num_graphs, h, hk, d, ctx.scale, _lib.ptr(mask), seg._ptr.data_ptr(), seg._sorted[-1], seg._tiles.data_ptr(), seg._n_tiles,
                       seg._blocks.data_ptr(), *seg._n_blocks, _lib.ptr(dq), _lib.ptr(dk), _lib.ptr(dv), ws.data_ptr(), nws, _lib.stream())
         return dq, dk if need[1] else None, dv if need[2] else None, None, None, None
 

@@ -606,14 +606,14 @@ int hgv_group_norm_bwd(const float* g, int64_t ldg, const float* x, int64_t ldx,
  * where D is a multiple of 4).  For row i of a graph over its keys j (mask[j] != 0, or all where mask is NULL):
  *   p = softmax_j(scale * q_i . k_j),  out_i = sum_j p_j v_j;   a graph without keys gives zeros, and zero gradients.
  * A masked row of k or v may hold anything; its dk and dv are zeros.  scale > 0.
- * Graphs: ptr [num_graphs + 1]; tiles [n_tiles][4] (graph, first row, first tile of the graph, tiles of the graph) of 64 rows;
+ * Graphs: ptr [num_graphs + 1], the largest has max_rows rows; tiles [n_tiles][4] (graph, first row, first tile of the graph, tiles of the graph) of 64 rows;
  * blocks [n64 + n128][4] (graph, first row, -, -): all tiles of 64 rows, then those of 128, in the order in which they are to run.
  * lse [H, N] (base 2, of the scaled logits; +inf for a row without keys) may be NULL in the forward pass; the backward pass
  * reads it and out.  dq, or dk and dv together, may be NULL. */
 size_t hgv_graph_attention_ws(int64_t N, int num_graphs, int H, int Hk, int D, int64_t n_tiles, int backward);
 int hgv_graph_attention_fwd(const float* q, int64_t q_row, int64_t q_head, const float* k, int64_t k_row, int64_t k_head, const float* v,
                             int64_t v_row, int64_t v_head, int64_t N, int num_graphs, int H, int Hk, int D, float scale,
-                            const uint8_t* mask, const int32_t* ptr, const int32_t* tiles, int n_tiles, const int32_t* blocks,
+                            const uint8_t* mask, const int32_t* ptr, int max_rows, const int32_t* tiles, int n_tiles, const int32_t* blocks,
                             int n64, int n128, float* out, float* lse, void* ws,
                             size_t ws_bytes, hgv_stream_t stream);
 int hgv_graph_attention_bwd(const float* q, int64_t q_row, int64_t q_head, const float* k, int64_t k_row, int64_t k_head, const float* v,
