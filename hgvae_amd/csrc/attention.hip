@@ -303,10 +303,13 @@ __device__ __forceinline__ void store4(float* p, int d, int D, f32x4 v) {
 constexpr float P_BITS = 8.f;                                   // probabilities start at 2^8 and may grow to 2^15 before a rescale
 constexpr float P_GROW = 7.f;
 
+// Waves per SIMD the registers are cut to: two (128-wide heads with 16 rows per wave and four waves: one, anything else spills).
+constexpr int at_bounds(int DP, int NW) { return DP == 128 && NW == 4 ? 1 : 2; }
+
 // ---- forward -----------------------------------------------------------------------------------------------------------------
-// A workgroup owns 32 * NW queries of one head (a wave 32), walks the keys of the graph in tiles of 64.
-template <int DP, int NW>
-__global__ __launch_bounds__(64 * NW, 2) void k_at_fwd(const AtArgs a) {
+// A workgroup owns 16 * QB * NW queries of one head (a wave 16 * QB), walks the keys of the graph in tiles of 64.
+template <int DP, int QB, int NW>
+__global__ __launch_bounds__(64 * NW, DP == 32 ? 4 : at_bounds(DP, NW)) void k_at_fwd(const AtArgs a) {
     constexpr int KC = DP / 32, DB = DP / 16;
     __shared__ __align__(16) unsigned char ldsK[64 * line_bytes<DP>()];
     __shared__ __align__(16) unsigned char ldsV[64 * line_bytes<DP>()];
@@ -315,18 +318,22 @@ __global__ __launch_bounds__(64 * NW, 2) void k_at_fwd(const AtArgs a) {
     const int blk = blockIdx.x / a.H, h = blockIdx.x - blk * a.H, hk = h / a.R;
     const int4 t = a.blocks[blk];
     const int64_t k0 = a.ptr[t.x], k1 = a.ptr[t.x + 1];
-    const int64_t q0 = (int64_t)t.y + 32 * wave;
+    const int64_t q0 = (int64_t)t.y + 16 * QB * wave;
     const int* ex = a.exps + ((int64_t)t.x * a.Hk + hk) * 4;
     const float c = fold_scale(a.scale, ex[TQ] + ex[TK] - 30);
-    Frag q[2][KC];
+    Frag q[QB][KC];
 #pragma unroll
-    for (int b = 0; b < 2; ++b)
+    for (int b = 0; b < QB; ++b)
 #pragma unroll
         for (int k = 0; k < KC; ++k) q[b][k] = own_frag<DP>(a.img[TQ] + (int64_t)h * a.N * (2 * DP), min(q0 + 16 * b + (lane & 15), k1 - 1), k, lane);
-    f32x4 acc[DB][2];
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};     // m: the exponent that is subtracted, base 2
+    f32x4 acc[DB][QB];
+    float m[QB], l[QB];                                         // m: the exponent that is subtracted, base 2
 #pragma unroll
-    for (int d = 0; d < DB; ++d) acc[d][0] = acc[d][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int b = 0; b < QB; ++b) { m[b] = -INFINITY; l[b] = 0.f; }
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int b = 0; b < QB; ++b) acc[d][b] = f32x4{0.f, 0.f, 0.f, 0.f};
     const _Float16* ki = a.img[TK] + ((int64_t)hk * a.N + k0) * (2 * DP);
     const _Float16* vi = a.img[TV] + ((int64_t)hk * a.N + k0) * (2 * DP);
     const int n = (int)(k1 - k0);
@@ -348,24 +355,25 @@ __global__ __launch_bounds__(64 * NW, 2) void k_at_fwd(const AtArgs a) {
             nb = threadIdx.x < 64 && j < n && (!a.mask || a.mask[k0 + j]) ? 0.f : -INFINITY;
         }
         const bool biased = a.mask != nullptr || kt + 64 > n;
-        f32x4 s[4][2];
+        f32x4 s[4][QB];
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
-            s[b][0] = s[b][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int j = 0; j < QB; ++j) s[b][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int k = 0; k < KC; ++k) {
                 const Frag f = row_frag<DP>(ldsK, 16 * b, k, lane);
-                s[b][0] = mma3(f, q[0][k], s[b][0]);
-                s[b][1] = mma3(f, q[1][k], s[b][1]);
+#pragma unroll
+                for (int j = 0; j < QB; ++j) s[b][j] = mma3(f, q[j][k], s[b][j]);
             }
             if (biased) {
                 const f32x4 o = *(const f32x4*)(bias + 16 * b + 4 * g);
-                s[b][0] += o;
-                s[b][1] += o;
+#pragma unroll
+                for (int j = 0; j < QB; ++j) s[b][j] += o;
             }
         }
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
+        for (int b = 0; b < QB; ++b) {
             float top = s[0][b][0];
 #pragma unroll
             for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i >> 2][b][i & 3]);
@@ -394,17 +402,19 @@ __global__ __launch_bounds__(64 * NW, 2) void k_at_fwd(const AtArgs a) {
         }
 #pragma unroll
         for (int kc = 0; kc < 2; ++kc) {
-            const Frag p0 = split_frag(s[2 * kc][0], s[2 * kc + 1][0], a.neg), p1 = split_frag(s[2 * kc][1], s[2 * kc + 1][1], a.neg);
+            Frag p[QB];
+#pragma unroll
+            for (int j = 0; j < QB; ++j) p[j] = split_frag(s[2 * kc][j], s[2 * kc + 1][j], a.neg);
 #pragma unroll
             for (int d = 0; d < DB; ++d) {
                 const Frag f = col_frag<DP>(ldsV, 32 * kc, d, lane);
-                acc[d][0] = mma3(f, p0, acc[d][0]);
-                acc[d][1] = mma3(f, p1, acc[d][1]);
+#pragma unroll
+                for (int j = 0; j < QB; ++j) acc[d][j] = mma3(f, p[j], acc[d][j]);
             }
         }
     }
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
+    for (int b = 0; b < QB; ++b) {
         l[b] += __shfl_xor(l[b], 16, 64);
         l[b] += __shfl_xor(l[b], 32, 64);
         const int64_t row = q0 + 16 * b + (lane & 15);
@@ -421,7 +431,7 @@ __global__ __launch_bounds__(64 * NW, 2) void k_at_fwd(const AtArgs a) {
 // ---- backward: dk and dv ---------------------------------------------------------------------------------------------------
 // A workgroup owns 16 * KB * NW keys of one key head (a wave 16 * KB), walks the queries of the graph, head by head, in tiles of 64 rows.
 template <int DP, int KB, int NW>
-__global__ __launch_bounds__(64 * NW, 2) void k_at_dkv(const AtArgs a) {
+__global__ __launch_bounds__(64 * NW, at_bounds(DP, NW)) void k_at_dkv(const AtArgs a) {
     constexpr int KC = DP / 32, DB = DP / 16;
     __shared__ __align__(16) unsigned char ldsQ[64 * line_bytes<DP>()];
     __shared__ __align__(16) unsigned char ldsG[64 * line_bytes<DP>()];
@@ -548,7 +558,7 @@ __global__ __launch_bounds__(64 * NW, 2) void k_at_dkv(const AtArgs a) {
 
 // ---- backward: dq -----------------------------------------------------------------------------------------------------------
 template <int DP, int QB, int NW>
-__global__ __launch_bounds__(64 * NW, 2) void k_at_dq(const AtArgs a) {
+__global__ __launch_bounds__(64 * NW, at_bounds(DP, NW)) void k_at_dq(const AtArgs a) {
     constexpr int KC = DP / 32, DB = DP / 16;
     __shared__ __align__(16) unsigned char ldsK[64 * line_bytes<DP>()];
     __shared__ __align__(16) unsigned char ldsV[64 * line_bytes<DP>()];
@@ -680,7 +690,8 @@ AtSizes at_sizes(int64_t N, int H, int Hk, int D, int64_t n_tiles, int64_t graph
 
 template <typename F>
 void at_rows(AtArgs& a, int heads, F launch) {
-    // blocks of 128 rows where that gives a workgroup to each of the 256 compute units, else of 64
+    // blocks of 128 rows where that gives a workgroup to each of the 256 compute units, else of 64 (one graph of 5 000 nodes, one
+    // head: forward and backward 0.47 ms)
     const int i = (int64_t)a.n_blocks[1] * heads >= 256 ? 1 : 0;
     a.blocks = a.block_list[i];
     launch(i, dim3((unsigned)((int64_t)a.n_blocks[i] * heads)));
@@ -705,21 +716,24 @@ int at_launch(AtArgs a, bool backward, hipStream_t stream) {
         vec = vec && hgv_aligned(a.src[i], 16) && a.row_stride[i] % 4 == 0 && a.head_stride[i] % 4 == 0;
     if (vec) at_images<DP, true>(a, TQ, backward ? TG : TV, stream);
     else at_images<DP, false>(a, TQ, backward ? TG : TV, stream);
+    // 32 rows per wave, four waves; wider heads (above 64 columns backward, 96 forward): 16 rows, eight waves, so that the accumulators
+    // do not push the operands out of the registers; blocks of 64 rows: 16 rows, four waves.  32 x 2 500 nodes, 64 columns, backward:
+    // 32 rows 2.05 ms, 16 rows 2.25; 128 columns forward: 32 rows (with spills) 1.15 ms, 16 rows 0.79.
+    constexpr int RB = DP <= 64 ? 2 : 1;
     if (!backward) {
+        constexpr int QB = DP <= 96 ? 2 : 1;
         at_rows(a, a.H, [&](int i, dim3 grid) {
-            if (i) hipLaunchKernelGGL((k_at_fwd<DP, 4>), grid, dim3(256), 0, stream, a);
-            else hipLaunchKernelGGL((k_at_fwd<DP, 2>), grid, dim3(128), 0, stream, a);
+            if (i) hipLaunchKernelGGL((k_at_fwd<DP, QB, 8 / QB>), grid, dim3(512 / QB), 0, stream, a);
+            else hipLaunchKernelGGL((k_at_fwd<DP, 1, 4>), grid, dim3(256), 0, stream, a);
         });
     } else {
-        // wide heads: 16 keys / queries per wave, so that the accumulators of 32 do not push the operands out of the registers
-        constexpr int KB = DP <= 64 ? 2 : 1;
         if (a.dk) at_rows(a, a.Hk, [&](int i, dim3 grid) {
-            if (i) hipLaunchKernelGGL((k_at_dkv<DP, KB, 8 / KB>), grid, dim3(512 / KB), 0, stream, a);
-            else hipLaunchKernelGGL((k_at_dkv<DP, KB, 4 / KB>), grid, dim3(256 / KB), 0, stream, a);
+            if (i) hipLaunchKernelGGL((k_at_dkv<DP, RB, 8 / RB>), grid, dim3(512 / RB), 0, stream, a);
+            else hipLaunchKernelGGL((k_at_dkv<DP, 1, 4>), grid, dim3(256), 0, stream, a);
         });
         if (a.dq) at_rows(a, a.H, [&](int i, dim3 grid) {
-            if (i) hipLaunchKernelGGL((k_at_dq<DP, KB, 8 / KB>), grid, dim3(512 / KB), 0, stream, a);
-            else hipLaunchKernelGGL((k_at_dq<DP, KB, 4 / KB>), grid, dim3(256 / KB), 0, stream, a);
+            if (i) hipLaunchKernelGGL((k_at_dq<DP, RB, 8 / RB>), grid, dim3(512 / RB), 0, stream, a);
+            else hipLaunchKernelGGL((k_at_dq<DP, 1, 4>), grid, dim3(256), 0, stream, a);
         });
     }
     HGV_CHECK_LAUNCH(backward ? "graph_attention_bwd" : "graph_attention_fwd");
