@@ -210,6 +210,10 @@ def stream():
     return torch.cuda.current_stream().cuda_stream
 
 
+def current_device() -> int:
+    return _cur_device() if _cur_device is not None else torch.cuda.current_device()
+
+
 def require_cuda(*tensors):
     for t in tensors:
         if t is not None and not t.is_cuda:

@@ -7,6 +7,7 @@ re-implementation.
 from __future__ import annotations
 
 import contextlib
+import functools
 import os
 from typing import Optional
 
@@ -2431,9 +2432,24 @@ def gather_i64(src: torch.Tensor, idx: torch.Tensor) -> torch.Tensor:
 # --------------------------------------------------------------------------------------
 # activation checkpoints in 8 bits
 # --------------------------------------------------------------------------------------
-def _on_device(t: torch.Tensor):
-    """Context in which the current device is the tensor's (the library launches on the current device's stream)."""
-    return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+def _on_device(t: torch.Tensor, fn, *args):
+    """``fn(*args)`` with the tensor's device as the current one (the library launches on the current device's stream)."""
+    index = t.device.index
+    if index == _lib.current_device():
+        return fn(*args)
+    with torch.cuda.device(index):
+        return fn(*args)
+
+
+def _first_order(backward):
+    """Gradients that cannot be differentiated again: a second derivative through them raises.  (torch's own wrapper does this
+    too; it is only entered when a graph of the gradients is being built.)"""
+    guarded = torch.autograd.function.once_differentiable(backward)
+
+    @functools.wraps(backward)
+    def run(ctx, g):
+        return guarded(ctx, g) if torch.is_grad_enabled() else backward(ctx, g)
+    return run
 
 
 def _check_matrix(name: str, t, device=None, columns: Optional[int] = None):
@@ -2468,9 +2484,8 @@ class Packed8:
         n, c = self.shape
         out = new_padded(n, c, self.q.device, zero_pad=False)
         if n:
-            with _on_device(self.q):
-                _lib.call("hgv_unpack8", self.q.data_ptr(), self.q.stride(0), self.scale.data_ptr(), n, c, out.data_ptr(), out.stride(0),
-                          _lib.stream())
+            _on_device(self.q, lambda: _lib.call("hgv_unpack8", self.q.data_ptr(), self.q.stride(0), self.scale.data_ptr(), n, c,
+                                                 out.data_ptr(), out.stride(0), _lib.stream()))
         return out
 
     def nbytes(self) -> int:
@@ -2490,13 +2505,17 @@ def pack8(x: torch.Tensor) -> Packed8:
     _check_matrix("x", x)
     if x.size(1) < 1:
         raise _lib.HgvError("pack8: x has no columns")
+    return _on_device(x, _pack8, x)
+
+
+def _pack8(x: torch.Tensor) -> Packed8:
     x = rowmajor(x)
     n, c = x.shape
-    q = torch.empty(n, (c + 15) // 16 * 16, dtype=torch.int8, device=x.device)
+    ldq = (c + 15) // 16 * 16
+    q = torch.empty(n, ldq, dtype=torch.int8, device=x.device)
     scale = torch.empty(n, (c + 31) // 32, dtype=torch.uint8, device=x.device)
     if n:
-        with _on_device(x):
-            _lib.call("hgv_pack8", x.data_ptr(), ld_of(x), n, c, q.data_ptr(), q.stride(0), scale.data_ptr(), _lib.stream())
+        _lib.call("hgv_pack8", x.data_ptr(), ld_of(x), n, c, q.data_ptr(), ldq, scale.data_ptr(), _lib.stream())
     return Packed8(q, scale, (n, c))
 
 
@@ -2520,7 +2539,7 @@ class _Linear8(torch.autograd.Function):
         y = _gemm_nt(x, fwd, None, bias, w.size(0))
         ctx.packed = None
         if need[1]:
-            p = pack8(x)
+            p = _pack8(x)
             ctx.packed = p.shape
             ctx.save_for_backward(w, p.q, p.scale)
         else:
@@ -2528,19 +2547,22 @@ class _Linear8(torch.autograd.Function):
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_first_order
     def backward(ctx, g):
+        return _on_device(g, _Linear8._grads, ctx, g)
+
+    @staticmethod
+    def _grads(ctx, g):
         need = ctx.needs_input_grad
-        w = ctx.saved_tensors[0]
+        w, *kept = ctx.saved_tensors
         gx = gw = gb = None
-        with _on_device(g):
-            g = _own_rows(g)
-            if need[1]:
-                gw, gb = _weight_grad8(g, Packed8(*ctx.saved_tensors[1:], ctx.packed), need[2])
-            elif need[2]:
-                gb = g.sum(0)
-            if need[0]:
-                gx = _gemm_nt(g, ctx.image, None, None, w.size(1))
+        g = _own_rows(g)
+        if need[1]:
+            gw, gb = _weight_grad8(g, Packed8(*kept, ctx.packed), need[2])
+        elif need[2]:
+            gb = g.sum(0)
+        if need[0]:
+            gx = _gemm_nt(g, ctx.image, None, None, w.size(1))
         return gx, gw, gb
 
 
@@ -2569,8 +2591,7 @@ def linear8(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = Non
     bias = _check_vector("bias", bias, w.size(0), x.device)
     if x.size(0) == 0:
         return torch.nn.functional.linear(x, w, bias)           # no rows: an empty matrix, zero gradients
-    with _on_device(x):
-        return _Linear8.apply(x, w, bias)
+    return _on_device(x, _Linear8.apply, x, w, bias)
 
 
 # --------------------------------------------------------------------------------------
@@ -2587,21 +2608,18 @@ class _GroupNormAct(torch.autograd.Function):
     def forward(ctx, x, w, b, seg: Segments, groups, act, eps, keep8):
         x = rowmajor(x)
         n, c = x.shape
-        lib = _lib.load()
-        out = new_padded(n, c, x.device, zero_pad=False)
-        mean = torch.empty(seg.num_graphs, groups, dtype=torch.float64, device=x.device)
-        rstd = torch.empty(seg.num_graphs, groups, dtype=torch.float32, device=x.device)
-        small, rows, chunk0, chunk1 = seg._norm_plan(lib.hgv_group_norm_small_rows(c, groups))
-        listed = len(seg._sorted)
-        nws = lib.hgv_group_norm_ws(chunk1 - chunk0, seg.num_graphs, listed, small, c, groups, 0)
-        ws = torch.empty(nws, dtype=torch.uint8, device=x.device)
-        _lib.call("hgv_group_norm_fwd", x.data_ptr(), ld_of(x), c, groups, act, float(eps), _lib.ptr(w), _lib.ptr(b), seg._ptr.data_ptr(),
-                  seg._order.data_ptr(), seg._chunks.data_ptr(), seg._first.data_ptr(), seg.num_graphs, listed, small, rows, chunk0,
-                  chunk1, out.data_ptr(), out.stride(0), mean.data_ptr(), rstd.data_ptr(), ws.data_ptr(), nws, _lib.stream())
+        dev = x.device
+        out = new_padded(n, c, dev, zero_pad=False)
+        mean = torch.empty(seg.num_graphs, groups, dtype=torch.float64, device=dev)
+        rstd = torch.empty(seg.num_graphs, groups, dtype=torch.float32, device=dev)
+        arrays, counts, nws, _ = seg._norm_plan(c, groups)
+        ws = torch.empty(nws, dtype=torch.uint8, device=dev)
+        _lib.call("hgv_group_norm_fwd", x.data_ptr(), ld_of(x), c, groups, act, eps, _lib.ptr(w), _lib.ptr(b), *arrays, *counts,
+                  out.data_ptr(), out.stride(0), mean.data_ptr(), rstd.data_ptr(), ws.data_ptr(), nws, _lib.stream())
         ctx.seg, ctx.cfg = seg, (groups, act)
         ctx.packed = None
         if keep8 and any(ctx.needs_input_grad[:3]):
-            p = pack8(x)
+            p = _pack8(x)
             ctx.packed = p.shape
             ctx.save_for_backward(w, b, mean, rstd, p.q, p.scale)
         else:
@@ -2609,28 +2627,30 @@ class _GroupNormAct(torch.autograd.Function):
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_first_order
     def backward(ctx, g):
+        return _on_device(g, _GroupNormAct._grads, ctx, g)
+
+    @staticmethod
+    def _grads(ctx, g):
         seg, (groups, act) = ctx.seg, ctx.cfg
-        w, b, mean, rstd = ctx.saved_tensors[:4]
-        x, q, scale = (None, *ctx.saved_tensors[4:]) if ctx.packed else (ctx.saved_tensors[4], None, None)
+        w, b, mean, rstd, *kept = ctx.saved_tensors
         need = ctx.needs_input_grad
-        with _on_device(g):
-            g = rowmajor(g)
-            n, c = g.shape
-            lib = _lib.load()
-            gx = new_padded(n, c, g.device, zero_pad=False) if need[0] else None
-            gw = torch.empty(c, dtype=torch.float32, device=g.device) if need[1] else None
-            gb = torch.empty(c, dtype=torch.float32, device=g.device) if need[2] else None
-            small, rows, chunk0, chunk1 = seg._norm_plan(lib.hgv_group_norm_small_rows(c, groups))
-            listed = len(seg._sorted)
-            nws = lib.hgv_group_norm_ws(chunk1 - chunk0, seg.num_graphs, listed, small, c, groups, 1)
-            ws = torch.empty(nws, dtype=torch.uint8, device=g.device)
-            _lib.call("hgv_group_norm_bwd", g.data_ptr(), ld_of(g), _lib.ptr(x), ld_of(x) if x is not None else 0, _lib.ptr(q),
-                      q.stride(0) if q is not None else 0, _lib.ptr(scale), c, groups, act, _lib.ptr(w), _lib.ptr(b), seg._ptr.data_ptr(),
-                      seg._order.data_ptr(), seg._chunks.data_ptr(), seg._first.data_ptr(), seg.num_graphs, listed, small, rows,
-                      chunk0, chunk1, mean.data_ptr(), rstd.data_ptr(), _lib.ptr(gx), gx.stride(0) if gx is not None else 0,
-                      _lib.ptr(gw), _lib.ptr(gb), ws.data_ptr(), nws, _lib.stream())
+        g = rowmajor(g)
+        n, c = g.shape
+        dev = g.device
+        gx = new_padded(n, c, dev, zero_pad=False) if need[0] else None
+        gw = torch.empty(c, dtype=torch.float32, device=dev) if need[1] else None
+        gb = torch.empty(c, dtype=torch.float32, device=dev) if need[2] else None
+        arrays, counts, _, nws = seg._norm_plan(c, groups)
+        ws = torch.empty(nws, dtype=torch.uint8, device=dev)
+        if ctx.packed is None:
+            source = (kept[0].data_ptr(), ld_of(kept[0]), None, 0, None)
+        else:
+            source = (None, 0, kept[0].data_ptr(), kept[0].stride(0), kept[1].data_ptr())
+        _lib.call("hgv_group_norm_bwd", g.data_ptr(), ld_of(g), *source, c, groups, act, _lib.ptr(w), _lib.ptr(b), *arrays, *counts,
+                  mean.data_ptr(), rstd.data_ptr(), _lib.ptr(gx), gx.stride(0) if gx is not None else 0, _lib.ptr(gw), _lib.ptr(gb),
+                  ws.data_ptr(), nws, _lib.stream())
         return gx, gw, gb, None, None, None, None, None
 
 
@@ -2655,14 +2675,17 @@ def group_norm_act(x: torch.Tensor, segments, groups: int, weight: Optional[torc
         raise _lib.HgvError(f"eps must be >= 0, got {eps}")
     weight = _check_vector("weight", weight, x.size(1), x.device)
     bias = _check_vector("bias", bias, x.size(1), x.device)
-    with _on_device(x):
-        seg = segments_of(segments, x.size(0))
-        if seg.device != x.device:
-            raise _lib.HgvError(f"segments are on {seg.device}, x is on {x.device}")
-        if x.size(0) == 0:                                      # an empty matrix whose gradients are zeros
-            y = x * 1.0 if weight is None else x * weight
-            return y if bias is None else y + bias
-        return _GroupNormAct.apply(x, weight, bias, seg, groups, _ACTS[act], eps, bool(keep8))
+    return _on_device(x, _group_norm_act, x, segments, groups, weight, bias, _ACTS[act], float(eps), bool(keep8))
+
+
+def _group_norm_act(x, segments, groups, weight, bias, act, eps, keep8):
+    seg = segments_of(segments, x.size(0))
+    if seg.device != x.device:
+        raise _lib.HgvError(f"segments are on {seg.device}, x is on {x.device}")
+    if x.size(0) == 0:                                          # an empty matrix whose gradients are zeros
+        y = x * 1.0 if weight is None else x * weight
+        return y if bias is None else y + bias
+    return _GroupNormAct.apply(x, weight, bias, seg, groups, act, eps, keep8)
 
 
 # --------------------------------------------------------------------------------------
@@ -2694,29 +2717,31 @@ class _GraphAttention(torch.autograd.Function):
         nws = _lib.load().hgv_graph_attention_ws(n, seg.num_graphs, h, hk, d, seg._n_tiles, 0)
         ws = torch.empty(nws, dtype=torch.uint8, device=q.device)
         _lib.call("hgv_graph_attention_fwd", *_strided(q), *_strided(k), *_strided(v), n, seg.num_graphs, h, hk, d, scale, _lib.ptr(mask),
-                  seg._ptr.data_ptr(), seg._sorted[-1], seg._tiles.data_ptr(), seg._n_tiles, seg._blocks.data_ptr(), *seg._n_blocks, out.data_ptr(),
-                  _lib.ptr(lse), ws.data_ptr(), nws, _lib.stream())
+                  *seg._attention_plan, out.data_ptr(), _lib.ptr(lse), ws.data_ptr(), nws, _lib.stream())
         ctx.seg, ctx.scale = seg, scale
         if train:
             ctx.save_for_backward(q, k, v, out, lse, mask)
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_first_order
     def backward(ctx, g):
+        return _on_device(g, _GraphAttention._grads, ctx, g)
+
+    @staticmethod
+    def _grads(ctx, g):
         q, k, v, out, lse, mask = ctx.saved_tensors
         seg, need = ctx.seg, ctx.needs_input_grad
         n, h, d = q.shape
         hk = k.size(1)
-        with _on_device(g):
-            g = _unit_rows(g)
-            dq = torch.empty(n, h, d, dtype=torch.float32, device=q.device) if need[0] else None
-            dk, dv = (torch.empty(n, hk, d, dtype=torch.float32, device=q.device) if need[1] or need[2] else None for _ in range(2))
-            nws = _lib.load().hgv_graph_attention_ws(n, seg.num_graphs, h, hk, d, seg._n_tiles, 1)
-            ws = torch.empty(nws, dtype=torch.uint8, device=q.device)
-            _lib.call("hgv_graph_attention_bwd", *_strided(q), *_strided(k), *_strided(v), *_strided(g), out.data_ptr(), lse.data_ptr(), n,
-                      seg.num_graphs, h, hk, d, ctx.scale, _lib.ptr(mask), seg._ptr.data_ptr(), seg._sorted[-1], seg._tiles.data_ptr(), seg._n_tiles,
-                      seg._blocks.data_ptr(), *seg._n_blocks, _lib.ptr(dq), _lib.ptr(dk), _lib.ptr(dv), ws.data_ptr(), nws, _lib.stream())
+        g = _unit_rows(g)
+        dq = torch.empty(n, h, d, dtype=torch.float32, device=q.device) if need[0] else None
+        dk, dv = (torch.empty(n, hk, d, dtype=torch.float32, device=q.device) if need[1] or need[2] else None for _ in range(2))
+        nws = _lib.load().hgv_graph_attention_ws(n, seg.num_graphs, h, hk, d, seg._n_tiles, 1)
+        ws = torch.empty(nws, dtype=torch.uint8, device=q.device)
+        _lib.call("hgv_graph_attention_bwd", *_strided(q), *_strided(k), *_strided(v), *_strided(g), out.data_ptr(), lse.data_ptr(), n,
+                  seg.num_graphs, h, hk, d, ctx.scale, _lib.ptr(mask), *seg._attention_plan, _lib.ptr(dq), _lib.ptr(dk), _lib.ptr(dv),
+                  ws.data_ptr(), nws, _lib.stream())
         return dq, dk if need[1] else None, dv if need[2] else None, None, None, None
 
 
@@ -2753,10 +2778,13 @@ def graph_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, segments,
         if not isinstance(mask, torch.Tensor) or mask.dtype != torch.bool or mask.shape != (n,) or mask.device != q.device:
             raise _lib.HgvError(f"mask must be a bool vector of {n} on {q.device}")
         mask = mask.contiguous().view(torch.uint8)
-    with _on_device(q):
-        seg = segments_of(segments, n)
-        if seg.device != q.device:
-            raise _lib.HgvError(f"segments are on {seg.device}, q is on {q.device}")
-        if n == 0:
-            return q * 1.0 + (k.sum() + v.sum()) * 0.0          # an empty result whose gradients are zeros
-        return _GraphAttention.apply(q, k, v, seg, mask, scale)
+    return _on_device(q, _graph_attention, q, k, v, segments, mask, scale)
+
+
+def _graph_attention(q, k, v, segments, mask, scale):
+    seg = segments_of(segments, q.size(0))
+    if seg.device != q.device:
+        raise _lib.HgvError(f"segments are on {seg.device}, q is on {q.device}")
+    if q.size(0) == 0:
+        return q * 1.0 + (k.sum() + v.sum()) * 0.0              # an empty result whose gradients are zeros
+    return _GraphAttention.apply(q, k, v, seg, mask, scale)

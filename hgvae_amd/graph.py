@@ -296,12 +296,15 @@ class Segments:
         # attention: tiles of 64 rows in row order, each with the first tile of its graph and their number, and blocks of 64
         # and of 128 rows, those of the largest graphs first
         tiles, blocks = self._tiles_of(sizes, ptr, np.flatnonzero(sizes), 64), [self._tiles_of(sizes, ptr, order[::-1], r) for r in (64, 128)]
-        self._n_tiles, self._n_blocks = len(tiles), [len(b) for b in blocks]
+        self._n_tiles = len(tiles)
         parts = [chunks.ravel(), tiles.ravel(), np.concatenate(blocks).ravel(), ptr, order, first]
         host = np.concatenate(parts).astype(np.int32)
         self._buf = torch.from_numpy(host).to(self.device)          # copied before the call returns: any stream may read it
         at = np.cumsum([0] + [p.size for p in parts])
         self._chunks, self._tiles, self._blocks, self._ptr, self._order, self._first = (self._buf[at[i]:at[i + 1]] for i in range(6))
+        self._norm_plans: "dict[tuple, tuple]" = {}
+        self._attention_plan = (self._ptr.data_ptr(), self._sorted[-1] if self._sorted else 0, self._tiles.data_ptr(), self._n_tiles,
+                                self._blocks.data_ptr(), *map(len, blocks))
 
     @staticmethod
     def _tiles_of(sizes, ptr, graphs, rows: int) -> np.ndarray:
@@ -345,12 +348,21 @@ class Segments:
             count = int(num_graphs)
         return cls(np.bincount(host, minlength=count) if host.size else np.zeros(count, dtype=np.int64), batch.device)
 
-    def _norm_plan(self, small_rows: int):
-        """(graphs that one workgroup reads at once, rows of the largest of them, first chunk of the others, end of the chunks)."""
-        n = bisect.bisect_right(self._sorted, small_rows)
-        if n < len(self._sorted) and 8 * sum(self._sorted[:n]) < self.num_rows:
-            n = 0                       # a few small graphs beside large ones: not worth a launch of their own
-        return n, self._sorted[n - 1] if n else 0, self._first_host[n], self._first_host[-1]
+    def _norm_plan(self, columns: int, groups: int):
+        """What a call of the norm passes on: (device arrays), (graphs, graphs with rows, how many of them one workgroup reads at
+        once, rows of the largest of those, first chunk of the others, end of the chunks), workspace bytes forward and backward."""
+        plan = self._norm_plans.get((columns, groups))
+        if plan is None:
+            lib = _lib.load()
+            n, listed = bisect.bisect_right(self._sorted, lib.hgv_group_norm_small_rows(columns, groups)), len(self._sorted)
+            if n < listed and 8 * sum(self._sorted[:n]) < self.num_rows:
+                n = 0                   # a few small graphs beside large ones: not worth a launch of their own
+            chunks = (self._first_host[n], self._first_host[-1])
+            ws = [lib.hgv_group_norm_ws(chunks[1] - chunks[0], self.num_graphs, listed, n, columns, groups, b) for b in (0, 1)]
+            plan = (tuple(t.data_ptr() for t in (self._ptr, self._order, self._chunks, self._first)),
+                    (self.num_graphs, listed, n, self._sorted[n - 1] if n else 0, *chunks), *ws)
+            self._norm_plans[columns, groups] = plan
+        return plan
 
     def __repr__(self):
         return f"Segments({self.num_graphs} graphs, {self.num_rows} rows, {self.device})"
