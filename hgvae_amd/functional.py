@@ -9,6 +9,7 @@ from __future__ import annotations
 import contextlib
 import functools
 import os
+import weakref
 from typing import Optional
 
 import torch
@@ -2441,13 +2442,45 @@ def _on_device(t: torch.Tensor, fn, *args):
         return fn(*args)
 
 
+class _LeafStream:
+    """The stream on which autograd accumulates one leaf's gradient: where the leaf entered the oldest graph that still lives."""
+    __slots__ = ("stream", "__weakref__")
+
+    def __init__(self, stream):
+        self.stream = stream
+
+
+_leaf_streams: "weakref.WeakValueDictionary[int, _LeafStream]" = weakref.WeakValueDictionary()
+
+
+def _leaves_of(*inputs):
+    """Autograd accumulates a leaf's gradient on the stream on which the leaf first entered a graph that still lives.  A
+    backward pass under capture would pull that stream into the capture, which ends the process where it is the default
+    stream.  Every node below keeps the streams of its leaves, and with them the entries here, for as long as it lives; a
+    leaf's address is not used again before that, since the node keeps the leaf too."""
+    held = []
+    for t in inputs:
+        if t is not None and t.requires_grad and t.is_leaf:
+            s = _leaf_streams.get(id(t))
+            if s is None:
+                s = _leaf_streams[id(t)] = _LeafStream(_lib.stream())
+            held.append(s)
+    return held
+
+
 def _first_order(backward):
-    """Gradients that cannot be differentiated again: a second derivative through them raises.  (torch's own wrapper does this
-    too; it is only entered when a graph of the gradients is being built.)"""
+    """Gradients that cannot be differentiated again: a second derivative through them raises (torch's own wrapper does this
+    too; it is only entered when a graph of the gradients is being built).  A captured backward pass whose leaves are still
+    held by an eager graph of another stream is refused here, before any of its gradients leaves the capture's stream."""
     guarded = torch.autograd.function.once_differentiable(backward)
 
     @functools.wraps(backward)
     def run(ctx, g):
+        if ctx.leaves and torch.cuda.is_current_stream_capturing():
+            here = _lib.stream()
+            if any(s.stream != here for s in ctx.leaves):
+                raise _lib.HgvError("a backward pass cannot be captured while a graph of the same parameters that was built on another "
+                                    "stream is alive: drop its outputs (losses, activations) before the capture")
         return guarded(ctx, g) if torch.is_grad_enabled() else backward(ctx, g)
     return run
 
@@ -2533,6 +2566,7 @@ class _Linear8(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, w, bias):
+        ctx.leaves = _leaves_of(x, w, bias)
         x = _own_rows(x)
         need = ctx.needs_input_grad
         fwd, ctx.image = _images((w, None, False), (w, None, True) if need[0] else None)
@@ -2606,6 +2640,7 @@ class _GroupNormAct(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, w, b, seg: Segments, groups, act, eps, keep8):
+        ctx.leaves = _leaves_of(x, w, b)
         x = rowmajor(x)
         n, c = x.shape
         dev = x.device
@@ -2708,6 +2743,7 @@ class _GraphAttention(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, seg: Segments, mask, scale):
+        ctx.leaves = _leaves_of(q, k, v)
         q, k, v = _unit_rows(q), _unit_rows(k), _unit_rows(v)
         n, h, d = q.shape
         hk = k.size(1)

@@ -1,0 +1,218 @@
+"""The per-graph operators together, as levels of a deeper encoder use them: norm and activation, projection, attention, residual."""
+import gc
+import math
+
+import pytest
+import torch
+from torch import nn
+
+from test_gpu_group_norm import values8
+
+pytestmark = pytest.mark.gpu
+
+FWD_RTOL, BWD_RTOL = 1e-5, 1e-4          # norm-wise, the tolerances of the other operators of the package
+
+
+def dev():
+    return torch.device("cuda:0")
+
+
+class Level(nn.Module):
+    """x + attention(linear(act(norm(x))))"""
+
+    def __init__(self, channels, groups, heads, kv_heads, keep8):
+        super().__init__()
+        from hgvae_amd.nn import GraphAttention, GroupNormAct, Linear8
+        self.norm = GroupNormAct(channels, groups, "silu", keep8=keep8)
+        self.lin = Linear8(channels, channels) if keep8 else nn.Linear(channels, channels)
+        self.att = GraphAttention(channels, heads, kv_heads, head_dim=channels // heads, keep8=keep8)
+        self.keep8 = keep8
+
+    def forward(self, x, segments, mask=None):
+        from hgvae_amd import functional as Fn
+        h = self.norm(x, segments)
+        h = self.lin(h) if self.keep8 else Fn.dual_linear(h, self.lin.weight, bias=self.lin.bias)
+        return x + self.att(h, segments, mask)
+
+
+def reference(level, x, sizes, mask):
+    """The same level in float64 torch operations on parameters given by name."""
+    p = {k: v for k, v in level.items()}
+    n, c = x.shape
+    heads, kv, groups = p["heads"], p["kv"], p["groups"]
+    out, at = [], 0
+    for s in sizes:
+        r = slice(at, at + s)
+        at += s
+        if s == 0:
+            continue
+        g = x[r].reshape(s, groups, c // groups)
+        mean = g.mean((0, 2), keepdim=True)
+        xh = (g - mean) / torch.sqrt(((g - mean) ** 2).mean((0, 2), keepdim=True) + 1e-5)
+        z = xh.reshape(s, c) * p["norm.weight"] + p["norm.bias"]
+        h = (z * torch.sigmoid(z)) @ p["lin.weight"].t() + p["lin.bias"]
+        q, k, v = ((h @ p[f"att.lin_{t}.weight"].t()).unflatten(1, (-1, c // heads)).transpose(0, 1) for t in "qkv")
+        k, v = (t.repeat_interleave(heads // kv, 0) for t in (k, v))
+        a = q @ k.transpose(1, 2) / math.sqrt(c // heads)
+        if mask is not None:
+            a = a.masked_fill(~mask[r], -math.inf)
+        o = (torch.softmax(a, -1) @ v).transpose(0, 1).reshape(s, c)
+        out.append(x[r] + o @ p["att.lin_out.weight"].t() + p["att.lin_out.bias"])
+    return torch.cat(out)
+
+
+@pytest.mark.parametrize("sizes,c,groups,heads,kv", [([138, 1, 60], 138, 6, 6, 2), ([40, 0, 300], 64, 8, 4, 4), ([2], 96, 1, 1, 1)])
+@pytest.mark.parametrize("masked", [False, True])
+def test_two_levels_match_float64(sizes, c, groups, heads, kv, masked):
+    from hgvae_amd import Segments
+    torch.manual_seed(c)
+    n = sum(sizes)
+    levels = [Level(c, groups, heads, kv, False).to(dev()) for _ in range(2)]
+    x = torch.randn(n, c, device=dev())
+    g = torch.randn(n, c, device=dev())
+    mask = None
+    if masked:
+        mask = torch.rand(n, device=dev()) < 0.7
+        at = 0
+        for s in sizes:
+            if s:
+                mask[at] = True                                 # the dense softmax of the reference has no empty rows
+            at += s
+    seg = Segments.from_sizes(sizes, dev())
+    xr = x.clone().requires_grad_()
+    out = levels[1](levels[0](xr, seg, mask), seg, mask)
+    out.backward(g)
+    x64 = x.double().cpu().requires_grad_()
+    params = []
+    h = x64
+    for level in levels:
+        p = {k: v.detach().double().cpu().requires_grad_() for k, v in level.named_parameters()}
+        params.append(p)
+        h = reference({**p, "heads": heads, "kv": kv, "groups": groups}, h, sizes, None if mask is None else mask.cpu())
+    h.backward(g.double().cpu())
+
+    def close(a, b, rtol, what):
+        a, b = a.detach().double().cpu(), b.detach()
+        assert (a - b).abs().max() <= rtol * b.abs().max() + 1e-6, what
+
+    close(out, h, FWD_RTOL, "out")
+    close(xr.grad, x64.grad, BWD_RTOL, "x")
+    for level, p in zip(levels, params):
+        for name, q in level.named_parameters():
+            close(q.grad, p[name].grad, BWD_RTOL, name)
+
+
+def test_8bit_level_is_the_sum_of_its_parts():
+    """Autograd through a level whose inputs are kept in 8 bits, against its operators called one by one with the gradients
+    handed on by hand.  The forward result is that of the level which keeps everything."""
+    from hgvae_amd import Segments
+    from hgvae_amd import functional as Fn
+    sizes, c = [70, 300], 64
+    torch.manual_seed(3)
+    level = Level(c, 8, 4, 2, True).to(dev())
+    seg = Segments.from_sizes(sizes, dev())
+    x, g = torch.randn(370, c, device=dev()), torch.randn(370, c, device=dev())
+    xr = x.clone().requires_grad_()
+    out = level(xr, seg)
+    out.backward(g)
+    full = Level(c, 8, 4, 2, False).to(dev())
+    full.load_state_dict(level.state_dict())
+    assert torch.equal(full(x, seg), out)
+
+    def leaf(t):
+        return t.detach().requires_grad_()
+
+    a = level.att
+    x0 = leaf(x)
+    h0 = Fn.group_norm_act(x0, seg, 8, level.norm.weight, level.norm.bias, keep8=True)
+    x1 = leaf(h0)
+    h1 = Fn.linear8(x1, level.lin.weight, level.lin.bias)
+    x2 = leaf(h1)
+    qkv = [Fn.linear8(x2, lin.weight) for lin in (a.lin_q, a.lin_k, a.lin_v)]
+    q, k, v = (leaf(t.unflatten(1, (-1, 16))) for t in qkv)
+    o = Fn.graph_attention(q, k, v, seg)
+    x3 = leaf(o.reshape(370, c))
+    y = Fn.linear8(x3, a.lin_out.weight, a.lin_out.bias)
+    grads = {}
+    g3, grads["att.lin_out.weight"], grads["att.lin_out.bias"] = torch.autograd.grad(y, (x3, a.lin_out.weight, a.lin_out.bias), g)
+    gq = torch.autograd.grad(o, (q, k, v), g3.view(370, 4, 16))
+    parts = [torch.autograd.grad(t, (x2, lin.weight), gt.reshape(370, -1)) for t, lin, gt in zip(qkv, (a.lin_q, a.lin_k, a.lin_v), gq)]
+    for name, (_, gw) in zip("qkv", parts):
+        grads[f"att.lin_{name}.weight"] = gw
+    g1, grads["lin.weight"], grads["lin.bias"] = torch.autograd.grad(h1, (x1, level.lin.weight, level.lin.bias), parts[2][0] + parts[1][0] + parts[0][0])
+    g0, grads["norm.weight"], grads["norm.bias"] = torch.autograd.grad(h0, (x0, level.norm.weight, level.norm.bias), g1)
+    for name, p in level.named_parameters():
+        # autograd may add the three gradients of h in another order: one rounding of each of two sums
+        bound = 0.0 if name.startswith("att") else 1e-5 * float(grads[name].abs().max())
+        assert float((p.grad - grads[name]).abs().max()) <= bound, name
+    assert float((xr.grad - (g0 + g)).abs().max()) <= 1e-5 * float(g0.abs().max())
+
+
+def test_8bit_weight_gradient_is_within_half_a_step():
+    from hgvae_amd import functional as Fn
+    gen = torch.Generator(device=dev()).manual_seed(5)
+    x, w, g = (torch.randn(*s, generator=gen, device=dev()) for s in ((900, 138), (40, 138), (900, 40)))
+    wr = w.clone().requires_grad_()
+    (g8,) = torch.autograd.grad(Fn.linear8(x, wr), (wr,), g)
+    exact = g.double().t() @ x.double()
+    off = (values8(x) - x.double()).abs()
+    bound = g.double().abs().t() @ off
+    assert bool(((g8.double() - exact).abs() <= bound + 1e-4 * exact.abs().max()).all())
+    assert float((g8.double() - exact).norm() / exact.norm()) < 0.01        # steps of 1/63 at most, errors of both signs
+
+
+def test_captured_training_step_replays_as_eager():
+    """Forward and backward of an 8-bit level replayed from one HIP graph, eager steps between the replays.  While an eager
+    graph of the same leaves lives, the captured backward pass is refused with an error; once it is gone the capture works."""
+    from hgvae_amd import Segments
+    from hgvae_amd._lib import HgvError
+    sizes, c = [138, 90], 64
+    torch.manual_seed(6)
+    level = Level(c, 8, 4, 4, True).to(dev())
+    seg = Segments.from_sizes(sizes, dev())
+    data = [torch.randn(228, c, device=dev()) for _ in range(2)]
+    g = torch.randn(228, c, device=dev())
+    params = list(level.parameters())
+    static = data[0].clone()
+
+    def step(x):
+        out = level(x, seg)
+        return (out.detach(), *torch.autograd.grad(out, params, g))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(static)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    alive = level(data[1], seg)                                  # an eager graph over the same leaves
+    with pytest.raises(HgvError, match="alive"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            step(static)
+    torch.autograd.grad(alive, params, g)                        # the eager graph itself is as good as before
+    del alive
+    gc.collect()                                                 # what the refused call left
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step(static)
+    for i in (0, 1, 0, 1):
+        static.copy_(data[i])
+        graph.replay()
+        torch.cuda.synchronize()
+        want = step(data[i])
+        assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
+def test_modules_repr_and_second_derivatives_are_refused():
+    from hgvae_amd import Segments
+    from hgvae_amd import functional as Fn
+    from hgvae_amd.nn import GraphAttention, GroupNormAct
+    assert "groups=3" in repr(GroupNormAct(12, 3)) and "heads=4" in repr(GraphAttention(64, 4, 2))
+    seg = Segments.from_sizes([5, 4], dev())
+    x = torch.randn(9, 12, device=dev(), requires_grad=True)
+    w = torch.randn(12, 12, device=dev(), requires_grad=True)
+    q = torch.randn(9, 2, 6, device=dev(), requires_grad=True)
+    for out, leaf in ((Fn.group_norm_act(x, seg, 3), x), (Fn.linear8(x, w), x), (Fn.graph_attention(q, q, q, seg), q)):
+        (first,) = torch.autograd.grad((out ** 2).sum(), (leaf,), create_graph=True)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(first.sum(), (leaf,))
