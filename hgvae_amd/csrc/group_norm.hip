@@ -19,6 +19,8 @@
 
 namespace {
 
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
 enum { ACT_NONE = 0, ACT_RELU = 1, ACT_SILU = 2, ACT_GELU = 3 };
 
 template <int ACT>
@@ -407,7 +409,7 @@ template <int VEC, int ACT, bool BWD, bool Q8>
 __global__ __launch_bounds__(256) void k_gn_apply(const GnArgs a, const int chunk0) {
     const GnLane l = gn_lane<VEC>(a);
     if (!l.live) return;
-    const int4 ch = a.chunks[chunk0 + blockIdx.x];
+    const int4 ch = a.chunks[chunk0 + (int)(gridDim.x - 1 - blockIdx.x)];
     GnCols<VEC> k;
     gn_cols<VEC>(a, ch.x, l.c, k);
     float m1[VEC], m2[VEC];
@@ -439,7 +441,8 @@ __global__ __launch_bounds__(256) void k_gn_apply(const GnArgs a, const int chun
 #pragma unroll
             for (int i = 0; i < VEC; ++i)
                 if (l.c + i >= a.C) o[i] = 0.f;                 // pad columns
-            *(float4*)(a.out + (int64_t)n * a.ldo + l.c) = make_float4(o[0], o[VEC > 1 ? 1 : 0], o[VEC > 2 ? 2 : 0], o[VEC > 3 ? 3 : 0]);
+            const f32x4 t = {o[0], o[VEC > 1 ? 1 : 0], o[VEC > 2 ? 2 : 0], o[VEC > 3 ? 3 : 0]};
+            __builtin_nontemporal_store(t, (f32x4*)(a.out + (int64_t)n * a.ldo + l.c));
         } else {
             store1(a, n, l.c, o[0]);
         }
