@@ -54,9 +54,11 @@ struct GnArgs {
     const int32_t* first_chunk;       // [listed + 1] first chunk of the k-th graph of that order
     float* out; int64_t ldo;          // out or gx
     double* mean; float* rstd;        // [B, groups]
+    int64_t rows;                     // of x, where its 8-bit form is kept
     double2* part;                    // [chunk][C] sums over a chunk's rows, from the first chunk of a larger graph on
     double2* colsum;                  // [rows of colsum][C] column sums (dz * xh, dz): one row per small workgroup, then per large graph
     float2* gsum;                     // [B, groups] mean(a), mean(a * xh)
+    int8_t* keep; uint8_t* keep_scale;                              // forward: where the 8-bit form of x goes (leading dimension ldq)
     int n_small, slab, nslabs, pad;   // pad: columns behind the last one that rows of out have for 16-byte access (zeroed)
 };
 
@@ -244,11 +246,12 @@ __device__ __forceinline__ void load_g(const GnArgs& a, int64_t n, int c, float 
 
 // thread -> (column block, row) of a chunk
 struct GnLane { int c, ty, ty_n, tx, tx_n; bool live; };
-template <int VEC>
+template <int VEC, bool PACK = false>                           // PACK: eight lanes to a block of 32 columns, also to the last one
 __device__ __forceinline__ GnLane gn_lane(const GnArgs& a) {
     GnLane l;
     const int c0 = blockIdx.y * 256 * VEC;
     l.tx_n = min(256, (a.C - c0 + VEC - 1) / VEC);
+    if (PACK) l.tx_n = (l.tx_n + 7) & ~7;
     l.ty_n = 256 / l.tx_n;
     l.ty = threadIdx.x / l.tx_n;
     l.tx = threadIdx.x - l.ty * l.tx_n;
@@ -405,10 +408,14 @@ __global__ __launch_bounds__(1024) void k_gn_join(const GnArgs a, const int chun
     }
 }
 
-template <int VEC, int ACT, bool BWD, bool Q8>
+// Streaming stores (the output does not push out what is read again: 8 bundled graphs 60 -> 51 us), and the chunks from the last to
+// the first, since the last ones read by the sums are the ones still in the memory-side cache (1.28 M x 138: 2 %).  PACK: the 8-bit
+// form of x on the way.
+template <int VEC, int ACT, bool BWD, bool Q8, bool PACK = false>
 __global__ __launch_bounds__(256) void k_gn_apply(const GnArgs a, const int chunk0) {
-    const GnLane l = gn_lane<VEC>(a);
-    if (!l.live) return;
+    static_assert(!PACK || (VEC == 4 && !BWD && !Q8), "packs x where it is read in 16 bytes");
+    const GnLane l = gn_lane<VEC, PACK>(a);
+    if (!l.live) return;                                        // whole blocks of eight lanes leave: the maxima below stay inside one
     const int4 ch = a.chunks[chunk0 + (int)(gridDim.x - 1 - blockIdx.x)];
     GnCols<VEC> k;
     gn_cols<VEC>(a, ch.x, l.c, k);
@@ -420,10 +427,29 @@ __global__ __launch_bounds__(256) void k_gn_apply(const GnArgs a, const int chun
             m1[i] = t.x; m2[i] = t.y;
         }
     }
+    const bool stored = !PACK || l.c < a.C;
 #pragma unroll 1
     for (int n = ch.y + l.ty; n < ch.z; n += l.ty_n) {
         float v[VEC], o[VEC];
-        load_x<VEC, Q8>(a, n, l.c, v);
+        if (stored) {
+            load_x<VEC, Q8>(a, n, l.c, v);
+        } else {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) v[i] = 0.f;
+        }
+        if (PACK) {
+            float p[4];
+            uint32_t m = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                p[i] = l.c + i < a.C ? v[VEC > i ? i : 0] : 0.f;
+                m = max(m, __float_as_uint(p[i]) & 0x7fffffffu);
+            }
+            const int byte = p8_byte(p8_max8(m));
+            const uint32_t w = p8_quantise4(p, byte);
+            if (l.c < a.ldq) __builtin_nontemporal_store(w, (uint32_t*)(a.keep + (int64_t)n * a.ldq + l.c));
+            if ((threadIdx.x & 7) == 0) a.keep_scale[(int64_t)n * a.nb + (l.c >> 5)] = (uint8_t)byte;
+        }
         if (BWD) {
             float g[VEC];
             load_g<VEC>(a, n, l.c, g);
@@ -442,7 +468,7 @@ __global__ __launch_bounds__(256) void k_gn_apply(const GnArgs a, const int chun
             for (int i = 0; i < VEC; ++i)
                 if (l.c + i >= a.C) o[i] = 0.f;                 // pad columns
             const f32x4 t = {o[0], o[VEC > 1 ? 1 : 0], o[VEC > 2 ? 2 : 0], o[VEC > 3 ? 3 : 0]};
-            __builtin_nontemporal_store(t, (f32x4*)(a.out + (int64_t)n * a.ldo + l.c));
+            if (stored) __builtin_nontemporal_store(t, (f32x4*)(a.out + (int64_t)n * a.ldo + l.c));
         } else {
             store1(a, n, l.c, o[0]);
         }
@@ -506,6 +532,13 @@ int gn_launch(const GnArgs& a, int listed, int small_rows, int chunk0, int chunk
                      (!BWD || (hgv_aligned(a.g, 16) && a.ldg % 4 == 0 && a.ldg >= (a.C + 3) / 4 * 4)) &&
                      (!a.out || (hgv_aligned(a.out, 16) && a.ldo % 4 == 0 && a.ldo >= (a.C + 3) / 4 * 4));
     const unsigned slabs = (unsigned)hgv_cdiv(a.C, vec ? 1024 : 256);
+    // The 8-bit form: with the last pass where that reads every row (320 000 rows forward: 20 columns 50 -> 46 us, 138 columns
+    // 127 -> 110, 256 columns 248 -> 197), else by itself.
+    const bool keeps = !BWD && a.keep && vec && a.n_small == 0;
+    if (!BWD && a.keep && !keeps) {
+        const int rc = hgv_pack8(a.x, a.ldx, a.rows, a.C, a.keep, a.ldq, a.keep_scale, stream);
+        if (rc) return rc;
+    }
     if (listed > a.n_small) {
         const dim3 grid((unsigned)(chunk1 - chunk0), slabs);
         if (vec) hipLaunchKernelGGL((k_gn_sums<4, ACT, BWD, Q8>), grid, dim3(256), 0, stream, a, chunk0);
@@ -513,7 +546,8 @@ int gn_launch(const GnArgs& a, int listed, int small_rows, int chunk0, int chunk
         hipLaunchKernelGGL(k_gn_join<BWD>, dim3((unsigned)(listed - a.n_small), (unsigned)a.nslabs), dim3(1024), 0, stream, a, chunk0,
                            small_wgs);
         if (a.out) {
-            if (vec) hipLaunchKernelGGL((k_gn_apply<4, ACT, BWD, Q8>), grid, dim3(256), 0, stream, a, chunk0);
+            if (!BWD && keeps) hipLaunchKernelGGL((k_gn_apply<4, ACT, false, false, true>), grid, dim3(256), 0, stream, a, chunk0);
+            else if (vec) hipLaunchKernelGGL((k_gn_apply<4, ACT, BWD, Q8>), grid, dim3(256), 0, stream, a, chunk0);
             else hipLaunchKernelGGL((k_gn_apply<1, ACT, BWD, Q8>), grid, dim3(256), 0, stream, a, chunk0);
         }
     }
@@ -549,14 +583,15 @@ extern "C" size_t hgv_group_norm_ws(int64_t n_chunks, int num_graphs, int listed
     return n + 256;
 }
 
-extern "C" int hgv_group_norm_fwd(const float* x, int64_t ldx, int C, int groups, int act, float eps, const float* w, const float* b,
+static int gn_fwd(const float* x, int64_t ldx, int C, int groups, int act, float eps, const float* w, const float* b,
                                   const int32_t* ptr, const int32_t* order, const int32_t* chunks, const int32_t* first_chunk,
                                   int num_graphs, int listed, int n_small, int small_rows, int chunk0, int chunk1,
-                                  float* out, int64_t ldo, double* mean, float* rstd, void* ws, size_t ws_bytes, hipStream_t stream) {
+                                  int64_t rows, int8_t* q, int64_t ldq, uint8_t* scale, float* out, int64_t ldo, double* mean, float* rstd, void* ws, size_t ws_bytes, hipStream_t stream) {
     GnArgs a = {};
     a.x = x; a.ldx = ldx; a.C = C; a.groups = groups; a.per = groups > 0 ? C / groups : 0; a.eps = eps; a.w = w; a.b = b;
     a.ptr = ptr; a.order = order; a.chunks = (const int4*)chunks; a.first_chunk = first_chunk; a.out = out; a.ldo = ldo;
     a.mean = mean; a.rstd = rstd; a.n_small = n_small;
+    a.rows = rows; a.keep = q; a.ldq = ldq; a.keep_scale = scale; a.nb = (C + 31) / 32;
     const int rc = gn_check(a, num_graphs, listed, n_small, small_rows, chunk0, chunk1, "group_norm_fwd");
     if (rc) return rc;
     HGV_REQUIRE(x && out && ldx >= C && ldo >= C, HGV_EINVAL, "group_norm_fwd: null buffer or bad leading dimension");
@@ -574,6 +609,25 @@ extern "C" int hgv_group_norm_fwd(const float* x, int64_t ldx, int C, int groups
     }
     hgv_set_error("group_norm_fwd: unknown activation %d", act);
     return HGV_EINVAL;
+}
+
+extern "C" int hgv_group_norm_fwd(const float* x, int64_t ldx, int C, int groups, int act, float eps, const float* w, const float* b,
+                                  const int32_t* ptr, const int32_t* order, const int32_t* chunks, const int32_t* first_chunk,
+                                  int num_graphs, int listed, int n_small, int small_rows, int chunk0, int chunk1,
+                                  float* out, int64_t ldo, double* mean, float* rstd, void* ws, size_t ws_bytes, hipStream_t stream) {
+    return gn_fwd(x, ldx, C, groups, act, eps, w, b, ptr, order, chunks, first_chunk, num_graphs, listed, n_small, small_rows, chunk0, chunk1,
+                  0, nullptr, 0, nullptr, out, ldo, mean, rstd, ws, ws_bytes, stream);
+}
+
+extern "C" int hgv_group_norm_fwd8(const float* x, int64_t ldx, int C, int groups, int act, float eps, const float* w, const float* b,
+                                   const int32_t* ptr, const int32_t* order, const int32_t* chunks, const int32_t* first_chunk,
+                                   int num_graphs, int listed, int n_small, int small_rows, int chunk0, int chunk1, int64_t rows,
+                                   int8_t* q, int64_t ldq, uint8_t* scale, float* out, int64_t ldo, double* mean, float* rstd, void* ws,
+                                   size_t ws_bytes, hipStream_t stream) {
+    HGV_REQUIRE(rows > 0 && q && scale && ldq >= C && ldq % 16 == 0 && ldq <= 32 * (int64_t)((C + 31) / 32) && hgv_aligned(q, 16), HGV_EINVAL,
+                "group_norm_fwd8: null / misaligned buffer or bad leading dimension");
+    return gn_fwd(x, ldx, C, groups, act, eps, w, b, ptr, order, chunks, first_chunk, num_graphs, listed, n_small, small_rows, chunk0, chunk1,
+                  rows, q, ldq, scale, out, ldo, mean, rstd, ws, ws_bytes, stream);
 }
 
 template <bool Q8>

@@ -2,12 +2,20 @@
 #pragma once
 #include "common.h"
 
+extern "C" int hgv_pack8(const float* x, int64_t ldx, int64_t N, int C, int8_t* q, int64_t ldq, uint8_t* scale, hipStream_t stream);
+
 // Byte of a block from the bits of its largest magnitude (compared as integers: a NaN or infinity wins).
 __device__ __forceinline__ int p8_byte(uint32_t amax) {
     const int field = (int)(amax >> 23);
     if (field == 255) return 255;
     // 127.5 * 2^e = 1.9921875 * 2^(e + 6): the mantissa field alone decides.  e stays at 121: 128 * 2^121 would not be finite
     return min(max(field - 6 + ((amax & 0x7fffffu) >= 0x7f0000u ? 1 : 0), 1), 248);
+}
+
+__device__ __forceinline__ uint32_t p8_max8(uint32_t v) {       // over the eight lanes of a block
+    v = max(v, (uint32_t)__shfl_xor((int)v, 1, 64));
+    v = max(v, (uint32_t)__shfl_xor((int)v, 2, 64));
+    return max(v, (uint32_t)__shfl_xor((int)v, 4, 64));
 }
 
 __device__ __forceinline__ uint32_t p8_quantise4(const float v[4], int byte) {

@@ -10,11 +10,7 @@
 
 namespace {
 
-__device__ __forceinline__ uint32_t max8(uint32_t v) {          // over the eight lanes of a block
-    v = max(v, (uint32_t)__shfl_xor((int)v, 1, 64));
-    v = max(v, (uint32_t)__shfl_xor((int)v, 2, 64));
-    return max(v, (uint32_t)__shfl_xor((int)v, 4, 64));
-}
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 // Eight lanes take one block of 32 columns of one row (a lane four columns); the 32 lane groups of a workgroup cover
 // floor(32 / blocks) rows at a time (wide matrices: 32 blocks of one row, further blocks in blockIdx.y), and walk rows with
@@ -48,7 +44,7 @@ __global__ __launch_bounds__(256) void k_pack8(const float* __restrict__ x, int6
         uint32_t m = 0;
 #pragma unroll
         for (int i = 0; i < 4; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
-        const int byte = p8_byte(max8(m));
+        const int byte = p8_byte(p8_max8(m));
         const uint32_t packed = p8_quantise4(v, byte);
         if (c < ldq) *(uint32_t*)(q + n * ldq + c) = packed;
         if (sub == 0) scale[n * nb + j] = (uint8_t)byte;
@@ -71,7 +67,7 @@ __global__ __launch_bounds__(256) void k_unpack8(const int8_t* __restrict__ q, i
         float v[4];
         p8_values4(w, scale[n * nb + j], v);
         float* p = out + n * ldo + c;
-        if (VEC) *(float4*)p = make_float4(v[0], v[1], v[2], v[3]);       // bytes behind the last column are zero
+        if (VEC) __builtin_nontemporal_store(f32x4{v[0], v[1], v[2], v[3]}, (f32x4*)p);      // bytes behind the last column are zero
         else {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
@@ -144,7 +140,6 @@ namespace {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int T8_ROWS = 32, T8_W = 144, T8_LINE = 2 * T8_W, T8_PIECE = T8_ROWS * T8_LINE, T8_BUF = 4 * T8_PIECE, T8_LDS = 2 * T8_BUF + T8_ROWS * 32, T8_THREADS = 576;
 constexpr int T8_SET = (81 + 9) * 256;                          // floats of a partial set: 81 tiles, nine tiles of column sums

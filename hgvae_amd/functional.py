@@ -2541,15 +2541,18 @@ def pack8(x: torch.Tensor) -> Packed8:
     return _on_device(x, _pack8, x)
 
 
+def _empty8(n: int, c: int, device) -> Packed8:
+    q = torch.empty(n, (c + 15) // 16 * 16, dtype=torch.int8, device=device)
+    return Packed8(q, torch.empty(n, (c + 31) // 32, dtype=torch.uint8, device=device), (n, c))
+
+
 def _pack8(x: torch.Tensor) -> Packed8:
     x = rowmajor(x)
     n, c = x.shape
-    ldq = (c + 15) // 16 * 16
-    q = torch.empty(n, ldq, dtype=torch.int8, device=x.device)
-    scale = torch.empty(n, (c + 31) // 32, dtype=torch.uint8, device=x.device)
+    p = _empty8(n, c, x.device)
     if n:
-        _lib.call("hgv_pack8", x.data_ptr(), ld_of(x), n, c, q.data_ptr(), ldq, scale.data_ptr(), _lib.stream())
-    return Packed8(q, scale, (n, c))
+        _lib.call("hgv_pack8", x.data_ptr(), ld_of(x), n, c, p.q.data_ptr(), p.q.stride(0), p.scale.data_ptr(), _lib.stream())
+    return p
 
 
 def _own_rows(t: torch.Tensor) -> torch.Tensor:
@@ -2649,15 +2652,17 @@ class _GroupNormAct(torch.autograd.Function):
         rstd = torch.empty(seg.num_graphs, groups, dtype=torch.float32, device=dev)
         arrays, counts, nws, _ = seg._norm_plan(c, groups)
         ws = torch.empty(nws, dtype=torch.uint8, device=dev)
-        _lib.call("hgv_group_norm_fwd", x.data_ptr(), ld_of(x), c, groups, act, eps, _lib.ptr(w), _lib.ptr(b), *arrays, *counts,
-                  out.data_ptr(), out.stride(0), mean.data_ptr(), rstd.data_ptr(), ws.data_ptr(), nws, _lib.stream())
+        head = (x.data_ptr(), ld_of(x), c, groups, act, eps, _lib.ptr(w), _lib.ptr(b), *arrays, *counts)
+        tail = (out.data_ptr(), out.stride(0), mean.data_ptr(), rstd.data_ptr(), ws.data_ptr(), nws, _lib.stream())
         ctx.seg, ctx.cfg = seg, (groups, act)
         ctx.packed = None
         if keep8 and any(ctx.needs_input_grad[:3]):
-            p = _pack8(x)
+            p = _empty8(n, c, dev)
+            _lib.call("hgv_group_norm_fwd8", *head, n, p.q.data_ptr(), p.q.stride(0), p.scale.data_ptr(), *tail)
             ctx.packed = p.shape
             ctx.save_for_backward(w, b, mean, rstd, p.q, p.scale)
         else:
+            _lib.call("hgv_group_norm_fwd", *head, *tail)
             ctx.save_for_backward(w, b, mean, rstd, x)
         return out
 

@@ -586,13 +586,18 @@ int hgv_gemm_tn8(const float* G, int64_t ldg, int N, const int8_t* q, int64_t ld
  * row, unused) of the listed graphs in that order; first_chunk [listed + 1].  The first n_small graphs of the list (none
  * above small_rows <= hgv_group_norm_small_rows(C, groups) rows) are read once; the others take chunks chunk0 .. chunk1 - 1.
  * mean [num_graphs, groups] fp64 and rstd [num_graphs, groups] are written by the forward and read by the backward pass
- * (entries of graphs without rows are left as they were).
+ * (entries of graphs without rows are left as they were).  hgv_group_norm_fwd8 also writes the 8-bit form of x (its rows 0 .. rows
+ * - 1, as hgv_pack8), in its last pass where that reads all of them.
  * Backward: from x, or (q != NULL) from its 8-bit form; gx, gw [C], gb [C] are written where not NULL. */
 int hgv_group_norm_small_rows(int C, int groups);
 size_t hgv_group_norm_ws(int64_t n_chunks, int num_graphs, int listed, int n_small, int C, int groups, int backward);
 int hgv_group_norm_fwd(const float* x, int64_t ldx, int C, int groups, int act, float eps, const float* w, const float* b,
                        const int32_t* ptr, const int32_t* order, const int32_t* chunks, const int32_t* first_chunk, int num_graphs,
                        int listed, int n_small, int small_rows, int chunk0, int chunk1, float* out, int64_t ldo, double* mean, float* rstd, void* ws, size_t ws_bytes, hgv_stream_t stream);
+int hgv_group_norm_fwd8(const float* x, int64_t ldx, int C, int groups, int act, float eps, const float* w, const float* b,
+                        const int32_t* ptr, const int32_t* order, const int32_t* chunks, const int32_t* first_chunk, int num_graphs,
+                        int listed, int n_small, int small_rows, int chunk0, int chunk1, int64_t rows, int8_t* q, int64_t ldq,
+                        uint8_t* scale, float* out, int64_t ldo, double* mean, float* rstd, void* ws, size_t ws_bytes, hgv_stream_t stream);
 int hgv_group_norm_bwd(const float* g, int64_t ldg, const float* x, int64_t ldx, const int8_t* q, int64_t ldq, const uint8_t* scale,
                        int C, int groups, int act, const float* w, const float* b, const int32_t* ptr, const int32_t* order,
                        const int32_t* chunks, const int32_t* first_chunk, int num_graphs, int listed, int n_small, int small_rows,

@@ -359,3 +359,22 @@ def test_refusals():
                  lambda: Segments.from_sizes([1.5], dev()), lambda: Segments.from_sizes([3], "cpu")):
         with pytest.raises(_lib.HgvError):
             call()
+
+
+@pytest.mark.parametrize("sizes", [[700, 2500], [3, 0, 2100], [1100]])
+@pytest.mark.parametrize("c,groups", [(36, 3), (64, 4), (65, 5), (138, 6), (256, 8), (1100, 2)])
+def test_kept_input_is_its_8bit_form(sizes, c, groups):
+    """What the forward pass leaves for the backward pass, with its last pass or by itself: the bytes of pack8(x)."""
+    from hgvae_amd import Segments
+    from hgvae_amd import functional as Fn
+    n = sum(sizes)
+    wide = torch.randn(n, c + 7, device=dev()) * torch.logspace(-3, 3, c + 7, device=dev())
+    wide[n // 2, c // 2], wide[n // 3, 0], wide[1, c - 1] = float("nan"), float("inf"), 3e38
+    seg = Segments.from_sizes(sizes, dev())
+    for x in (wide[:, :c].contiguous(), wide[:, 3:c + 3], wide[:, 7:]):
+        out = Fn.group_norm_act(x.detach().requires_grad_(), seg, groups, keep8=True)
+        want = Fn.pack8(x)
+        kept = [t for t in out.grad_fn.saved_tensors if t is not None and t.dtype in (torch.int8, torch.uint8)]
+        assert torch.equal(kept[0][:, :c], want.q[:, :c]) and torch.equal(kept[1], want.scale)
+        assert torch.equal(Fn.group_norm_act(x, seg, groups).isnan(), out.isnan())
+        assert torch.equal(Fn.group_norm_act(x, seg, groups).nan_to_num(), out.detach().nan_to_num())
