@@ -16,7 +16,7 @@
 // of two - whenever a later chunk would exceed 2^15 with it (fp16 overflows at 2^16).  Entries far below the row's
 // largest keep an absolute accuracy of 2^-25 (fp16 subnormal spacing) on the 2^12 scale, i.e. 2^-37 of the row maximum.
 // Layout of the image, LDS residency, the two-part launch and its pacing are those of the bf16 kernel.
-#include "common.h"
+#include "pack8.h"
 #include <type_traits>
 #include <utility>
 
@@ -203,6 +203,8 @@ struct NtHArgs {
     // passes of a train step, gvae/gvae_skipcon.py:166-171): C and stat_partial take the draw of act_bits, C2 and stat_partial2
     // the draw of act_bits2 (same leading dimensions)
     float* C2; const uint32_t* act_bits2; float* stat_partial2;
+    // ACT = 6: plain store, and the 8-bit form of A1 (its values are in the movers' registers anyway): q and the byte per block of 32
+    int8_t* keep_q; int64_t keep_ldq; uint8_t* keep_scale;
 };
 
 template <int CTRL> __device__ __forceinline__ float dpp_mov(float x) {
@@ -765,7 +767,8 @@ __global__ __launch_bounds__(MAXT) void k_gemm_nt16r(const NtHArgs a) {
     // loads are counted ones) and hand them over here: a load inside the multipliers' loop made every interval wait for the
     // completion of the store in front of it
     uint32_t* kbits = reinterpret_cast<uint32_t*>(rowinv + 2 * R);
-    constexpr bool BWD = ACT == 3 || ACT == 4, KEEP = ACT == 1 || ACT == 2 || ACT == 5, PAIR = ACT == 5;
+    constexpr bool BWD = ACT == 3 || ACT == 4, KEEP = ACT == 1 || ACT == 2 || ACT == 5, PAIR = ACT == 5, P8 = ACT == 6;
+    static_assert(!P8 || NSRC == 1, "one source is kept");
     constexpr int KW = 16;                                           // words per row in the ring: 8 per draw
     // ACT = 3: the rows of d that belong to the last four blocks of output, [4][R][NTR_LDC], handed over by the movers likewise
     float* dring = reinterpret_cast<float*>(kbits + 4 * R * KW);
@@ -939,14 +942,26 @@ __global__ __launch_bounds__(MAXT) void k_gemm_nt16r(const NtHArgs a) {
     } else {
         // ---- mover thread (row mr of the block, lane mj of the row's 16): float4 f = min(mj, 11) + 12 u (u = 0, 1, 2) of the row,
         // the last one repeated where the row is shorter - same loads, same staged bytes; lanes 12 ... 15 repeat lane 11
-        const int tl = t - mwaves * 64, mr = tl >> 4, mj = min(tl & 15, 11);
+        // (P8: half j of the sixteen lanes takes block 2 u + j of 32 columns, so that a block's maximum stays within eight lanes; lanes
+        // past the last word of the row's 8-bit form repeat that word, halves past the last block repeat that block)
+        const int tl = t - mwaves * 64, mr = tl >> 4, mj = P8 ? tl & 15 : min(tl & 15, 11);
+        int qoff[EPT], soff[EPT];                     // P8: byte offsets of this lane's words and blocks from the block's first row
+        bool qpad[EPT];                               // ... and whether the word lies behind the last column (zero)
         int eoff[NSRC][EPT], ewr[NSRC][EPT];          // element offset (floats) from the block's first row; byte offset of its h halves in a stage buffer
 #pragma unroll
         for (int sidx = 0; sidx < NSRC; ++sidx) {
             const int nf4 = ((sidx ? g.K2 : g.K1) + 3) / 4;
 #pragma unroll
             for (int u = 0; u < EPT; ++u) {
-                const int f = min(mj + 12 * u, nf4 - 1);
+                int f = min(mj + 12 * u, nf4 - 1);
+                if (P8) {
+                    const int nb = (g.K1 + 31) / 32, blk = min(2 * u + (mj >> 3), nb - 1);
+                    const int word = min(8 * blk + (mj & 7), (int)(a.keep_ldq / 4) - 1);
+                    qoff[u] = mr * (int)a.keep_ldq + 4 * word;
+                    soff[u] = mr * nb + blk;
+                    qpad[u] = word >= nf4;
+                    f = min(word, nf4 - 1);
+                }
                 eoff[sidx][u] = mr * (int)(sidx ? a.lda2 : a.lda1) + 4 * f;
                 const int kc = (sidx ? 8 * g.nb1 : 0) + 4 * f;            // column of the concatenation
                 const int c = kc >> 5, c4 = (kc >> 2) & 7;          // piece c4 >> 1 of the chunk (its columns 8 q ... 8 q + 7), half c4 & 1
@@ -1033,6 +1048,28 @@ __global__ __launch_bounds__(MAXT) void k_gemm_nt16r(const NtHArgs a) {
             float inv;
             const float sc = scale_for(m, inv);
             rowinv[(it & 1) * R + mr] = inv;
+            if (P8) {
+                const int64_t r0 = block_of(min(it, last)) * R;
+                const int over = rows_over(r0), nb = (g.K1 + 31) / 32;
+                int8_t* qrow = a.keep_q + r0 * a.keep_ldq;
+                uint8_t* srow = a.keep_scale + r0 * nb;
+#pragma unroll
+                for (int u = 0; u < EPT; ++u) {
+                    float v[4];
+                    uint32_t top = 0;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        v[e] = qpad[u] ? 0.f : raw[S][0][u][e];
+                        top = max(top, __float_as_uint(v[e]) & 0x7fffffffu);
+                    }
+                    top = max(top, __float_as_uint(dpp_mov<0xB1>(__uint_as_float(top))));       // lanes ^ 1, ^ 2, mirrored in eight
+                    top = max(top, __float_as_uint(dpp_mov<0x4E>(__uint_as_float(top))));
+                    top = max(top, __float_as_uint(dpp_mov<0x141>(__uint_as_float(top))));
+                    const int byte = p8_byte(top);
+                    *reinterpret_cast<uint32_t*>(qrow + (unsigned)(qoff[u] - over * (int)a.keep_ldq)) = p8_quantise4(v, byte);
+                    srow[(unsigned)(soff[u] - over * nb)] = (uint8_t)byte;
+                }
+            }
             if (BWD) {
 #pragma unroll
                 for (int u = 0; u < EPT; ++u) *reinterpret_cast<f32x4*>(dring + (it & 3) * R * NTR_LDC + dwr[u]) = draw[S][u];
@@ -1228,7 +1265,10 @@ int launch_ntr_k(const NtHArgs& a, const NtrPlan& p, hipStream_t st) {
 bool ntr_bwd_shape(const GeoH& g, const NtrPlan& p, bool two) {
     return p.ok && !p.wide && p.vparts == 1 && g.N <= 144 && (two ? (g.chunks == 4 || g.chunks == 9) : (g.chunks == 4 || g.chunks == 5));
 }
+// ... whose operand's 8-bit form the same launch can leave
+bool ntr_keep_shape(const GeoH& g, const NtrPlan& p) { return p.ok && !p.wide && p.vparts == 1 && (g.chunks == 4 || g.chunks == 5); }
 int launch_ntr(const NtHArgs& a, const NtrPlan& p, hipStream_t st) {
+    if (a.keep_q) return a.g.chunks == 4 ? launch_ntr_k<4, 1, 6>(a, p, st) : launch_ntr_k<5, 1, 6>(a, p, st);
     if (a.act_bits2) return launch_ntr_k<7, 2, 5>(a, p, st);
     if (a.bwd_d && a.bwd_add) {
         if (a.A2) return a.g.chunks == 9 ? launch_ntr_k<9, 2, 4>(a, p, st) : HGV_EUNSUPPORTED;
@@ -1400,10 +1440,12 @@ extern "C" int hgv_pack16h_weights_affine(const float* W1, int64_t sn1, int64_t 
 // C[M,N] = A1 W1^T (+ A2 W2^T) (+ bias) from the scaled fp16 image.  Buffer rules as for hgv_gemm_nt16.
 struct NtHPair { float* C2; const uint32_t* bits2; float* partial2; };
 struct NtHBwd { const float* d; int64_t ldd; const float* gamma; const float* mean; const float* rstd; const float* sums; const float* add; int64_t ldadd; };
+struct NtHKeep { int8_t* q; int64_t ldq; uint8_t* scale; };
 static int gemm_nt16h_any(const float* A1, int64_t lda1, int K1, const float* A2, int64_t lda2, int K2, const void* Wp,
                           const float* bias, int64_t M, int N, float* C, int64_t ldc, const int* gate, int gate_run_if,
                           hipStream_t stream, const uint32_t* act_bits = nullptr, int64_t act_ldb = 0, int act_relu = 0,
-                          float act_scale = 1.f, float* stat_partial = nullptr, const NtHBwd* bwd = nullptr, const NtHPair* pair = nullptr) {
+                          float act_scale = 1.f, float* stat_partial = nullptr, const NtHBwd* bwd = nullptr, const NtHPair* pair = nullptr,
+                          const NtHKeep* keep = nullptr) {
     HGV_REQUIRE(M >= 0 && N > 0 && K1 > 0, HGV_EINVAL, "gemm_nt16h: bad sizes");
     if (M == 0) return HGV_OK;
     NtHArgs a{};
@@ -1441,6 +1483,14 @@ static int gemm_nt16h_any(const float* A1, int64_t lda1, int K1, const float* A2
             a.bwd_add = bwd->add; a.bwd_ldadd = bwd->ldadd;
         }
     }
+    if (keep) {
+        if (ntr_keep_shape(a.g, plan)) {
+            a.keep_q = keep->q; a.keep_ldq = keep->ldq; a.keep_scale = keep->scale;
+        } else {
+            rc = hgv_pack8(A1, lda1, M, K1, keep->q, keep->ldq, keep->scale, stream);
+            if (rc != HGV_OK) return rc;
+        }
+    }
     if (plan.ok) {
         rc = launch_ntr(a, plan, stream);
     } else if (a.g.stream) {
@@ -1463,6 +1513,16 @@ static int gemm_nt16h_any(const float* A1, int64_t lda1, int K1, const float* A2
 extern "C" int hgv_gemm_nt16h(const float* A1, int64_t lda1, int K1, const float* A2, int64_t lda2, int K2, const void* Wp,
                               const float* bias, int64_t M, int N, float* C, int64_t ldc, hipStream_t stream) {
     return gemm_nt16h_any(A1, lda1, K1, A2, lda2, K2, Wp, bias, M, N, C, ldc, nullptr, 0, stream);
+}
+
+// hgv_gemm_nt16h of one source that also leaves the source's 8-bit form (hgv_pack8): from the same launch where the kernel with the
+// weights in registers runs unsplit (97 ... 144 columns, 33 ... 144 outputs), else by a pass of its own.
+extern "C" int hgv_gemm_nt16h_keep8(const float* A, int64_t lda, int K, const void* Wp, const float* bias, int64_t M, int N, float* C,
+                                    int64_t ldc, int8_t* q, int64_t ldq, uint8_t* scale, hipStream_t stream) {
+    HGV_REQUIRE(K > 0 && q && scale && ldq >= K && ldq % 16 == 0 && ldq <= 32 * (int64_t)((K + 31) / 32) && hgv_aligned(q, 16), HGV_EINVAL,
+                "gemm_nt16h_keep8: null / misaligned buffer or bad leading dimension");
+    const NtHKeep keep{q, ldq, scale};
+    return gemm_nt16h_any(A, lda, K, nullptr, 0, 0, Wp, bias, M, N, C, ldc, nullptr, 0, stream, nullptr, 0, 0, 1.f, nullptr, nullptr, nullptr, &keep);
 }
 
 // 1 when hgv_gemm_nt16h_act can run this shape

@@ -2573,14 +2573,20 @@ class _Linear8(torch.autograd.Function):
         x = _own_rows(x)
         need = ctx.needs_input_grad
         fwd, ctx.image = _images((w, None, False), (w, None, True) if need[0] else None)
-        y = _gemm_nt(x, fwd, None, bias, w.size(0))
         ctx.packed = None
-        if need[1]:
-            p = _pack8(x)
-            ctx.packed = p.shape
-            ctx.save_for_backward(w, p.q, p.scale)
-        else:
+        if not need[1]:
             ctx.save_for_backward(w)
+            return _gemm_nt(x, fwd, None, bias, w.size(0))
+        if fwd.kind == "f16x3" and _probe is None and not _CHECK_PADS:
+            n, k = x.shape
+            y = new_padded(n, w.size(0), x.device, zero_pad=False)
+            p = _empty8(n, k, x.device)
+            _lib.call("hgv_gemm_nt16h_keep8", x.data_ptr(), ld_of(x), k, fwd.a.data_ptr(), _lib.ptr(bias), n, w.size(0), y.data_ptr(), ld_of(y),
+                      p.q.data_ptr(), p.q.stride(0), p.scale.data_ptr(), _lib.stream())
+        else:
+            y, p = _gemm_nt(x, fwd, None, bias, w.size(0)), _pack8(x)
+        ctx.packed = p.shape
+        ctx.save_for_backward(w, p.q, p.scale)
         return y
 
     @staticmethod

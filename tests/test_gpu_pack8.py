@@ -175,3 +175,21 @@ def test_pack8_linear8_empty_and_refusals():
                  lambda: Fn.linear8(x, torch.randn(300, 5, device=dev())), lambda: Fn.linear8(x, w.detach().double())):
         with pytest.raises(_lib.HgvError):
             call()
+
+
+@pytest.mark.parametrize("n", [1, 15, 16, 17, 4113, 8191])
+@pytest.mark.parametrize("k,m", [(96, 40), (97, 40), (100, 138), (105, 256), (128, 33), (138, 138), (140, 100), (144, 144), (145, 144), (256, 64)])
+def test_projection_keeps_the_8bit_form(n, k, m):
+    """What the product leaves for the weight gradient, in one launch or by itself: pack8(x) byte for byte, zeros behind the last
+    column; and the product itself is what it is without."""
+    from hgvae_amd import functional as Fn
+    gen = torch.Generator(device=dev()).manual_seed(n + k)
+    x = torch.randn(n, k, generator=gen, device=dev()) * torch.exp2(torch.randint(-40, 40, (n, 1), generator=gen, device=dev()).float())
+    x[:, k - 1] *= 1e-3
+    x[n // 2] = 0.0
+    w, b = torch.randn(m, k, generator=gen, device=dev()), torch.randn(m, generator=gen, device=dev())
+    y = Fn.linear8(x, w.clone().requires_grad_(), b)
+    q, scale = (t for t in y.grad_fn.saved_tensors if t.dtype in (torch.int8, torch.uint8))
+    want = Fn.pack8(x)
+    assert torch.equal(q, want.q) and torch.equal(scale, want.scale)
+    assert torch.equal(y.detach(), Fn.linear8(x, w, b))
