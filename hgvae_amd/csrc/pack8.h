@@ -18,13 +18,17 @@ __device__ __forceinline__ uint32_t p8_max8(uint32_t v) {       // over the eigh
     return max(v, (uint32_t)__shfl_xor((int)v, 4, 64));
 }
 
+// Four integers of a block as bytes.  x * 2^-e + 1.5 * 2^23 in one rounding: the low byte of the sum's bits is round_to_nearest_even
+// (x * 2^-e) in two's complement (|q| < 2^22), so a value takes two instructions: the cut to 127 * 2^e, which only bites beyond
+// 127.5 * 2^121, and the multiply-add.
 __device__ __forceinline__ uint32_t p8_quantise4(const float v[4], int byte) {
-    if (byte == 255) return 0;
     const float inv = __uint_as_float((uint32_t)(254 - byte) << 23);            // 2^-e, e = byte - 127 in [-126, 121]
-    uint32_t w = 0;
+    const float lim = __uint_as_float(((uint32_t)(byte + 6) << 23) | 0x7e0000u);  // 127 * 2^e
+    uint32_t b[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) w |= ((uint32_t)(int)fminf(fmaxf(rintf(v[i] * inv), -127.f), 127.f) & 255u) << (8 * i);
-    return w;
+    for (int i = 0; i < 4; ++i) b[i] = __float_as_uint(fmaf(__builtin_amdgcn_fmed3f(v[i], -lim, lim), inv, 12582912.f));
+    const uint32_t lo = __builtin_amdgcn_perm(b[1], b[0], 0x0c0c0400), hi = __builtin_amdgcn_perm(b[3], b[2], 0x04000c0c);
+    return byte == 255 ? 0u : lo | hi;
 }
 
 __device__ __forceinline__ float p8_step(int byte) {                               // 2^e, or NaN
