@@ -9,7 +9,8 @@
 // Forward: one pass over the keys with the running maximum and sum of the softmax.  The logits are formed transposed
 // (S^T = K Q^T), so a lane owns one query: the maximum and the sum are a lane's own business up to two exchanges, and the
 // probabilities leave the product in the layout in which the next one (O^T = V^T P^T) takes them; V comes from LDS through the
-// transposing loads.  Kept for the backward pass: the output and one number per row and head (lse, base 2; +inf for a row without
+// transposing loads.  Graphs of few rows are taken from the operands as they are, larger ones from images of the pieces that a pass
+// of its own leaves.  Kept for the backward pass: the output and one number per row and head (lse, base 2; +inf for a row without
 // keys).  Backward: probabilities are recomputed, once by key tiles (dk, dv) and once by query tiles (dq): no atomics, the same
 // bits every time.  A masked key's rows of k and v are taken as zeros, whatever they hold.
 #include "common.h"
@@ -307,6 +308,99 @@ constexpr float P_GROW = 7.f;
 constexpr int at_bounds(int DP, int NW) { return DP == 128 && NW == 4 ? 1 : 2; }
 
 // ---- forward -----------------------------------------------------------------------------------------------------------------
+// Two pieces of operands, both rounded to nearest: 2^-24.  The values come out of v_ldexp_f32, which no conversion is merged with.
+__device__ __forceinline__ void split2_rn(float x, float y, f16x2& hi, f16x2& lo, float neg) {
+    hi = f16x2{(_Float16)x, (_Float16)y};
+    lo = f16x2{(_Float16)fmaf((float)hi[0], neg, x), (_Float16)fmaf((float)hi[1], neg, y)};
+}
+
+// One tile of 64 keys (pieces in LDS) against a wave's queries.  c: what a product of the pieces is multiplied by, base 2.
+template <int DP, int QB>
+__device__ __forceinline__ void fwd_tile(const unsigned char* ldsK, const unsigned char* ldsV, const float* bias, bool biased, int lane,
+                                         const float (&c)[QB], const Frag (&q)[QB][DP / 32], float (&m)[QB], float (&l)[QB],
+                                         f32x4 (&acc)[DP / 16][QB], float neg) {
+    constexpr int KC = DP / 32, DB = DP / 16;
+    const int g = lane >> 4;
+    f32x4 s[4][QB];
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+#pragma unroll
+        for (int j = 0; j < QB; ++j) s[b][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < KC; ++k) {
+            const Frag f = row_frag<DP>(ldsK, 16 * b, k, lane);
+#pragma unroll
+            for (int j = 0; j < QB; ++j) s[b][j] = mma3(f, q[j][k], s[b][j]);
+        }
+        if (biased) {
+            const f32x4 o = *(const f32x4*)(bias + 16 * b + 4 * g);
+#pragma unroll
+            for (int j = 0; j < QB; ++j) s[b][j] += o;
+        }
+    }
+#pragma unroll
+    for (int b = 0; b < QB; ++b) {
+        float top = s[0][b][0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i >> 2][b][i & 3]);
+        top = fmaxf(top, __shfl_xor(top, 16, 64));
+        top = fmaxf(top, __shfl_xor(top, 32, 64)) * c[b];
+        // rescale only when a probability would leave its range
+        if (__any(top > m[b] + P_GROW || (m[b] == -INFINITY && top > -INFINITY))) {
+            const float mn = fmaxf(m[b], top);
+            const float f = m[b] == -INFINITY ? 0.f : exp2_fast(m[b] - mn);
+            m[b] = mn;
+            l[b] *= f;
+#pragma unroll
+            for (int d = 0; d < DB; ++d) acc[d][b] *= f;
+        }
+        const float off = m[b] == -INFINITY ? 0.f : P_BITS - m[b];
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float p = exp2_fast(fmaf(s[i][b][j], c[b], off));
+                s[i][b][j] = p;
+                sum[j] += p;
+            }
+        l[b] += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    }
+#pragma unroll
+    for (int kc = 0; kc < 2; ++kc) {
+        Frag p[QB];
+#pragma unroll
+        for (int j = 0; j < QB; ++j) p[j] = split_frag(s[2 * kc][j], s[2 * kc + 1][j], neg);
+#pragma unroll
+        for (int d = 0; d < DB; ++d) {
+            const Frag f = col_frag<DP>(ldsV, 32 * kc, d, lane);
+#pragma unroll
+            for (int j = 0; j < QB; ++j) acc[d][j] = mma3(f, p[j], acc[d][j]);
+        }
+    }
+}
+
+// The rows of a wave's queries, and their lse; ev: exponent of the values' scale.
+template <int DP, int QB>
+__device__ __forceinline__ void fwd_rows(const AtArgs& a, int64_t q0, int64_t k1, int h, int lane, int ev, const float (&m)[QB], float (&l)[QB],
+                                         const f32x4 (&acc)[DP / 16][QB]) {
+    constexpr int DB = DP / 16;
+    const int g = lane >> 4;
+#pragma unroll
+    for (int b = 0; b < QB; ++b) {
+        l[b] += __shfl_xor(l[b], 16, 64);
+        l[b] += __shfl_xor(l[b], 32, 64);
+        const int64_t row = q0 + 16 * b + (lane & 15);
+        if (row >= k1) continue;
+        const bool none = l[b] == 0.f;
+        const float f = none ? 0.f : ldexpf(1.f / l[b], ev - 15);
+        float* o = row_out(a.out, row, a.H, h, a.D);
+#pragma unroll
+        for (int d = 0; d < DB; ++d) store4(o, 16 * d + 4 * g, a.D, none ? f32x4{0.f, 0.f, 0.f, 0.f} : acc[d][b] * f);
+        if (g == 0 && a.lse) a.lse[(int64_t)h * a.N + row] = none ? INFINITY : m[b] - P_BITS + log2f(l[b]);
+    }
+}
+
 // A workgroup owns 16 * QB * NW queries of one head (a wave 16 * QB), walks the keys of the graph in tiles of 64.
 template <int DP, int QB, int NW>
 __global__ __launch_bounds__(64 * NW, DP == 32 ? 4 : at_bounds(DP, NW)) void k_at_fwd(const AtArgs a) {
@@ -314,13 +408,15 @@ __global__ __launch_bounds__(64 * NW, DP == 32 ? 4 : at_bounds(DP, NW)) void k_a
     __shared__ __align__(16) unsigned char ldsK[64 * line_bytes<DP>()];
     __shared__ __align__(16) unsigned char ldsV[64 * line_bytes<DP>()];
     __shared__ __align__(16) float bias[64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int blk = blockIdx.x / a.H, h = blockIdx.x - blk * a.H, hk = h / a.R;
     const int4 t = a.blocks[blk];
     const int64_t k0 = a.ptr[t.x], k1 = a.ptr[t.x + 1];
     const int64_t q0 = (int64_t)t.y + 16 * QB * wave;
     const int* ex = a.exps + ((int64_t)t.x * a.Hk + hk) * 4;
-    const float c = fold_scale(a.scale, ex[TQ] + ex[TK] - 30);
+    float c[QB];
+#pragma unroll
+    for (int b = 0; b < QB; ++b) c[b] = fold_scale(a.scale, ex[TQ] + ex[TK] - 30);
     Frag q[QB][KC];
 #pragma unroll
     for (int b = 0; b < QB; ++b)
@@ -355,77 +451,155 @@ __global__ __launch_bounds__(64 * NW, DP == 32 ? 4 : at_bounds(DP, NW)) void k_a
             nb = threadIdx.x < 64 && j < n && (!a.mask || a.mask[k0 + j]) ? 0.f : -INFINITY;
         }
         const bool biased = a.mask != nullptr || kt + 64 > n;
-        f32x4 s[4][QB];
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-#pragma unroll
-            for (int j = 0; j < QB; ++j) s[b][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int k = 0; k < KC; ++k) {
-                const Frag f = row_frag<DP>(ldsK, 16 * b, k, lane);
-#pragma unroll
-                for (int j = 0; j < QB; ++j) s[b][j] = mma3(f, q[j][k], s[b][j]);
-            }
-            if (biased) {
-                const f32x4 o = *(const f32x4*)(bias + 16 * b + 4 * g);
-#pragma unroll
-                for (int j = 0; j < QB; ++j) s[b][j] += o;
-            }
-        }
-#pragma unroll
-        for (int b = 0; b < QB; ++b) {
-            float top = s[0][b][0];
-#pragma unroll
-            for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i >> 2][b][i & 3]);
-            top = fmaxf(top, __shfl_xor(top, 16, 64));
-            top = fmaxf(top, __shfl_xor(top, 32, 64)) * c;
-            // rescale only when a probability would leave its range
-            if (__any(top > m[b] + P_GROW || (m[b] == -INFINITY && top > -INFINITY))) {
-                const float mn = fmaxf(m[b], top);
-                const float f = m[b] == -INFINITY ? 0.f : exp2_fast(m[b] - mn);
-                m[b] = mn;
-                l[b] *= f;
-#pragma unroll
-                for (int d = 0; d < DB; ++d) acc[d][b] *= f;
-            }
-            const float off = m[b] == -INFINITY ? 0.f : P_BITS - m[b];
-            float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float p = exp2_fast(fmaf(s[i][b][j], c, off));
-                    s[i][b][j] = p;
-                    sum[j] += p;
-                }
-            l[b] += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        }
-#pragma unroll
-        for (int kc = 0; kc < 2; ++kc) {
-            Frag p[QB];
-#pragma unroll
-            for (int j = 0; j < QB; ++j) p[j] = split_frag(s[2 * kc][j], s[2 * kc + 1][j], a.neg);
-#pragma unroll
-            for (int d = 0; d < DB; ++d) {
-                const Frag f = col_frag<DP>(ldsV, 32 * kc, d, lane);
-#pragma unroll
-                for (int j = 0; j < QB; ++j) acc[d][j] = mma3(f, p[j], acc[d][j]);
-            }
-        }
+        fwd_tile<DP, QB>(ldsK, ldsV, bias, biased, lane, c, q, m, l, acc, a.neg);
     }
+    fwd_rows<DP, QB>(a, q0, k1, h, lane, ex[TV], m, l, acc);
+}
+
+// Graphs of few rows: the operands as they are, without images.  Every workgroup splits what it multiplies on the way into the
+// registers (a query's scale is its own) and into LDS (keys: a scale per tile of 64;  values: of the largest entry so far, the sums
+// follow when it grows), which saves a launch and the round trip through memory.
+__device__ __forceinline__ uint32_t finite_bits(float x) {      // |x| as an integer that orders like it; infinities and NaN do not count
+    const uint32_t u = __float_as_uint(x) & 0x7fffffffu;
+    return u < 0x7f800000u ? u : 0u;
+}
+__device__ __forceinline__ int exp_above(uint32_t bits) { return max((int)(bits >> 23), 1) - 126; }      // |x| < 2^e
+template <bool VEC>
+__device__ __forceinline__ f32x4 four(const float* p, int d, int D, bool live) {
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    if (VEC) {
+        if (live) v = *(const f32x4*)(p + d);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (live && d + i < D) v[i] = p[d + i];
+    }
+    return v;
+}
+
+template <int DP, int QB, int NW, bool VEC>
+__global__ __launch_bounds__(64 * NW, DP == 32 ? 3 : at_bounds(DP, NW)) void k_at_fwd_small(const AtArgs a) {
+    constexpr int KC = DP / 32, DB = DP / 16, NT = 64 * NW, CH = 64 * (DP / 4) / NT;
+    __shared__ __align__(16) unsigned char ldsK[64 * line_bytes<DP>()];
+    __shared__ __align__(16) unsigned char ldsV[64 * line_bytes<DP>()];
+    __shared__ __align__(16) float bias[64];
+    __shared__ uint32_t top[2][NW];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
+    const int blk = blockIdx.x / a.H, h = blockIdx.x - blk * a.H, hk = h / a.R;
+    const int4 t = a.blocks[blk];
+    const int64_t k0 = a.ptr[t.x], k1 = a.ptr[t.x + 1];
+    const int64_t q0 = (int64_t)t.y + 16 * QB * wave;
+    const int n = (int)(k1 - k0);
+    const float* kp = a.src[TK] + hk * a.head_stride[TK];
+    const float* vp = a.src[TV] + hk * a.head_stride[TV];
+    f32x4 sk[CH], sv[CH];
+    float nb;
+    auto load = [&](int kt) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < CH; ++i) {
+            const int f = threadIdx.x + NT * i, r = f / (DP / 4), d = 4 * (f - r * (DP / 4));
+            const int64_t row = k0 + kt + r;
+            const bool live = kt + r < n && (!a.mask || a.mask[row]);
+            sk[i] = four<VEC>(kp + row * a.row_stride[TK], d, a.D, live);
+            sv[i] = four<VEC>(vp + row * a.row_stride[TV], d, a.D, live);
+        }
+        const int j = kt + (int)threadIdx.x;
+        nb = threadIdx.x < 64 && j < n && (!a.mask || a.mask[k0 + j]) ? 0.f : -INFINITY;
+    };
+    load(0);
+    Frag q[QB][KC];
+    int eq[QB];
 #pragma unroll
     for (int b = 0; b < QB; ++b) {
-        l[b] += __shfl_xor(l[b], 16, 64);
-        l[b] += __shfl_xor(l[b], 32, 64);
-        const int64_t row = q0 + 16 * b + (lane & 15);
-        if (row >= k1) continue;
-        const bool none = l[b] == 0.f;
-        const float f = none ? 0.f : ldexpf(1.f / l[b], ex[TV] - 15);
-        float* o = row_out(a.out, row, a.H, h, a.D);
+        const float* p = a.src[TQ] + min(q0 + 16 * b + (lane & 15), k1 - 1) * a.row_stride[TQ] + h * a.head_stride[TQ];
+        f32x4 x[KC][2];
+        uint32_t big = 0;
 #pragma unroll
-        for (int d = 0; d < DB; ++d) store4(o, 16 * d + 4 * g, a.D, none ? f32x4{0.f, 0.f, 0.f, 0.f} : acc[d][b] * f);
-        if (g == 0 && a.lse) a.lse[(int64_t)h * a.N + row] = none ? INFINITY : m[b] - P_BITS + log2f(l[b]);
+        for (int k = 0; k < KC; ++k)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                x[k][i] = four<VEC>(p, 32 * k + 8 * g + 4 * i, a.D, true);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) big = max(big, finite_bits(x[k][i][j]));
+            }
+        big = max(big, (uint32_t)__shfl_xor((int)big, 16, 64));
+        big = max(big, (uint32_t)__shfl_xor((int)big, 32, 64));
+        eq[b] = exp_above(big);
+#pragma unroll
+        for (int k = 0; k < KC; ++k) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x[k][i][j] = ldexpf(x[k][i][j], 15 - eq[b]);
+            union { Frag f; struct { f16x2 hi[4], lo[4]; } p; } u;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                split2_rn(x[k][i][0], x[k][i][1], u.p.hi[2 * i], u.p.lo[2 * i], a.neg);
+                split2_rn(x[k][i][2], x[k][i][3], u.p.hi[2 * i + 1], u.p.lo[2 * i + 1], a.neg);
+            }
+            q[b][k] = u.f;
+        }
     }
+    f32x4 acc[DB][QB];
+    float m[QB], l[QB];
+#pragma unroll
+    for (int b = 0; b < QB; ++b) { m[b] = -INFINITY; l[b] = 0.f; }
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int b = 0; b < QB; ++b) acc[d][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+    int ev = -126;
+    for (int kt = 0; kt < n; kt += 64) {
+        uint32_t uk = 0, uv = 0;
+#pragma unroll
+        for (int i = 0; i < CH; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) { uk = max(uk, finite_bits(sk[i][j])); uv = max(uv, finite_bits(sv[i][j])); }
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            uk = max(uk, (uint32_t)__shfl_xor((int)uk, o, 64));
+            uv = max(uv, (uint32_t)__shfl_xor((int)uv, o, 64));
+        }
+        if (lane == 0) { top[0][wave] = uk; top[1][wave] = uv; }
+        __syncthreads();                                        // also: the tile before this one has been read
+#pragma unroll
+        for (int w = 0; w < NW; ++w) { uk = max(uk, top[0][w]); uv = max(uv, top[1][w]); }
+        const int ek = exp_above(uk), e_new = max(ev, exp_above(uv));
+        if (e_new > ev) {                                       // the same for the whole workgroup
+            const float f = ldexpf(1.f, ev - e_new);
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int b = 0; b < QB; ++b) acc[d][b] *= f;
+            ev = e_new;
+        }
+#pragma unroll
+        for (int i = 0; i < CH; ++i) {
+            const int f = threadIdx.x + NT * i, r = f / (DP / 4), c4 = f - r * (DP / 4);
+            const int off = line_of(r) * line_bytes<DP>() + c4 * 8;
+            f32x4 x, y;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) { x[j] = ldexpf(sk[i][j], 15 - ek); y[j] = ldexpf(sv[i][j], 15 - ev); }
+            f16x2 hi[2], lo[2];
+            split2_rn(x[0], x[1], hi[0], lo[0], a.neg);
+            split2_rn(x[2], x[3], hi[1], lo[1], a.neg);
+            *(f16x4*)(ldsK + off) = f16x4{hi[0][0], hi[0][1], hi[1][0], hi[1][1]};
+            *(f16x4*)(ldsK + off + 2 * DP) = f16x4{lo[0][0], lo[0][1], lo[1][0], lo[1][1]};
+            split2_rn(y[0], y[1], hi[0], lo[0], a.neg);
+            split2_rn(y[2], y[3], hi[1], lo[1], a.neg);
+            *(f16x4*)(ldsV + off) = f16x4{hi[0][0], hi[0][1], hi[1][0], hi[1][1]};
+            *(f16x4*)(ldsV + off + 2 * DP) = f16x4{lo[0][0], lo[0][1], lo[1][0], lo[1][1]};
+        }
+        if (threadIdx.x < 64) bias[threadIdx.x] = nb;
+        const bool biased = a.mask != nullptr || kt + 64 > n;
+        if (kt + 64 < n) load(kt + 64);
+        __syncthreads();
+        float c[QB];
+#pragma unroll
+        for (int b = 0; b < QB; ++b) c[b] = fold_scale(a.scale, eq[b] + ek - 30);
+        fwd_tile<DP, QB>(ldsK, ldsV, bias, biased, lane, c, q, m, l, acc, a.neg);
+    }
+    fwd_rows<DP, QB>(a, q0, k1, h, lane, ev, m, l, acc);
 }
 
 // ---- backward: dk and dv ---------------------------------------------------------------------------------------------------
@@ -714,6 +888,21 @@ int at_launch(AtArgs a, bool backward, hipStream_t stream) {
     bool vec = a.D == DP;
     for (int i = 0; i < (backward ? 4 : 3); ++i)
         vec = vec && hgv_aligned(a.src[i], 16) && a.row_stride[i] % 4 == 0 && a.head_stride[i] % 4 == 0;
+    // Without images where no graph is large: what splitting every operand once per workgroup costs stays below a pass of its own over
+    // memory (four heads of 64, with and without: 32 graphs of 138 nodes 15 and 26 us, 2 000 of 250 0.70 and 1.74 ms, 200 of 512 0.26
+    // and 0.37, 100 of 1 000 0.43 and 0.51, 16 of 5 000 1.44 and 1.29; six heads of 23: 200 of 512 0.24 and 0.26, 100 of 1 000 0.39
+    // and 0.35).
+    if (!backward && a.max_rows <= 512) {
+        constexpr int QB = DP <= 64 ? 2 : 1;
+        at_rows(a, a.H, [&](int i, dim3 grid) {
+            if (i && vec) hipLaunchKernelGGL((k_at_fwd_small<DP, QB, 8 / QB, true>), grid, dim3(512 / QB), 0, stream, a);
+            else if (i) hipLaunchKernelGGL((k_at_fwd_small<DP, QB, 8 / QB, false>), grid, dim3(512 / QB), 0, stream, a);
+            else if (vec) hipLaunchKernelGGL((k_at_fwd_small<DP, 1, 4, true>), grid, dim3(256), 0, stream, a);
+            else hipLaunchKernelGGL((k_at_fwd_small<DP, 1, 4, false>), grid, dim3(256), 0, stream, a);
+        });
+        HGV_CHECK_LAUNCH("graph_attention_fwd");
+        return HGV_OK;
+    }
     if (vec) at_images<DP, true>(a, TQ, backward ? TG : TV, stream);
     else at_images<DP, false>(a, TQ, backward ? TG : TV, stream);
     // 32 rows per wave, four waves; wider heads (above 64 columns backward, 96 forward): 16 rows, eight waves, so that the accumulators

@@ -629,7 +629,7 @@ int hgv_graph_attention_fwd(const float* q, int64_t q_row, int64_t q_head, const
 int hgv_graph_attention_bwd(const float* q, int64_t q_row, int64_t q_head, const float* k, int64_t k_row, int64_t k_head, const float* v,
                             int64_t v_row, int64_t v_head, const float* g, int64_t g_row, int64_t g_head, const float* out,
                             const float* lse, int64_t N, int num_graphs, int H, int Hk, int D, float scale, const uint8_t* mask,
-                            const int32_t* ptr, const int32_t* tiles, int n_tiles, const int32_t* blocks, int n64, int n128, float* dq,
+                            const int32_t* ptr, int max_rows, const int32_t* tiles, int n_tiles, const int32_t* blocks, int n64, int n128, float* dq,
                             float* dk, float* dv, void* ws, size_t ws_bytes, hgv_stream_t stream);
 
 #ifdef __cplusplus

@@ -121,3 +121,17 @@ def test_c_abi_refusals_without_a_gpu():
     refused(-4, "hgv_graph_attention_fwd", *att(2, 2, 8, 1.0, 16))
     assert lib.hgv_group_norm_small_rows(10, 3) == 0 and lib.hgv_group_norm_small_rows(138, 6) > 0
     assert lib.hgv_graph_attention_ws(0, 1, 1, 1, 8, 1, 0) == 0 and lib.hgv_graph_attention_ws(100, 1, 2, 1, 8, 2, 1) > lib.hgv_graph_attention_ws(100, 1, 2, 1, 8, 2, 0) > 0
+
+
+def test_header_and_bindings_agree_on_the_number_of_arguments():
+    import os
+    import re
+    from hgvae_amd import _lib
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    with open(os.path.join(root, "include", "hgvae_hip.h")) as f:
+        text = re.sub(r"/\*.*?\*/", "", f.read(), flags=re.S)
+    for name, (_, args) in _lib.SIGNATURES.items():
+        found = re.search(rf"\b{name}\s*\(([^)]*)\)", text)
+        assert found, name
+        params = found.group(1).strip()
+        assert (0 if params in ("", "void") else params.count(",") + 1) == len(args), name
