@@ -257,12 +257,21 @@ __device__ __forceinline__ void split2(float x, float y, f16x2& hi, f16x2& lo, f
     lo = f16x2{(_Float16)rx, (_Float16)ry};
 }
 
+// ... both rounded to nearest: 2^-24.  For values that do not come out of a multiplication (v_ldexp_f32, v_exp_f32).
+__device__ __forceinline__ void split2_rn(float x, float y, f16x2& hi, f16x2& lo, float neg) {
+    hi = f16x2{(_Float16)x, (_Float16)y};
+    lo = f16x2{(_Float16)fmaf((float)hi[0], neg, x), (_Float16)fmaf((float)hi[1], neg, y)};
+}
+
+template <bool RN = false>
 __device__ __forceinline__ Frag split_frag(const f32x4& x, const f32x4& y, float neg) {
     union { Frag f; struct { f16x2 hi[4], lo[4]; } p; } u;
-    split2(x[0], x[1], u.p.hi[0], u.p.lo[0], neg);
-    split2(x[2], x[3], u.p.hi[1], u.p.lo[1], neg);
-    split2(y[0], y[1], u.p.hi[2], u.p.lo[2], neg);
-    split2(y[2], y[3], u.p.hi[3], u.p.lo[3], neg);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float v0 = i < 2 ? x[2 * i] : y[2 * i - 4], v1 = i < 2 ? x[2 * i + 1] : y[2 * i - 3];
+        if (RN) split2_rn(v0, v1, u.p.hi[i], u.p.lo[i], neg);
+        else split2(v0, v1, u.p.hi[i], u.p.lo[i], neg);
+    }
     return u.f;
 }
 
@@ -308,14 +317,10 @@ constexpr float P_GROW = 7.f;
 constexpr int at_bounds(int DP, int NW) { return DP == 128 && NW == 4 ? 1 : 2; }
 
 // ---- forward -----------------------------------------------------------------------------------------------------------------
-// Two pieces of operands, both rounded to nearest: 2^-24.  The values come out of v_ldexp_f32, which no conversion is merged with.
-__device__ __forceinline__ void split2_rn(float x, float y, f16x2& hi, f16x2& lo, float neg) {
-    hi = f16x2{(_Float16)x, (_Float16)y};
-    lo = f16x2{(_Float16)fmaf((float)hi[0], neg, x), (_Float16)fmaf((float)hi[1], neg, y)};
-}
-
-// One tile of 64 keys (pieces in LDS) against a wave's queries.  c: what a product of the pieces is multiplied by, base 2.
-template <int DP, int QB>
+// One tile of 64 keys (pieces in LDS) against a wave's queries.  c: what a product of the pieces is multiplied by, base 2.  RN: the
+// probabilities' pieces to nearest, which shows in the sums over a few keys (graphs of two rows: 1.0e-7 -> 6.5e-8 of the result) and
+// would take 3 (64 columns) to 7 % (23) of the time of large graphs.
+template <int DP, int QB, bool RN>
 __device__ __forceinline__ void fwd_tile(const unsigned char* ldsK, const unsigned char* ldsV, const float* bias, bool biased, int lane,
                                          const float (&c)[QB], const Frag (&q)[QB][DP / 32], float (&m)[QB], float (&l)[QB],
                                          f32x4 (&acc)[DP / 16][QB], float neg) {
@@ -370,7 +375,7 @@ __device__ __forceinline__ void fwd_tile(const unsigned char* ldsK, const unsign
     for (int kc = 0; kc < 2; ++kc) {
         Frag p[QB];
 #pragma unroll
-        for (int j = 0; j < QB; ++j) p[j] = split_frag(s[2 * kc][j], s[2 * kc + 1][j], neg);
+        for (int j = 0; j < QB; ++j) p[j] = split_frag<RN>(s[2 * kc][j], s[2 * kc + 1][j], neg);
 #pragma unroll
         for (int d = 0; d < DB; ++d) {
             const Frag f = col_frag<DP>(ldsV, 32 * kc, d, lane);
@@ -451,7 +456,7 @@ __global__ __launch_bounds__(64 * NW, DP == 32 ? 4 : at_bounds(DP, NW)) void k_a
             nb = threadIdx.x < 64 && j < n && (!a.mask || a.mask[k0 + j]) ? 0.f : -INFINITY;
         }
         const bool biased = a.mask != nullptr || kt + 64 > n;
-        fwd_tile<DP, QB>(ldsK, ldsV, bias, biased, lane, c, q, m, l, acc, a.neg);
+        fwd_tile<DP, QB, false>(ldsK, ldsV, bias, biased, lane, c, q, m, l, acc, a.neg);
     }
     fwd_rows<DP, QB>(a, q0, k1, h, lane, ex[TV], m, l, acc);
 }
@@ -531,13 +536,7 @@ __global__ __launch_bounds__(64 * NW, DP == 32 ? 3 : at_bounds(DP, NW)) void k_a
             for (int i = 0; i < 2; ++i)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) x[k][i][j] = ldexpf(x[k][i][j], 15 - eq[b]);
-            union { Frag f; struct { f16x2 hi[4], lo[4]; } p; } u;
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                split2_rn(x[k][i][0], x[k][i][1], u.p.hi[2 * i], u.p.lo[2 * i], a.neg);
-                split2_rn(x[k][i][2], x[k][i][3], u.p.hi[2 * i + 1], u.p.lo[2 * i + 1], a.neg);
-            }
-            q[b][k] = u.f;
+            q[b][k] = split_frag<true>(x[k][0], x[k][1], a.neg);
         }
     }
     f32x4 acc[DB][QB];
@@ -597,7 +596,7 @@ __global__ __launch_bounds__(64 * NW, DP == 32 ? 3 : at_bounds(DP, NW)) void k_a
         float c[QB];
 #pragma unroll
         for (int b = 0; b < QB; ++b) c[b] = fold_scale(a.scale, eq[b] + ek - 30);
-        fwd_tile<DP, QB>(ldsK, ldsV, bias, biased, lane, c, q, m, l, acc, a.neg);
+        fwd_tile<DP, QB, true>(ldsK, ldsV, bias, biased, lane, c, q, m, l, acc, a.neg);
     }
     fwd_rows<DP, QB>(a, q0, k1, h, lane, ev, m, l, acc);
 }
