@@ -10,9 +10,9 @@
 // (S^T = K Q^T), so a lane owns one query: the maximum and the sum are a lane's own business up to two exchanges, and the
 // probabilities leave the product in the layout in which the next one (O^T = V^T P^T) takes them; V comes from LDS through the
 // transposing loads.  Graphs of few rows are taken from the operands as they are, larger ones from images of the pieces that a pass
-// of its own leaves.  Kept for the backward pass: the output and one number per row and head (lse, base 2; +inf for a row without
-// keys).  Backward: probabilities are recomputed, once by key tiles (dk, dv) and once by query tiles (dq): no atomics, the same
-// bits every time.  A masked key's rows of k and v are taken as zeros, whatever they hold.
+// of its own leaves.  Kept for the backward pass: the output and two numbers per row and head (the exponent that is subtracted and the
+// inverse of the sum that is left; +inf and 0 for a row without keys).  Backward: probabilities are recomputed, once by key tiles
+// (dk, dv) and once by query tiles (dq): no atomics, the same bits every time.  A masked key's rows of k and v are taken as zeros, whatever they hold.
 #include "common.h"
 
 namespace {
@@ -44,7 +44,7 @@ struct AtArgs {
     int* exps;                                                  // [B][Hk][4]
     _Float16* img[4];                                           // [heads][N][hi DP | lo DP]
     float* out;                                                 // [N, H, D]
-    float* lse;                                                 // [H, N]
+    float2* stats;                                              // [H, N] of a row: whole M with sum_j 2^(logit_j - M) in [1, 2), and 1 / that sum
     float* delta;                                               // [H, N] sum_d do * o, scaled (backward)
     float* dq; float* dk; float* dv;                            // [N, H or Hk, D]
 };
@@ -76,6 +76,15 @@ __device__ __forceinline__ void load_part(const float* p, int sub, int D, bool l
     }
 }
 
+// The output's gradient is divided by the row's sum here, once: the products then run on 2^(logit - M), M whole.  (With one number per
+// row, log2 of the sum, its rounding alone put 3e-7 on every probability, and 2e-7 to 4e-6 of the gradients more than this way.)
+template <int E>
+__device__ __forceinline__ void over_sum(const AtArgs& a, int64_t n, int h, float v[E]) {
+    const float f = a.stats[(int64_t)h * a.N + n].y;
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] *= f;
+}
+
 // The exponent e with |row| < 2^e of the longest row among rows n0 .. n0 + rows - 1 of key head hk, over the whole workgroup
 // (NO_EXP: none that is finite and not zero).  red: four ints of LDS, free to be written.
 template <int DP, bool VEC>
@@ -88,6 +97,7 @@ __device__ __forceinline__ int longest_row(const AtArgs& a, int ten, int hk, int
         const int64_t n = n0 + r;
         float v[DP / 16];
         load_part<DP, VEC>(a.src[ten] + n * a.row_stride[ten] + h * a.head_stride[ten], sub, a.D, !(masked && !a.mask[n]), v);
+        if (ten == TG) over_sum<DP / 16>(a, n, h, v);
         double s = 0.0;
 #pragma unroll
         for (int e = 0; e < DP / 16; ++e) s = fma((double)v[e], (double)v[e], s);
@@ -153,6 +163,7 @@ __global__ __launch_bounds__(256) void k_at_split(const AtArgs a, const int firs
         const int64_t n = tile.y + r;
         float v[E];
         load_part<DP, VEC>(a.src[ten] + n * a.row_stride[ten] + h * a.head_stride[ten], sub, a.D, !(masked && !a.mask[n]), v);
+        if (ten == TG) over_sum<E>(a, n, h, v);
         f16x2 hi[E / 2], lo[E / 2];
 #pragma unroll
         for (int j = 0; j < E; ++j) v[j] = ldexpf(v[j], 15 - e);
@@ -175,7 +186,7 @@ __global__ __launch_bounds__(256) void k_at_split(const AtArgs a, const int firs
                 if (sub * E + j < a.D) dot = fmaf(v[j], o[sub * E + j], dot);
 #pragma unroll
             for (int w = 1; w < 16; w <<= 1) dot += __shfl_xor(dot, w, 64);
-            if (sub == 0) a.delta[(int64_t)h * a.N + n] = ldexpf(dot, -16 - ev);
+            if (sub == 0) a.delta[(int64_t)h * a.N + n] = ldexpf(dot, -2 - ev);
         }
     }
 }
@@ -352,7 +363,7 @@ __device__ __forceinline__ void fwd_tile(const unsigned char* ldsK, const unsign
         top = fmaxf(top, __shfl_xor(top, 32, 64)) * c[b];
         // rescale only when a probability would leave its range
         if (__any(top > m[b] + P_GROW || (m[b] == -INFINITY && top > -INFINITY))) {
-            const float mn = fmaxf(m[b], top);
+            const float mn = ceilf(fmaxf(m[b], top));      // whole: what is subtracted is then exact, and so are the rescales
             const float f = m[b] == -INFINITY ? 0.f : exp2_fast(m[b] - mn);
             m[b] = mn;
             l[b] *= f;
@@ -385,7 +396,7 @@ __device__ __forceinline__ void fwd_tile(const unsigned char* ldsK, const unsign
     }
 }
 
-// The rows of a wave's queries, and their lse; ev: exponent of the values' scale.
+// The rows of a wave's queries, and their stats; ev: exponent of the values' scale.
 template <int DP, int QB>
 __device__ __forceinline__ void fwd_rows(const AtArgs& a, int64_t q0, int64_t k1, int h, int lane, int ev, const float (&m)[QB], float (&l)[QB],
                                          const f32x4 (&acc)[DP / 16][QB]) {
@@ -402,7 +413,10 @@ __device__ __forceinline__ void fwd_rows(const AtArgs& a, int64_t q0, int64_t k1
         float* o = row_out(a.out, row, a.H, h, a.D);
 #pragma unroll
         for (int d = 0; d < DB; ++d) store4(o, 16 * d + 4 * g, a.D, none ? f32x4{0.f, 0.f, 0.f, 0.f} : acc[d][b] * f);
-        if (g == 0 && a.lse) a.lse[(int64_t)h * a.N + row] = none ? INFINITY : m[b] - P_BITS + log2f(l[b]);
+        if (g == 0 && a.stats) {
+            const int e = (int)(__float_as_uint(l[b]) >> 23) - 127;         // l = 2^e * (1 ... 2)
+            a.stats[(int64_t)h * a.N + row] = none ? make_float2(INFINITY, 0.f) : make_float2(m[b] - P_BITS + (float)e, ldexpf(1.f / l[b], e));
+        }
     }
 }
 
@@ -641,7 +655,7 @@ __global__ __launch_bounds__(64 * NW, at_bounds(DP, NW)) void k_at_dkv(const AtA
         sg.load(a.img[TG] + at * (2 * DP), rows);
         nl = INFINITY; nd = 0.f;
         if ((int)threadIdx.x < rows) {
-            nl = a.lse[at + threadIdx.x];
+            nl = a.stats[at + threadIdx.x].x;
             nd = a.delta[at + threadIdx.x];
         }
     };
@@ -651,7 +665,7 @@ __global__ __launch_bounds__(64 * NW, at_bounds(DP, NW)) void k_at_dkv(const AtA
         sq.store(ldsQ);
         sg.store(ldsG);
         if (threadIdx.x < 64) {
-            ldsL[threadIdx.x] = 15.f - nl;
+            ldsL[threadIdx.x] = -nl;
             ldsD[threadIdx.x] = nd;
         }
         __syncthreads();
@@ -684,7 +698,8 @@ __global__ __launch_bounds__(64 * NW, at_bounds(DP, NW)) void k_at_dkv(const AtA
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             p[b][j][i] = exp2_fast(fmaf(p[b][j][i], c, ls[i]));
-                            s[b][j][i] = p[b][j][i] * fmaf(s[b][j][i], 0x1p-31f, -de[i]);
+                            s[b][j][i] = p[b][j][i] * fmaf(s[b][j][i], 0x1p-17f, -de[i]);
+                            p[b][j][i] *= 0x1p14f;
                         }
                 }
 #pragma unroll
@@ -714,7 +729,7 @@ __global__ __launch_bounds__(64 * NW, at_bounds(DP, NW)) void k_at_dkv(const AtA
         const bool live = !a.mask || a.mask[row];
         float* pk = row_out(a.dk, row, a.Hk, hk, a.D);
         float* pv = row_out(a.dv, row, a.Hk, hk, a.D);
-        const int ek = ex[TG] + ex[TV] + ex[TQ] - 29, ev = ex[TG] - 30;
+        const int ek = ex[TG] + ex[TV] + ex[TQ] - 28, ev = ex[TG] - 29;
 #pragma unroll
         for (int d = 0; d < DB; ++d) {
             f32x4 x, y;
@@ -753,7 +768,7 @@ __global__ __launch_bounds__(64 * NW, at_bounds(DP, NW)) void k_at_dq(const AtAr
             q[b][k] = own_frag<DP>(a.img[TQ] + (int64_t)h * a.N * (2 * DP), row, k, lane);
             go[b][k] = own_frag<DP>(a.img[TG] + (int64_t)h * a.N * (2 * DP), row, k, lane);
         }
-        ls[b] = 15.f - a.lse[(int64_t)h * a.N + row];
+        ls[b] = -a.stats[(int64_t)h * a.N + row].x;
         de[b] = a.delta[(int64_t)h * a.N + row];
     }
     f32x4 acc[DB][QB];
@@ -814,7 +829,7 @@ __global__ __launch_bounds__(64 * NW, at_bounds(DP, NW)) void k_at_dq(const AtAr
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             const float e = exp2_fast(fmaf(p[b][j][i], c, ls[j]));
-                            s[b][j][i] = e * fmaf(s[b][j][i], 0x1p-31f, -de[j]);
+                            s[b][j][i] = e * fmaf(s[b][j][i], 0x1p-17f, -de[j]);
                         }
                 }
 #pragma unroll
@@ -833,7 +848,7 @@ __global__ __launch_bounds__(64 * NW, at_bounds(DP, NW)) void k_at_dq(const AtAr
         const int64_t row = q0 + 16 * b + (lane & 15);
         if (row >= k1) continue;
         float* o = row_out(a.dq, row, a.H, h, a.D);
-        const int e = ex[TG] + ex[TV] + ex[TK] - 29;
+        const int e = ex[TG] + ex[TV] + ex[TK] - 28;
 #pragma unroll
         for (int d = 0; d < DB; ++d) {
             f32x4 x;
@@ -969,33 +984,33 @@ extern "C" size_t hgv_graph_attention_ws(int64_t N, int num_graphs, int H, int H
 extern "C" int hgv_graph_attention_fwd(const float* q, int64_t q_row, int64_t q_head, const float* k, int64_t k_row, int64_t k_head,
                                        const float* v, int64_t v_row, int64_t v_head, int64_t N, int num_graphs, int H, int Hk, int D,
                                        float scale, const uint8_t* mask, const int32_t* ptr, int max_rows, const int32_t* tiles, int n_tiles,
-                                       const int32_t* blocks, int n64, int n128, float* out, float* lse, void* ws, size_t ws_bytes,
+                                       const int32_t* blocks, int n64, int n128, float* out, float* stats, void* ws, size_t ws_bytes,
                                        hipStream_t stream) {
     AtArgs a = {};
     const int rc = at_fill(a, "graph_attention_fwd", N, num_graphs, H, Hk, D, scale, mask, ptr, max_rows, tiles, n_tiles, blocks, n64, n128, ws, ws_bytes, false);
     if (rc) return rc;
-    HGV_REQUIRE(q && k && v && out && (D % 4 || hgv_aligned(out, 16)), HGV_EINVAL, "graph_attention_fwd: null or misaligned buffer");
+    HGV_REQUIRE(q && k && v && out && (D % 4 || hgv_aligned(out, 16)) && hgv_aligned(stats, 8), HGV_EINVAL, "graph_attention_fwd: null or misaligned buffer");
     a.src[TQ] = q; a.row_stride[TQ] = q_row; a.head_stride[TQ] = q_head;
     a.src[TK] = k; a.row_stride[TK] = k_row; a.head_stride[TK] = k_head;
     a.src[TV] = v; a.row_stride[TV] = v_row; a.head_stride[TV] = v_head;
-    a.out = out; a.lse = lse;
+    a.out = out; a.stats = (float2*)stats;
     return at_dispatch(a, false, stream);
 }
 
 extern "C" int hgv_graph_attention_bwd(const float* q, int64_t q_row, int64_t q_head, const float* k, int64_t k_row, int64_t k_head,
                                        const float* v, int64_t v_row, int64_t v_head, const float* g, int64_t g_row, int64_t g_head,
-                                       const float* out, const float* lse, int64_t N, int num_graphs, int H, int Hk, int D, float scale,
+                                       const float* out, const float* stats, int64_t N, int num_graphs, int H, int Hk, int D, float scale,
                                        const uint8_t* mask, const int32_t* ptr, int max_rows, const int32_t* tiles, int n_tiles, const int32_t* blocks,
                                        int n64, int n128, float* dq, float* dk, float* dv, void* ws, size_t ws_bytes, hipStream_t stream) {
     AtArgs a = {};
     const int rc = at_fill(a, "graph_attention_bwd", N, num_graphs, H, Hk, D, scale, mask, ptr, max_rows, tiles, n_tiles, blocks, n64, n128, ws, ws_bytes, true);
     if (rc) return rc;
-    HGV_REQUIRE(q && k && v && g && out && lse && (dq || dk) && !dk == !dv, HGV_EINVAL, "graph_attention_bwd: null buffer (dk and dv come together)");
+    HGV_REQUIRE(q && k && v && g && out && stats && hgv_aligned(stats, 8) && (dq || dk) && !dk == !dv, HGV_EINVAL, "graph_attention_bwd: null buffer (dk and dv come together)");
     HGV_REQUIRE(D % 4 || (hgv_aligned(dq, 16) && hgv_aligned(dk, 16) && hgv_aligned(dv, 16)), HGV_EINVAL, "graph_attention_bwd: misaligned buffer");
     a.src[TQ] = q; a.row_stride[TQ] = q_row; a.head_stride[TQ] = q_head;
     a.src[TK] = k; a.row_stride[TK] = k_row; a.head_stride[TK] = k_head;
     a.src[TV] = v; a.row_stride[TV] = v_row; a.head_stride[TV] = v_head;
     a.src[TG] = g; a.row_stride[TG] = g_row; a.head_stride[TG] = g_head;
-    a.out = (float*)out; a.lse = (float*)lse; a.dq = dq; a.dk = dk; a.dv = dv;
+    a.out = (float*)out; a.stats = (float2*)stats; a.dq = dq; a.dk = dk; a.dv = dv;
     return at_dispatch(a, true, stream);
 }

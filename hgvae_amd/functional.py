@@ -2749,7 +2749,7 @@ def _strided(t: torch.Tensor):
 
 
 class _GraphAttention(torch.autograd.Function):
-    """softmax(scale q k^T) v within each graph; keeps the output and one number per row and head, and recomputes the
+    """softmax(scale q k^T) v within each graph; keeps the output and two numbers per row and head, and recomputes the
     probabilities in the backward pass."""
 
     @staticmethod
@@ -2760,14 +2760,14 @@ class _GraphAttention(torch.autograd.Function):
         hk = k.size(1)
         out = torch.empty(n, h, d, dtype=torch.float32, device=q.device)
         train = any(ctx.needs_input_grad[:3])
-        lse = torch.empty(h, n, dtype=torch.float32, device=q.device) if train else None
+        stats = torch.empty(h, n, 2, dtype=torch.float32, device=q.device) if train else None
         nws = _lib.load().hgv_graph_attention_ws(n, seg.num_graphs, h, hk, d, seg._n_tiles, 0)
         ws = torch.empty(nws, dtype=torch.uint8, device=q.device)
         _lib.call("hgv_graph_attention_fwd", *_strided(q), *_strided(k), *_strided(v), n, seg.num_graphs, h, hk, d, scale, _lib.ptr(mask),
-                  *seg._attention_plan, out.data_ptr(), _lib.ptr(lse), ws.data_ptr(), nws, _lib.stream())
+                  *seg._attention_plan, out.data_ptr(), _lib.ptr(stats), ws.data_ptr(), nws, _lib.stream())
         ctx.seg, ctx.scale = seg, scale
         if train:
-            ctx.save_for_backward(q, k, v, out, lse, mask)
+            ctx.save_for_backward(q, k, v, out, stats, mask)
         return out
 
     @staticmethod
@@ -2777,7 +2777,7 @@ class _GraphAttention(torch.autograd.Function):
 
     @staticmethod
     def _grads(ctx, g):
-        q, k, v, out, lse, mask = ctx.saved_tensors
+        q, k, v, out, stats, mask = ctx.saved_tensors
         seg, need = ctx.seg, ctx.needs_input_grad
         n, h, d = q.shape
         hk = k.size(1)
@@ -2786,7 +2786,7 @@ class _GraphAttention(torch.autograd.Function):
         dk, dv = (torch.empty(n, hk, d, dtype=torch.float32, device=q.device) if need[1] or need[2] else None for _ in range(2))
         nws = _lib.load().hgv_graph_attention_ws(n, seg.num_graphs, h, hk, d, seg._n_tiles, 1)
         ws = torch.empty(nws, dtype=torch.uint8, device=q.device)
-        _lib.call("hgv_graph_attention_bwd", *_strided(q), *_strided(k), *_strided(v), *_strided(g), out.data_ptr(), lse.data_ptr(), n,
+        _lib.call("hgv_graph_attention_bwd", *_strided(q), *_strided(k), *_strided(v), *_strided(g), out.data_ptr(), stats.data_ptr(), n,
                   seg.num_graphs, h, hk, d, ctx.scale, _lib.ptr(mask), *seg._attention_plan, _lib.ptr(dq), _lib.ptr(dk), _lib.ptr(dv),
                   ws.data_ptr(), nws, _lib.stream())
         return dq, dk if need[1] else None, dv if need[2] else None, None, None, None
@@ -2802,7 +2802,7 @@ def graph_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, segments,
     ``mask`` ``[N]`` bool: nodes that take part as keys; a graph without any gives zeros, and what a masked row of ``k`` or
     ``v`` holds does not matter.  ``scale`` (positive) defaults to ``D ** -0.5``.  Returns ``[N, H, D]``.
 
-    The backward pass recomputes the probabilities from the output and one number per row and head; its results do not
+    The backward pass recomputes the probabilities from the output and two numbers per row and head; its results do not
     depend on the order in which workgroups run.  Gradients cannot be differentiated again."""
     for name, t in (("q", q), ("k", k), ("v", v)):
         if not isinstance(t, torch.Tensor) or t.dim() != 3 or t.dtype != torch.float32:

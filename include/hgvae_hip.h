@@ -618,17 +618,18 @@ int hgv_group_norm_bwd(const float* g, int64_t ldg, const float* x, int64_t ldx,
  * A masked row of k or v may hold anything; its dk and dv are zeros.  scale > 0.
  * Graphs: ptr [num_graphs + 1], the largest has max_rows rows; tiles [n_tiles][4] (graph, first row, first tile of the graph, tiles of the graph) of 64 rows;
  * blocks [n64 + n128][4] (graph, first row, -, -): all tiles of 64 rows, then those of 128, in the order in which they are to run.
- * lse [H, N] (base 2, of the scaled logits; +inf for a row without keys) may be NULL in the forward pass; the backward pass
+ * stats [H, N, 2] (8-byte aligned; per row a whole M with sum_j 2^(logit_j - M) in [1, 2), base 2 of the scaled logits, and the
+ * inverse of that sum; +inf and 0 for a row without keys) may be NULL in the forward pass; the backward pass
  * reads it and out.  dq, or dk and dv together, may be NULL. */
 size_t hgv_graph_attention_ws(int64_t N, int num_graphs, int H, int Hk, int D, int64_t n_tiles, int backward);
 int hgv_graph_attention_fwd(const float* q, int64_t q_row, int64_t q_head, const float* k, int64_t k_row, int64_t k_head, const float* v,
                             int64_t v_row, int64_t v_head, int64_t N, int num_graphs, int H, int Hk, int D, float scale,
                             const uint8_t* mask, const int32_t* ptr, int max_rows, const int32_t* tiles, int n_tiles, const int32_t* blocks,
-                            int n64, int n128, float* out, float* lse, void* ws,
+                            int n64, int n128, float* out, float* stats, void* ws,
                             size_t ws_bytes, hgv_stream_t stream);
 int hgv_graph_attention_bwd(const float* q, int64_t q_row, int64_t q_head, const float* k, int64_t k_row, int64_t k_head, const float* v,
                             int64_t v_row, int64_t v_head, const float* g, int64_t g_row, int64_t g_head, const float* out,
-                            const float* lse, int64_t N, int num_graphs, int H, int Hk, int D, float scale, const uint8_t* mask,
+                            const float* stats, int64_t N, int num_graphs, int H, int Hk, int D, float scale, const uint8_t* mask,
                             const int32_t* ptr, int max_rows, const int32_t* tiles, int n_tiles, const int32_t* blocks, int n64, int n128, float* dq,
                             float* dk, float* dv, void* ws, size_t ws_bytes, hgv_stream_t stream);
 
