@@ -12,9 +12,12 @@
 //
 // Two ways to run:  graphs whose columns of one slab (whole groups, 32 columns or more) fit into the registers of a workgroup
 // are read once (k_gn_small);  larger ones take a pass for the sums over row chunks, a small pass that joins them per graph and
-// a pass that applies them.  Bound by memory: 3 passes over the matrix forward (2 would be the least), 5 backward (3).  Taking the
-// graphs in batches of 48 ... 192 MB, so that the second read meets the memory-side cache, was measured and is slower (1.78 ... 1.37
-// against 1.23 ms for 1.28 M x 138 forward and backward): the ends of the many short launches cost more than the cache brings.
+// a pass that applies them.  Bound by memory: 3 passes over the matrix forward (2 would be the least), 5 backward (3).  1.28 M x 138
+// forward: sums 135 us (5.2 TB/s), applied 280 (5.1);  backward: sums 275 (5.2), applied 423 (5.0); a large copy on the same card
+// reaches 5.2.  Taking the graphs in batches of 48 ... 192 MB, so that the second read meets the memory-side cache, was measured and
+// is slower (forward and backward 1.78 ... 1.37 ms against 1.23 in one piece): the ends of the many short launches cost more than the
+// cache brings.  Streaming loads in the last pass: 160 001 x 256 3 % faster, 1.28 M x 138 (rows that share lines) 1 % slower, not taken.
+// Small graphs (32 x 138 rows x 138): forward 9.4 us, backward 10.5 + 2.8, where the host takes 140.
 #include "pack8.h"
 
 namespace {
