@@ -213,6 +213,11 @@ def stream():
     return torch.cuda.current_stream().cuda_stream
 
 
+def stream_of(index: int):
+    """Handle of torch's current stream on device ``index``."""
+    return _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(index).cuda_stream
+
+
 def current_device() -> int:
     return _cur_device() if _cur_device is not None else torch.cuda.current_device()
 

@@ -946,7 +946,7 @@ __global__ __launch_bounds__(MAXT) void k_gemm_nt16r(const NtHArgs a) {
         // past the last word of the row's 8-bit form repeat that word, halves past the last block repeat that block)
         const int tl = t - mwaves * 64, mr = tl >> 4, mj = P8 ? tl & 15 : min(tl & 15, 11);
         int qoff[EPT], soff[EPT];                     // P8: byte offsets of this lane's words and blocks from the block's first row
-        bool qpad[EPT];                               // ... and whether the word lies behind the last column (zero)
+        int qlive[EPT];                               // ... and how many of a word's four columns there are (the others are zeros)
         int eoff[NSRC][EPT], ewr[NSRC][EPT];          // element offset (floats) from the block's first row; byte offset of its h halves in a stage buffer
 #pragma unroll
         for (int sidx = 0; sidx < NSRC; ++sidx) {
@@ -959,7 +959,7 @@ __global__ __launch_bounds__(MAXT) void k_gemm_nt16r(const NtHArgs a) {
                     const int word = min(8 * blk + (mj & 7), (int)(a.keep_ldq / 4) - 1);
                     qoff[u] = mr * (int)a.keep_ldq + 4 * word;
                     soff[u] = mr * nb + blk;
-                    qpad[u] = word >= nf4;
+                    qlive[u] = g.K1 - 4 * word;
                     f = min(word, nf4 - 1);
                 }
                 eoff[sidx][u] = mr * (int)(sidx ? a.lda2 : a.lda1) + 4 * f;
@@ -1060,7 +1060,7 @@ __global__ __launch_bounds__(MAXT) void k_gemm_nt16r(const NtHArgs a) {
                     uint32_t top = 0;
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        v[e] = qpad[u] ? 0.f : raw[S][0][u][e];
+                        v[e] = e < qlive[u] ? raw[S][0][u][e] : 0.f;
                         top = max(top, __float_as_uint(v[e]) & 0x7fffffffu);
                     }
                     top = max(top, __float_as_uint(dpp_mov<0xB1>(__uint_as_float(top))));       // lanes ^ 1, ^ 2, mirrored in eight

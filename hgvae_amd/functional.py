@@ -2568,10 +2568,10 @@ class _Linear8(torch.autograd.Function):
     """y = x W^T + b that keeps x in 8 bits; the weight gradient is formed from the kept values."""
 
     @staticmethod
-    def forward(ctx, x, w, bias):
-        ctx.leaves = _leaves_of(x, w, bias)
+    def forward(ctx, x, w, bias, train):
+        need = ctx.needs_input_grad if train else (False, False, False)      # a parameter asks for its gradient under no_grad too
+        ctx.leaves = _leaves_of(x, w, bias) if train else ()
         x = _own_rows(x)
-        need = ctx.needs_input_grad
         fwd, ctx.image = _images((w, None, False), (w, None, True) if need[0] else None)
         ctx.packed = None
         if not need[1]:
@@ -2606,7 +2606,7 @@ class _Linear8(torch.autograd.Function):
             gb = g.sum(0)
         if need[0]:
             gx = _gemm_nt(g, ctx.image, None, None, w.size(1))
-        return gx, gw, gb
+        return gx, gw, gb, None
 
 
 def _weight_grad8(g: torch.Tensor, x8: Packed8, want_bias: bool):
@@ -2625,7 +2625,8 @@ def linear8(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = Non
     """``x @ w.T + bias`` with fp32 results, as :func:`dual_linear`, that keeps ``x`` in 8 bits (:func:`pack8`) for the
     backward pass: a quarter of the memory.  The gradients with respect to ``x`` and ``bias`` are those of the exact
     product; the weight gradient is ``g.T @ v`` with ``v`` the 8-bit values of ``x``.  Gradients cannot be differentiated
-    again."""
+    again.  As for every projection, a matrix whose rows are ``K`` rounded up to a multiple of 4 apart holds zeros behind its
+    last column, as all matrices of this package do; other layouts are copied."""
     x = plain(x)
     _check_matrix("x", x)
     _check_matrix("w", w, x.device, x.size(1))
@@ -2634,7 +2635,7 @@ def linear8(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = Non
     bias = _check_vector("bias", bias, w.size(0), x.device)
     if x.size(0) == 0:
         return torch.nn.functional.linear(x, w, bias)           # no rows: an empty matrix, zero gradients
-    return _on_device(x, _Linear8.apply, x, w, bias)
+    return _on_device(x, _Linear8.apply, x, w, bias, torch.is_grad_enabled())
 
 
 # --------------------------------------------------------------------------------------
@@ -2648,8 +2649,8 @@ class _GroupNormAct(torch.autograd.Function):
     from x, or from its 8-bit form."""
 
     @staticmethod
-    def forward(ctx, x, w, b, seg: Segments, groups, act, eps, keep8):
-        ctx.leaves = _leaves_of(x, w, b)
+    def forward(ctx, x, w, b, seg: Segments, groups, act, eps, keep8, train):
+        ctx.leaves = _leaves_of(x, w, b) if train else ()
         x = rowmajor(x)
         n, c = x.shape
         dev = x.device
@@ -2662,7 +2663,7 @@ class _GroupNormAct(torch.autograd.Function):
         tail = (out.data_ptr(), out.stride(0), mean.data_ptr(), rstd.data_ptr(), ws.data_ptr(), nws, _lib.stream())
         ctx.seg, ctx.cfg = seg, (groups, act)
         ctx.packed = None
-        if keep8 and any(ctx.needs_input_grad[:3]):
+        if keep8 and train and any(ctx.needs_input_grad[:3]):
             p = _empty8(n, c, dev)
             _lib.call("hgv_group_norm_fwd8", *head, n, p.q.data_ptr(), p.q.stride(0), p.scale.data_ptr(), *tail)
             ctx.packed = p.shape
@@ -2697,7 +2698,7 @@ class _GroupNormAct(torch.autograd.Function):
         _lib.call("hgv_group_norm_bwd", g.data_ptr(), ld_of(g), *source, c, groups, act, _lib.ptr(w), _lib.ptr(b), *arrays, *counts,
                   mean.data_ptr(), rstd.data_ptr(), _lib.ptr(gx), gx.stride(0) if gx is not None else 0, _lib.ptr(gw), _lib.ptr(gb),
                   ws.data_ptr(), nws, _lib.stream())
-        return gx, gw, gb, None, None, None, None, None
+        return gx, gw, gb, None, None, None, None, None, None
 
 
 def group_norm_act(x: torch.Tensor, segments, groups: int, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
@@ -2714,7 +2715,8 @@ def group_norm_act(x: torch.Tensor, segments, groups: int, weight: Optional[torc
     _check_matrix("x", x)
     if act not in _ACTS:
         raise _lib.HgvError(f"unknown activation {act!r} (one of {', '.join(_ACTS)})")
-    groups = int(groups)
+    if not isinstance(groups, int):
+        raise _lib.HgvError(f"groups must be an integer, got {groups!r}")
     if groups < 1 or x.size(1) < 1 or x.size(1) % groups:
         raise _lib.HgvError(f"{x.size(1)} columns cannot be split into {groups} groups")
     if not eps >= 0.0:
@@ -2731,7 +2733,7 @@ def _group_norm_act(x, segments, groups, weight, bias, act, eps, keep8):
     if x.size(0) == 0:                                          # an empty matrix whose gradients are zeros
         y = x * 1.0 if weight is None else x * weight
         return y if bias is None else y + bias
-    return _GroupNormAct.apply(x, weight, bias, seg, groups, act, eps, keep8)
+    return _GroupNormAct.apply(x, weight, bias, seg, groups, act, eps, keep8, torch.is_grad_enabled())
 
 
 # --------------------------------------------------------------------------------------
@@ -2753,13 +2755,13 @@ class _GraphAttention(torch.autograd.Function):
     probabilities in the backward pass."""
 
     @staticmethod
-    def forward(ctx, q, k, v, seg: Segments, mask, scale):
-        ctx.leaves = _leaves_of(q, k, v)
+    def forward(ctx, q, k, v, seg: Segments, mask, scale, train):
+        ctx.leaves = _leaves_of(q, k, v) if train else ()
         q, k, v = _unit_rows(q), _unit_rows(k), _unit_rows(v)
         n, h, d = q.shape
         hk = k.size(1)
         out = torch.empty(n, h, d, dtype=torch.float32, device=q.device)
-        train = any(ctx.needs_input_grad[:3])
+        train = train and any(ctx.needs_input_grad[:3])
         stats = torch.empty(h, n, 2, dtype=torch.float32, device=q.device) if train else None
         nws = _lib.load().hgv_graph_attention_ws(n, seg.num_graphs, h, hk, d, seg._n_tiles, 0)
         ws = torch.empty(nws, dtype=torch.uint8, device=q.device)
@@ -2789,7 +2791,7 @@ class _GraphAttention(torch.autograd.Function):
         _lib.call("hgv_graph_attention_bwd", *_strided(q), *_strided(k), *_strided(v), *_strided(g), out.data_ptr(), stats.data_ptr(), n,
                   seg.num_graphs, h, hk, d, ctx.scale, _lib.ptr(mask), *seg._attention_plan, _lib.ptr(dq), _lib.ptr(dk), _lib.ptr(dv),
                   ws.data_ptr(), nws, _lib.stream())
-        return dq, dk if need[1] else None, dv if need[2] else None, None, None, None
+        return dq, dk if need[1] else None, dv if need[2] else None, None, None, None, None
 
 
 def graph_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, segments, mask: Optional[torch.Tensor] = None,
@@ -2834,4 +2836,4 @@ def _graph_attention(q, k, v, segments, mask, scale):
         raise _lib.HgvError(f"segments are on {seg.device}, q is on {q.device}")
     if q.size(0) == 0:
         return q * 1.0 + (k.sum() + v.sum()) * 0.0              # an empty result whose gradients are zeros
-    return _GraphAttention.apply(q, k, v, seg, mask, scale)
+    return _GraphAttention.apply(q, k, v, seg, mask, scale, torch.is_grad_enabled())

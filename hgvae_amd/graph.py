@@ -258,7 +258,7 @@ class Segments:
     have no rows.  Building one uploads a few arrays (and, from a device tensor, reads the sizes back: one host
     synchronisation); a plan serves every call, stream and captured graph afterwards, so a loop keeps it next to its batch.
     """
-    MAX_ROWS = 2 ** 31 - 1
+    MAX_ROWS = 2 ** 31 - 2 ** 16                                # row numbers are 32 bits, and loops step beyond the last one
 
     def __init__(self, sizes: Sequence[int], device):
         sizes = np.asarray(list(sizes) if not isinstance(sizes, np.ndarray) else sizes)
@@ -266,7 +266,7 @@ class Segments:
             raise _lib.HgvError("Segments: sizes must be a sequence of integers")
         sizes = sizes.astype(np.int64)
         if sizes.size and (int(sizes.min()) < 0 or int(sizes.max()) > self.MAX_ROWS or int(sizes.sum()) > self.MAX_ROWS):
-            raise _lib.HgvError("Segments: sizes must be >= 0 and sum to less than 2^31 rows")
+            raise _lib.HgvError(f"Segments: sizes must be >= 0 and sum to at most {self.MAX_ROWS} rows")
         self.device = torch.device(device)
         if self.device.type != "cuda":
             raise _lib.HgvError("hgvae_amd operators run on the GPU only (Segments needs a cuda device)")
@@ -300,11 +300,15 @@ class Segments:
         parts = [chunks.ravel(), tiles.ravel(), np.concatenate(blocks).ravel(), ptr, order, first]
         host = np.concatenate(parts).astype(np.int32)
         self._buf = torch.from_numpy(host).to(self.device)          # copied before the call returns: any stream may read it
+        self._home = _lib.stream_of(self.device.index)
         at = np.cumsum([0] + [p.size for p in parts])
         self._chunks, self._tiles, self._blocks, self._ptr, self._order, self._first = (self._buf[at[i]:at[i + 1]] for i in range(6))
         self._norm_plans: "dict[tuple, tuple]" = {}
         self._attention_plan = (self._ptr.data_ptr(), self._sorted[-1] if self._sorted else 0, self._tiles.data_ptr(), self._n_tiles,
                                 self._blocks.data_ptr(), *map(len, blocks))
+
+    def __reduce__(self):
+        return Segments, (self.sizes, str(self.device))             # copies and pickles get arrays of their own
 
     @staticmethod
     def _tiles_of(sizes, ptr, graphs, rows: int) -> np.ndarray:
@@ -346,6 +350,8 @@ class Segments:
             if int(num_graphs) < count:
                 raise _lib.HgvError(f"Segments: batch names graph {count - 1} of {num_graphs}")
             count = int(num_graphs)
+        if count > cls.MAX_ROWS:
+            raise _lib.HgvError(f"Segments: {count} graphs")
         return cls(np.bincount(host, minlength=count) if host.size else np.zeros(count, dtype=np.int64), batch.device)
 
     def _norm_plan(self, columns: int, groups: int):
@@ -376,4 +382,7 @@ def segments_of(segments, num_rows: int) -> Segments:
         segments = Segments.from_batch(segments)
     if segments.num_rows != num_rows:
         raise _lib.HgvError(f"the matrix has {num_rows} rows but the graphs have {segments.num_rows}")
+    index = segments.device.index
+    if _lib.stream_of(index) != segments._home and not torch.cuda.is_current_stream_capturing():
+        segments._buf.record_stream(torch.cuda.current_stream(index))       # a plan that is dropped outlives what reads it there
     return segments

@@ -216,3 +216,71 @@ def test_modules_repr_and_second_derivatives_are_refused():
         (first,) = torch.autograd.grad((out ** 2).sum(), (leaf,), create_graph=True)
         with pytest.raises(RuntimeError):
             torch.autograd.grad(first.sum(), (leaf,))
+
+
+def test_evaluation_keeps_nothing(monkeypatch):
+    """Under no_grad a module's parameters still ask for gradients: no 8-bit forms, statistics or leaves are kept for them."""
+    from hgvae_amd import Segments, _lib
+    from hgvae_amd import functional as Fn
+    level = Level(64, 8, 4, 2, True).to(dev())
+    seg = Segments.from_sizes([1500, 300], dev())
+    x = torch.randn(1800, 64, device=dev())
+    want = level(x, seg).detach()
+    names, real = [], _lib.call
+    count = len(Fn._leaf_streams)
+    monkeypatch.setattr(_lib, "call", lambda name, *args: (names.append(name), real(name, *args))[1])
+    with torch.no_grad():
+        got = level(x, seg)
+    assert torch.equal(got, want) and not [n for n in names if n.endswith("8") or n == "hgv_pack8"]
+    assert len(Fn._leaf_streams) == count
+    names.clear()
+    level(x, seg)
+    assert "hgv_group_norm_fwd8" in names and "hgv_gemm_nt16h_keep8" in names
+
+
+def test_plan_dropped_while_another_stream_reads_it():
+    """A plan used on a second stream and dropped at once: its memory is not handed out before that stream is done."""
+    from hgvae_amd import Segments
+    from hgvae_amd import functional as Fn
+    n = 300 * 700
+    x = torch.randn(n, 64, device=dev())
+    want = Fn.group_norm_act(x, Segments.from_sizes([300] * 700, dev()), 8)
+    side = torch.cuda.Stream()
+    for _ in range(5):
+        seg = Segments.from_sizes([300] * 700, dev())
+        size = seg._buf.numel()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            for _ in range(8):
+                got = Fn.group_norm_act(x, seg, 8)
+        del seg
+        torch.zeros(size, dtype=torch.int32, device=dev())        # would land in the plan's memory, on the first stream
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+
+
+def test_copies_of_a_plan_have_arrays_of_their_own():
+    import copy
+    import pickle
+    from hgvae_amd import Segments
+    from hgvae_amd import functional as Fn
+    x = torch.randn(430, 24, device=dev())
+    seg = Segments.from_sizes([400, 0, 30], dev())
+    want = Fn.group_norm_act(x, seg, 3), Fn.graph_attention(*(x.view(430, 3, 8),) * 3, seg)
+    for other in (copy.deepcopy(seg), copy.copy(seg), pickle.loads(pickle.dumps(seg))):
+        assert other.sizes == seg.sizes and other.device == seg.device and other._ptr.data_ptr() != seg._ptr.data_ptr()
+        assert other._attention_plan[0] == other._ptr.data_ptr()
+        got = Fn.group_norm_act(x, other, 3), Fn.graph_attention(*(x.view(430, 3, 8),) * 3, other)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_empty_batches_through_the_modules():
+    from hgvae_amd import Segments
+    level = Level(24, 3, 4, 2, True).to(dev())
+    for sizes in ([], [0, 0]):
+        x = torch.zeros(0, 24, device=dev(), requires_grad=True)
+        out = level(x, Segments.from_sizes(sizes, dev()))
+        assert out.shape == (0, 24)
+        out.sum().backward()
+        assert x.grad.shape == (0, 24) and all(not bool(p.grad.any()) for p in level.parameters())
+        level.zero_grad()

@@ -193,3 +193,16 @@ def test_projection_keeps_the_8bit_form(n, k, m):
     want = Fn.pack8(x)
     assert torch.equal(q, want.q) and torch.equal(scale, want.scale)
     assert torch.equal(y.detach(), Fn.linear8(x, w, b))
+
+
+@pytest.mark.parametrize("k", [97, 138, 143])
+def test_kept_form_ignores_what_lies_behind_the_last_column(k):
+    """Row pitch K rounded up to 4, foreign values there: they are not part of the last block."""
+    from hgvae_amd import functional as Fn
+    wide = torch.randn(500, (k + 3) // 4 * 4, device=dev())
+    wide[:, k:] = 1e4
+    x = wide[:, :k]
+    y = Fn.linear8(x, torch.randn(40, k, device=dev(), requires_grad=True))
+    q, scale = (t for t in y.grad_fn.saved_tensors if t.dtype in (torch.int8, torch.uint8))
+    want = Fn.pack8(x.contiguous())
+    assert torch.equal(q, want.q) and torch.equal(scale, want.scale)

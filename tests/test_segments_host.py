@@ -12,7 +12,7 @@ def test_segments_refuse_what_they_cannot_hold():
                  lambda: Segments.from_sizes([2 ** 31 - 1, 2]), lambda: Segments.from_sizes([0.5]), lambda: Segments.from_sizes(np.zeros((2, 2), dtype=np.int64)),
                  lambda: Segments.from_ptr(torch.tensor([1, 2])), lambda: Segments.from_ptr(torch.tensor([0, 3, 2])), lambda: Segments.from_ptr(torch.zeros(0, dtype=torch.long)),
                  lambda: Segments.from_ptr(torch.tensor([0.0, 1.0])), lambda: Segments.from_batch(torch.tensor([1, 0])), lambda: Segments.from_batch(torch.tensor([-1, 0])),
-                 lambda: Segments.from_batch(torch.tensor([0, 2]), num_graphs=2), lambda: Segments.from_batch(torch.zeros(2, 2, dtype=torch.long))):
+                 lambda: Segments.from_batch(torch.tensor([0, 2]), num_graphs=2), lambda: Segments.from_batch(torch.tensor([0, 2 ** 40])), lambda: Segments.from_batch(torch.zeros(2, 2, dtype=torch.long))):
         with pytest.raises(_lib.HgvError):
             call()
 
