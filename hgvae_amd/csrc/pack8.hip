@@ -7,6 +7,7 @@
 // significant bits: it is exact in bf16 too, which is what the weight gradient reads.  |value - x| <= 2^(e-1) <= amax / 126
 // for amax >= 2^-120.  A block that holds an infinity or a NaN gets the byte 255 and reads back as NaN.
 #include "pack8.h"
+#include <type_traits>
 
 namespace {
 
@@ -142,7 +143,8 @@ namespace {
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
-constexpr int T8_ROWS = 32, T8_W = 144, T8_LINE = 2 * T8_W, T8_PIECE = T8_ROWS * T8_LINE, T8_BUF = 4 * T8_PIECE, T8_LDS = 2 * T8_BUF + T8_ROWS * 32, T8_THREADS = 576;
+constexpr int T8_ROWS = 32, T8_W = 144, T8_LINE = 2 * T8_W, T8_PIECE = T8_ROWS * T8_LINE, T8_BUF = 4 * T8_PIECE, T8_LDS = 2 * T8_BUF + T8_ROWS * 32;
+constexpr int T8_MOVERS = 384, T8_THREADS = 576 + T8_MOVERS, T8_Q = T8_ROWS * (T8_W / 4) / T8_MOVERS;      // three quads of four columns per mover and tile
 constexpr int T8_SET = (81 + 9) * 256;                          // floats of a partial set: 81 tiles, nine tiles of column sums
 
 struct Tn8Args {
@@ -165,107 +167,133 @@ __device__ __forceinline__ bf16x8 t8_read(const unsigned char* p, int line = T8_
     return u.v;
 }
 
-__global__ __launch_bounds__(T8_THREADS, 5) void k_gemm_tn8(const Tn8Args a) {
+// Waves 0 ... 8 multiply, waves 9 ... 14 move: between two barriers the products of a tile run beside the splitting of the next one
+// and the loads of the one after that.
+__global__ __launch_bounds__(T8_THREADS) void k_gemm_tn8(const Tn8Args a) {
     extern __shared__ __align__(16) unsigned char t8_lds[];
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int per = a.ngrps * a.kgrps, grp = blockIdx.x % per, set = blockIdx.x / per;
     const int ng = grp / a.kgrps, kg = grp - ng * a.kgrps;
     const int n0 = T8_W * ng, k0 = T8_W * kg, n_w = min(T8_W, a.N - n0), k_w = min(T8_W, a.K - k0);
-    const int64_t lo = set, hi = a.steps, by_n = a.sets;
     const int nt = (n_w + 15) / 16, kt = (k_w + 15) / 16;
-    // this thread's two quads of the tile: the same four columns, 16 rows apart
-    const int row = t / 36, c = 4 * (t - 36 * row);
-    const bool g_live = c < n_w, v_live = c < k_w;
-    // one offset per lane; what depends on the tile is uniform
-    const uint32_t go = (uint32_t)(row * a.ldg + c), qo = (uint32_t)(row * a.ldq + c), so = (uint32_t)(row * a.nb + ((k0 + c) >> 5));
-    float4 g[2];
-    uint32_t w[2];
-    int by[2];
-    auto load = [&](int64_t s) __attribute__((always_inline)) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int64_t n = s * T8_ROWS + 16 * i;
-            const float* gp = a.G + n * a.ldg + n0;
-            const int8_t* qp = a.q + n * a.ldq + k0;
-            const uint8_t* sp = a.scale + n * a.nb;
-            g[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-            w[i] = 0; by[i] = 127;
-            if (n + row < a.M) {
-                if (g_live) g[i] = *(const float4*)(gp + go);
-                if (v_live) {
-                    w[i] = *(const uint32_t*)(qp + qo);
-                    by[i] = sp[so];
-                }
-            }
-        }
-    };
-    auto put = [&](int b) __attribute__((always_inline)) {
-        unsigned char* base = t8_lds + b * T8_BUF + row * T8_LINE + 2 * c;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const float x[4] = {g[i].x, g[i].y, g[i].z, g[i].w};
-            uint32_t p[3][4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                p[0][e] = __float_as_uint(x[e]);
-                const float r = x[e] - __uint_as_float(p[0][e] & 0xffff0000u);          // exact
-                p[1][e] = __float_as_uint(r);
-                p[2][e] = __float_as_uint(r - __uint_as_float(p[1][e] & 0xffff0000u));  // exact, eight bits left
-            }
-            float v[4];
-            p8_values4(w[i], by[i], v);
-            const uint32_t vb[4] = {__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
-            unsigned char* at = base + 16 * i * T8_LINE;
-#pragma unroll
-            for (int j = 0; j < 3; ++j) *(uint2*)(at + j * T8_PIECE) = t8_pack(p[j]);
-            *(uint2*)(at + 3 * T8_PIECE) = t8_pack(vb);
-        }
-    };
-    f32x4 acc[9], accb = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int k = 0; k < 9; ++k) acc[k] = f32x4{0.f, 0.f, 0.f, 0.f};
+    // tiles set, set + sets, ...; the intervals are a multiple of two (the slot of a tile is a compile-time index), past the end the
+    // movers bring the last tile again and nobody multiplies it
+    const int64_t mine = (a.steps - set + a.sets - 1) / a.sets, intervals = (mine + 1) / 2 * 2, last = mine - 1;
     // a tile of ones behind the two buffers, for the column sums
     for (int i = t; i < T8_ROWS * 4; i += T8_THREADS) *(uint2*)(t8_lds + 2 * T8_BUF + i * 8) = make_uint2(0x3f803f80u, 0x3f803f80u);
-    const int i16 = lane & 15;
-    const int at = (4 * (lane >> 4) + (i16 >> 2)) * T8_LINE + (i16 & 3) * 8;
-    if (lo < hi) {
-        load(lo);
-        put(0);
-        if (lo + by_n < hi) load(lo + by_n);
-    }
-    __syncthreads();
-    int b = 0;
-    for (int64_t s = lo; s < hi; s += by_n, b ^= 1) {
-        if (s + by_n < hi) {
-            put(b ^ 1);
-            if (s + 2 * by_n < hi) load(s + 2 * by_n);
+    if (wave < 9) {
+        f32x4 acc[9], accb = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < 9; ++k) acc[k] = f32x4{0.f, 0.f, 0.f, 0.f};
+        const int i16 = lane & 15;
+        const int at = (4 * (lane >> 4) + (i16 >> 2)) * T8_LINE + (i16 & 3) * 8;
+        __syncthreads();
+        for (int64_t it = 0; it < intervals; ++it) {
+            if (it < mine && wave < nt) {
+                const unsigned char* base = t8_lds + (it & 1) * T8_BUF + at;
+                bf16x8 gf[3];
+#pragma unroll
+                for (int j = 0; j < 3; ++j) gf[j] = t8_read(base + j * T8_PIECE + wave * 32);
+#pragma unroll
+                for (int k = 0; k < 9; ++k)
+                    if (k < kt) {
+                        const bf16x8 v = t8_read(base + 3 * T8_PIECE + k * 32);
+#pragma unroll
+                        for (int j = 2; j >= 0; --j) acc[k] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(gf[j], v, acc[k], 0, 0, 0);
+                    }
+                if (kg == 0) {
+                    const bf16x8 ones = t8_read(t8_lds + 2 * T8_BUF + (4 * (lane >> 4) + (i16 >> 2)) * 32 + (i16 & 3) * 8, 32);
+#pragma unroll
+                    for (int j = 2; j >= 0; --j) accb = __builtin_amdgcn_mfma_f32_16x16x32_bf16(gf[j], ones, accb, 0, 0, 0);
+                }
+            }
+            __syncthreads();
         }
         if (wave < nt) {
-            const unsigned char* base = t8_lds + b * T8_BUF + at;
-            bf16x8 gf[3];
-#pragma unroll
-            for (int j = 0; j < 3; ++j) gf[j] = t8_read(base + j * T8_PIECE + wave * 32);
+            float* out = a.partial + ((int64_t)grp * a.sets + set) * T8_SET + lane * 4;
 #pragma unroll
             for (int k = 0; k < 9; ++k)
-                if (k < kt) {
-                    const bf16x8 v = t8_read(base + 3 * T8_PIECE + k * 32);
-#pragma unroll
-                    for (int j = 2; j >= 0; --j) acc[k] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(gf[j], v, acc[k], 0, 0, 0);
-                }
-            if (kg == 0) {
-                const bf16x8 ones = t8_read(t8_lds + 2 * T8_BUF + (4 * (lane >> 4) + (i16 >> 2)) * 32 + (i16 & 3) * 8, 32);
-#pragma unroll
-                for (int j = 2; j >= 0; --j) accb = __builtin_amdgcn_mfma_f32_16x16x32_bf16(gf[j], ones, accb, 0, 0, 0);
-            }
+                if (k < kt) *(f32x4*)(out + (wave * 9 + k) * 256) = acc[k];
+            if (kg == 0) *(f32x4*)(out + (81 + wave) * 256) = accb;
         }
-        __syncthreads();
-    }
-    if (wave < nt) {
-        float* out = a.partial + ((int64_t)grp * a.sets + set) * T8_SET + lane * 4;
+    } else {
+        // quads m, m + 384, m + 768 of the tile's 32 x 36.  One offset per quad; what depends on the tile is uniform; quads outside the
+        // matrices read their first columns or last row and count as zeros.
+        const int m = t - 9 * 64;
+        uint32_t go[T8_Q], qo[T8_Q], so[T8_Q];
+        int row[T8_Q], to[T8_Q];
+        bool g_live[T8_Q], v_live[T8_Q];
 #pragma unroll
-        for (int k = 0; k < 9; ++k)
-            if (k < kt) *(f32x4*)(out + (wave * 9 + k) * 256) = acc[k];
-        if (kg == 0) *(f32x4*)(out + (81 + wave) * 256) = accb;
+        for (int i = 0; i < T8_Q; ++i) {
+            const int f = m + T8_MOVERS * i, c = 4 * (f % (T8_W / 4));
+            row[i] = f / (T8_W / 4);
+            g_live[i] = c < n_w; v_live[i] = c < k_w;
+            go[i] = (uint32_t)(g_live[i] ? c : 0); qo[i] = (uint32_t)(v_live[i] ? c : 0);
+            so[i] = (k0 + qo[i]) >> 5;
+            to[i] = row[i] * T8_LINE + 2 * c;
+        }
+        f32x4 g[2][T8_Q];
+        uint32_t w[2][T8_Q];
+        int by[2][T8_Q];
+        auto load = [&](auto slot, int64_t it) __attribute__((always_inline)) {
+            constexpr int S = decltype(slot)::value;
+            const int64_t r0 = (set + min(it, last) * a.sets) * T8_ROWS;
+            const int rows = (int)min(a.M - r0, (int64_t)T8_ROWS);          // 1 ... 32
+            const float* gp = a.G + r0 * a.ldg + n0;
+            const int8_t* qp = a.q + r0 * a.ldq + k0;
+            const uint8_t* sp = a.scale + r0 * a.nb;
+#pragma unroll
+            for (int i = 0; i < T8_Q; ++i) {
+                const int r = min(row[i], rows - 1);
+                g[S][i] = *(const f32x4*)(gp + (uint32_t)(r * (int)a.ldg) + go[i]);
+                w[S][i] = *(const uint32_t*)(qp + (uint32_t)(r * (int)a.ldq) + qo[i]);
+                by[S][i] = sp[(uint32_t)(r * a.nb) + so[i]];
+            }
+        };
+        auto put = [&](auto slot, int64_t it) __attribute__((always_inline)) {
+            constexpr int S = decltype(slot)::value;
+            unsigned char* base = t8_lds + (it & 1) * T8_BUF;
+            const int rows = (int)min(a.M - (set + min(it, last) * a.sets) * T8_ROWS, (int64_t)T8_ROWS);
+#pragma unroll
+            for (int i = 0; i < T8_Q; ++i) asm volatile("" : "+v"(g[S][i]), "+v"(w[S][i]), "+v"(by[S][i]));      // used from here on
+#pragma unroll
+            for (int i = 0; i < T8_Q; ++i) {
+                const bool in = row[i] < rows, gi = in && g_live[i], vi = in && v_live[i];
+                uint32_t p[3][4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float x = gi ? g[S][i][e] : 0.f;
+                    p[0][e] = __float_as_uint(x);
+                    const float r = x - __uint_as_float(p[0][e] & 0xffff0000u);              // exact
+                    p[1][e] = __float_as_uint(r);
+                    p[2][e] = __float_as_uint(r - __uint_as_float(p[1][e] & 0xffff0000u));  // exact, eight bits left
+                }
+                float v[4];
+                p8_values4(vi ? w[S][i] : 0u, vi ? by[S][i] : 127, v);
+                const uint32_t vb[4] = {__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
+                unsigned char* at = base + to[i];
+#pragma unroll
+                for (int j = 0; j < 3; ++j) *(uint2*)(at + j * T8_PIECE) = t8_pack(p[j]);
+                *(uint2*)(at + 3 * T8_PIECE) = t8_pack(vb);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        };
+        constexpr std::integral_constant<int, 0> S0{};
+        constexpr std::integral_constant<int, 1> S1{};
+        load(S0, 0);
+        load(S1, 1);
+        put(S0, 0);
+        __syncthreads();
+        for (int64_t it = 0; it < intervals; it += 2) {
+            load(S0, it + 2);
+            __builtin_amdgcn_sched_barrier(0);
+            put(S1, it + 1);
+            __syncthreads();
+            load(S1, it + 3);
+            __builtin_amdgcn_sched_barrier(0);
+            put(S0, it + 2);
+            __syncthreads();
+        }
     }
 }
 
