@@ -131,13 +131,12 @@ extern "C" int hgv_unpack8(const int8_t* q, int64_t ldq, const uint8_t* scale, i
 // bf16 pieces of G (8 bits each, cut: together all 24) make the product exact up to its fp32 accumulation: three piece products
 // where two fp32 operands take six.
 //
-// A workgroup of nine waves takes 144 x 144 outputs over every sets-th tile of 32 rows: G is split and V widened on the way into
-// LDS (row-major, 288 bytes per row, which spreads the eight rows of a transposing load over all banks), two buffers, the next
-// tile's loads in flight during the products.  Wave w owns columns 16 w .. of G and all columns of V; the column sums are a product
-// with a tile of ones.  Partial sums are added in fp64 in a fixed order by k_tn8_reduce.
-// 1.28 M rows, 138 x 138: 260 us = 3.4 TB/s (the six-product kernel over the unpacked matrix: 400, and 165 for unpacking).  Matrix
-// cores 30 %, vector units 36 %, LDS 21 % of the time: splitting, LDS and products of a tile follow one another behind one barrier.
-// Measured without effect: two workgroups per unit, two to four tiles in flight, half of the waves splitting behind their products.
+// A workgroup takes 144 x 144 outputs over every sets-th tile of 32 rows: G is split and V widened on the way into LDS (row-major,
+// 288 bytes per row, which spreads the eight rows of a transposing load over all banks), two buffers.  Wave w of nine owns columns
+// 16 w .. of G and all columns of V; the column sums are a product with a tile of ones.  Six more waves load and split, so that this
+// runs beside the products.  Partial sums are added in fp64 in a fixed order by k_tn8_reduce.
+// 1.28 M rows, 138 x 138: 219 us = 4.1 TB/s (nine waves that split and multiply in turn 260, with four movers 227; the six-product
+// kernel over the unpacked matrix 400, and 165 for unpacking).  Three or four tiles in flight instead of two: 241 and 235.
 namespace {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
