@@ -45,7 +45,7 @@ struct AtArgs {
     _Float16* img[4];                                           // [heads][N][hi DP | lo DP]
     float* out;                                                 // [N, H, D]
     float2* stats;                                              // [H, N] of a row: whole M with sum_j 2^(logit_j - M) in [1, 2), and 1 / that sum
-    float* delta;                                               // [H, N] sum_d do * o, scaled (backward)
+    float* delta;                                               // [H, N] sum_d do * o over the row's sum, times 2^(13 - exponent of do)
     float* dq; float* dk; float* dv;                            // [N, H or Hk, D]
 };
 
@@ -85,19 +85,36 @@ __device__ __forceinline__ void over_sum(const AtArgs& a, int64_t n, int h, floa
     for (int e = 0; e < E; ++e) v[e] *= f;
 }
 
-// The exponent e with |row| < 2^e of the longest row among rows n0 .. n0 + rows - 1 of key head hk, over the whole workgroup
-// (NO_EXP: none that is finite and not zero).  red: four ints of LDS, free to be written.
+// A vector of an operand, as it is split: masked keys are zeros, the gradient is over its row's sum.
 template <int DP, bool VEC>
-__device__ __forceinline__ int longest_row(const AtArgs& a, int ten, int hk, int64_t n0, int rows, int* red) {
-    const int per = (ten == TQ || ten == TG) ? a.R : 1, sub = threadIdx.x & 15;
+__device__ __forceinline__ void load_vec(const AtArgs& a, int ten, int64_t n, int h, float v[DP / 16]) {
     const bool masked = a.mask && (ten == TK || ten == TV);
+    load_part<DP, VEC>(a.src[ten] + n * a.row_stride[ten] + h * a.head_stride[ten], threadIdx.x & 15, a.D, !(masked && !a.mask[n]), v);
+    if (ten == TG) over_sum<DP / 16>(a, n, h, v);
+}
+
+// The largest of the workgroup's values.  red: four ints of LDS.
+__device__ __forceinline__ int max_of_all(int v, int* red) {
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) v = max(v, __shfl_xor(v, o, 64));
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    return max(max(red[0], red[1]), max(red[2], red[3]));
+}
+
+// One workgroup per (tile, tensor, key head) leaves the exponent e with |row| < 2^e of the tile's longest row (NO_EXP: none that is
+// finite and not zero).
+template <int DP, bool VEC>
+__global__ __launch_bounds__(256) void k_at_norms(const AtArgs a, const int first) {
+    __shared__ int red[4];
+    const int ten = first + blockIdx.y, hk = blockIdx.z;
+    const int4 tile = a.tiles[blockIdx.x];
+    const int rows = min(64, (int)(a.ptr[tile.x + 1] - tile.y)), per = (ten == TQ || ten == TG) ? a.R : 1;
     int best = NO_EXP;
     for (int i = threadIdx.x >> 4; i < rows * per; i += 16) {
-        const int r = i / per, h = hk * per + i - r * per;
-        const int64_t n = n0 + r;
+        const int r = i / per;
         float v[DP / 16];
-        load_part<DP, VEC>(a.src[ten] + n * a.row_stride[ten] + h * a.head_stride[ten], sub, a.D, !(masked && !a.mask[n]), v);
-        if (ten == TG) over_sum<DP / 16>(a, n, h, v);
+        load_vec<DP, VEC>(a, ten, tile.y + r, hk * per + i - r * per, v);
         double s = 0.0;
 #pragma unroll
         for (int e = 0; e < DP / 16; ++e) s = fma((double)v[e], (double)v[e], s);
@@ -106,64 +123,32 @@ __device__ __forceinline__ int longest_row(const AtArgs& a, int ten, int hk, int
         const int e2 = (int)((__double_as_longlong(s) >> 52) & 2047) - 1023;
         if (s > 0.0 && s < 1e300) best = max(best, (e2 >> 1) + 1);      // rows that hold an infinity or NaN do not count
     }
-#pragma unroll
-    for (int o = 16; o < 64; o <<= 1) best = max(best, __shfl_xor(best, o, 64));
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = best;
-    __syncthreads();
-    best = max(max(red[0], red[1]), max(red[2], red[3]));
-    __syncthreads();
-    return best;
-}
-
-// Graphs of more than four tiles: one workgroup per (tile, tensor, key head) leaves the exponent of its tile.
-template <int DP, bool VEC>
-__global__ __launch_bounds__(256) void k_at_norms(const AtArgs a, const int first) {
-    __shared__ int red[4];
-    const int ten = first + blockIdx.y, hk = blockIdx.z;
-    const int4 tile = a.tiles[blockIdx.x];
-    const int best = longest_row<DP, VEC>(a, ten, hk, tile.y, min(64, (int)(a.ptr[tile.x + 1] - tile.y)), red);
+    best = max_of_all(best, red);
     if (threadIdx.x == 0) a.part[((int64_t)blockIdx.x * 4 + ten) * a.Hk + hk] = best;
 }
 
-// The exponent of a (graph, tensor, key head): from its tiles, or (SELF, graphs of up to four tiles) from the rows themselves, which
-// saves a launch.
-template <int DP, bool VEC, bool SELF>
-__device__ __forceinline__ int graph_exp(const AtArgs& a, int4 tile, int ten, int hk, int* red) {
-    int e = NO_EXP;
-    if (SELF) {
-        e = longest_row<DP, VEC>(a, ten, hk, a.ptr[tile.x], (int)(a.ptr[tile.x + 1] - a.ptr[tile.x]), red);
-    } else {
-        for (int i = threadIdx.x; i < tile.w; i += 256) e = max(e, a.part[((int64_t)(tile.z + i) * 4 + ten) * a.Hk + hk]);
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) e = max(e, __shfl_xor(e, o, 64));
-        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = e;
-        __syncthreads();
-        e = max(max(red[0], red[1]), max(red[2], red[3]));
-        __syncthreads();
-    }
-    return e == NO_EXP ? 0 : e;
-}
-
-// One workgroup per (tile, tensor, key head).  The gradient's also takes the dot products with the output.
-template <int DP, bool VEC, bool SELF>
+// One workgroup per (tile, tensor, key head) splits its rows with the exponent of the graph.  The gradient's also takes the dot products
+// with the output.  Bound by memory: 32 graphs of about 5 000 nodes, four heads of 64: exponents 95 us (5.2 TB/s), pieces 168 (5.8).
+// (Small graphs without the first launch, every workgroup looking through its whole graph, or one workgroup per graph that keeps it in
+// registers: 32 x 138 nodes with the gradient 25 us, in two launches 19; 2 000 x 250 nodes 2.1 and 3.1 ms, in two launches 1.4.)
+template <int DP, bool VEC>
 __global__ __launch_bounds__(256) void k_at_split(const AtArgs a, const int first) {
     constexpr int E = DP / 16;
     __shared__ int red[4];
     const int ten = first + blockIdx.y, hk = blockIdx.z;
     const int4 tile = a.tiles[blockIdx.x];
-    const int e = graph_exp<DP, VEC, SELF>(a, tile, ten, hk, red);
-    const int64_t at = ((int64_t)tile.x * a.Hk + hk) * 4;
-    const int ev = ten != TG ? 0 : first == TG ? a.exps[at + TV] : graph_exp<DP, VEC, SELF>(a, tile, TV, hk, red);
-    if (threadIdx.x == 0 && (int)blockIdx.x == tile.z) a.exps[at + ten] = e;
+    int e = NO_EXP;
+    for (int i = threadIdx.x; i < tile.w; i += 256) e = max(e, a.part[((int64_t)(tile.z + i) * 4 + ten) * a.Hk + hk]);
+    e = max_of_all(e, red);
+    if (e == NO_EXP) e = 0;
+    if (threadIdx.x == 0 && (int)blockIdx.x == tile.z) a.exps[((int64_t)tile.x * a.Hk + hk) * 4 + ten] = e;
     const int rows = min(64, (int)(a.ptr[tile.x + 1] - tile.y));
     const int per = (ten == TQ || ten == TG) ? a.R : 1, sub = threadIdx.x & 15;
-    const bool masked = a.mask && (ten == TK || ten == TV);
     for (int i = threadIdx.x >> 4; i < rows * per; i += 16) {
         const int r = i / per, h = hk * per + i - r * per;
         const int64_t n = tile.y + r;
         float v[E];
-        load_part<DP, VEC>(a.src[ten] + n * a.row_stride[ten] + h * a.head_stride[ten], sub, a.D, !(masked && !a.mask[n]), v);
-        if (ten == TG) over_sum<E>(a, n, h, v);
+        load_vec<DP, VEC>(a, ten, n, h, v);
         f16x2 hi[E / 2], lo[E / 2];
 #pragma unroll
         for (int j = 0; j < E; ++j) v[j] = ldexpf(v[j], 15 - e);
@@ -186,7 +171,7 @@ __global__ __launch_bounds__(256) void k_at_split(const AtArgs a, const int firs
                 if (sub * E + j < a.D) dot = fmaf(v[j], o[sub * E + j], dot);
 #pragma unroll
             for (int w = 1; w < 16; w <<= 1) dot += __shfl_xor(dot, w, 64);
-            if (sub == 0) a.delta[(int64_t)h * a.N + n] = ldexpf(dot, -2 - ev);
+            if (sub == 0) a.delta[(int64_t)h * a.N + n] = ldexpf(dot, -2);
         }
     }
 }
@@ -672,7 +657,7 @@ __global__ __launch_bounds__(64 * NW, at_bounds(DP, NW)) void k_at_dkv(const AtA
         sg.store(ldsG);
         if (threadIdx.x < 64) {
             ldsL[threadIdx.x] = -nl;
-            ldsD[threadIdx.x] = nd;
+            ldsD[threadIdx.x] = ldexpf(nd, -ex[TV]);
         }
         __syncthreads();
         if (step + 1 < steps) fetch(step + 1);
@@ -778,7 +763,7 @@ __global__ __launch_bounds__(64 * NW, at_bounds(DP, NW)) void k_at_dq(const AtAr
             go[b][k] = own_frag<DP>(a.img[TG] + (int64_t)h * a.N * (2 * DP), row, k, lane);
         }
         ls[b] = -a.stats[(int64_t)h * a.N + row].x;
-        de[b] = a.delta[(int64_t)h * a.N + row];
+        de[b] = ldexpf(a.delta[(int64_t)h * a.N + row], -ex[TV]);
     }
     f32x4 acc[DB][QB];
 #pragma unroll
@@ -898,12 +883,8 @@ void at_rows(AtArgs& a, int heads, F launch) {
 template <int DP, bool VEC>
 void at_images(const AtArgs& a, int first, int last, hipStream_t stream) {
     const dim3 grid((unsigned)a.n_tiles, (unsigned)(last - first + 1), (unsigned)a.Hk);
-    if (a.max_rows <= 256) {
-        hipLaunchKernelGGL((k_at_split<DP, VEC, true>), grid, dim3(256), 0, stream, a, first);
-    } else {
-        hipLaunchKernelGGL((k_at_norms<DP, VEC>), grid, dim3(256), 0, stream, a, first);
-        hipLaunchKernelGGL((k_at_split<DP, VEC, false>), grid, dim3(256), 0, stream, a, first);
-    }
+    hipLaunchKernelGGL((k_at_norms<DP, VEC>), grid, dim3(256), 0, stream, a, first);
+    hipLaunchKernelGGL((k_at_split<DP, VEC>), grid, dim3(256), 0, stream, a, first);
 }
 
 template <int DP>
