@@ -2603,7 +2603,7 @@ class _Linear8(torch.autograd.Function):
         if need[1]:
             gw, gb = _weight_grad8(g, Packed8(*kept, ctx.packed), need[2])
         elif need[2]:
-            gb = g.sum(0)
+            gb = _gemm_tn(g, g[:, :1], True)[1]                 # a frozen weight: the column sums of a product one column wide
         if need[0]:
             gx = _gemm_nt(g, ctx.image, None, None, w.size(1))
         return gx, gw, gb, None

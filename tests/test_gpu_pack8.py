@@ -206,3 +206,34 @@ def test_kept_form_ignores_what_lies_behind_the_last_column(k):
     q, scale = (t for t in y.grad_fn.saved_tensors if t.dtype in (torch.int8, torch.uint8))
     want = Fn.pack8(x.contiguous())
     assert torch.equal(q, want.q) and torch.equal(scale, want.scale)
+
+
+@pytest.mark.parametrize("n,m", [(1, 5), (700, 138), (70001, 33)])
+def test_bias_gradient_beside_a_frozen_weight(n, m):
+    """Only the bias (and the input) learn: nothing is packed, the bias gradient is the column sums, also in a captured pass."""
+    from hgvae_amd import functional as Fn
+    x, w, g = (torch.randn(*s, device=dev()) for s in ((n, 100), (m, 100), (n, m)))
+    b = torch.randn(m, device=dev(), requires_grad=True)
+
+    def step():
+        y = Fn.linear8(x, w, b)
+        assert len(y.grad_fn.saved_tensors) == 1
+        return torch.autograd.grad(y, b, g)[0]
+
+    # sums of n values: one rounding per partial sum, at most n / 16 of them on the longest chain of the kernel
+    want = g.double().sum(0)
+    bound = (n / 16 + 8) * U * g.double().abs().sum(0)
+    assert bool(((step().double() - want).abs() <= bound).all())
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for _ in range(3):
+        g.normal_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, step())
