@@ -250,6 +250,11 @@ def graph_of(edge_index, num_nodes: Optional[int] = None) -> Graph:
     return g
 
 
+def _not_captured() -> None:
+    if torch.cuda.is_current_stream_capturing():
+        raise _lib.HgvError("Segments copies between host and device: make it before the capture")
+
+
 class Segments:
     """Which rows of a batched matrix belong to which graph: the plan that the per-graph operators
     (:func:`~hgvae_amd.functional.group_norm_act`, :func:`~hgvae_amd.functional.graph_attention`) take.
@@ -272,6 +277,7 @@ class Segments:
             raise _lib.HgvError("hgvae_amd operators run on the GPU only (Segments needs a cuda device)")
         if self.device.index is None:
             self.device = torch.device("cuda", torch.cuda.current_device())
+        _not_captured()
         self.sizes = [int(s) for s in sizes]
         self.num_graphs, self.num_rows = len(self.sizes), int(sizes.sum())
         ptr = np.zeros(self.num_graphs + 1, dtype=np.int64)
@@ -332,6 +338,8 @@ class Segments:
         """From the first row of each graph and the end (``Batch.ptr``)."""
         if ptr.dim() != 1 or ptr.numel() < 1 or ptr.dtype not in (torch.int32, torch.int64):
             raise _lib.HgvError("Segments: ptr must be a 1-D integer tensor with at least one entry")
+        if ptr.is_cuda:
+            _not_captured()
         host = ptr.detach().cpu().numpy().astype(np.int64)
         if host[0] != 0:
             raise _lib.HgvError("Segments: ptr must start at 0")
@@ -342,6 +350,8 @@ class Segments:
         """From the graph number of each row (``Batch.batch``), which must not decrease."""
         if batch.dim() != 1 or batch.dtype not in (torch.int32, torch.int64):
             raise _lib.HgvError("Segments: batch must be a 1-D integer tensor")
+        if batch.is_cuda:
+            _not_captured()
         host = batch.detach().cpu().numpy().astype(np.int64)
         if host.size and (host[0] < 0 or (np.diff(host) < 0).any()):
             raise _lib.HgvError("Segments: the rows of a graph must be consecutive and graphs in order")

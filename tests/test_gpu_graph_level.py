@@ -284,3 +284,80 @@ def test_empty_batches_through_the_modules():
         out.sum().backward()
         assert x.grad.shape == (0, 24) and all(not bool(p.grad.any()) for p in level.parameters())
         level.zero_grad()
+
+
+def test_plans_are_made_before_a_capture():
+    """A batch vector or a new plan inside a capture is an error that leaves the capture usable."""
+    from hgvae_amd import Segments
+    from hgvae_amd import functional as Fn
+    from hgvae_amd._lib import HgvError
+    x = torch.randn(50, 12, device=dev())
+    batch = torch.zeros(50, dtype=torch.long, device=dev())
+    seg = Segments.from_sizes([50], dev())
+    want = Fn.group_norm_act(x, seg, 3)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for call in (lambda: Fn.group_norm_act(x, batch, 3), lambda: Segments.from_sizes([50], dev()), lambda: Segments.from_ptr(batch[:1])):
+            with pytest.raises(HgvError, match="before the capture"):
+                call()
+        out = Fn.group_norm_act(x, seg, 3)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("op", ["norm", "linear8", "attention"])
+def test_offsets_beyond_32_bits(op):
+    """Matrices of more than 2^31 elements: the last graph's rows give what they give by themselves (to rounding: the order of sums
+    follows the plan)."""
+    from hgvae_amd import Segments
+    from hgvae_amd import functional as Fn
+    rows, last = 16_000_000, 1000
+    if op == "norm":
+        x, g = torch.randn(rows, 140, device=dev()), torch.randn(last, 140, device=dev())
+        assert x.numel() > 2 ** 31
+        w = torch.randn(140, device=dev(), requires_grad=True)
+        seg = Segments.from_sizes([8000] * ((rows - last) // 8000) + [(rows - last) % 8000, last], dev())
+        xr = x.requires_grad_()
+        out = Fn.group_norm_act(xr, seg, 7, w, keep8=True)
+        tail = out[-last:].detach().clone()
+        full = torch.zeros_like(out)
+        full[-last:] = g
+        gx, gw = torch.autograd.grad(out, (xr, w), full)
+        small = x.detach()[-last:].clone().requires_grad_()
+        ref = Fn.group_norm_act(small, Segments.from_sizes([last], dev()), 7, w, keep8=True)
+        rx, rw = torch.autograd.grad(ref, (small, w), g)
+        pairs = ((tail, ref), (gx[-last:], rx), (gw, rw))
+    elif op == "linear8":
+        x = torch.randn(rows, 140, device=dev())
+        w = torch.randn(24, 140, device=dev(), requires_grad=True)
+        xr = x.requires_grad_()
+        out = Fn.linear8(xr, w)
+        tail = out[-last:].detach().clone()
+        full = torch.zeros_like(out)
+        full[-last:] = 1.0
+        gx, gw = torch.autograd.grad(out, (xr, w), full)
+        small = x.detach()[-last:].clone().requires_grad_()
+        ref = Fn.linear8(small, w)
+        rx, rw = torch.autograd.grad(ref, (small, w), torch.ones_like(ref))
+        pairs = ((tail, ref), (gx[-last:], rx), (gw, rw))
+    else:
+        rows, h, d = 9_000_000, 4, 64
+        q = torch.randn(rows, h, d, device=dev()).requires_grad_()
+        assert q.numel() > 2 ** 31
+        k, v = (torch.randn(rows, h, d, device=dev()).requires_grad_() for _ in range(2))
+        seg = Segments.from_sizes([100] * ((rows - last) // 100) + [last], dev())
+        out = Fn.graph_attention(q, k, v, seg)
+        tail = out[-last:].detach().clone()
+        g = torch.randn(last, h, d, device=dev())
+        full = torch.zeros_like(out)
+        full[-last:] = g
+        grads = torch.autograd.grad(out, (q, k, v), full)
+        small = [t.detach()[-last:].clone().requires_grad_() for t in (q, k, v)]
+        ref = Fn.graph_attention(*small, Segments.from_sizes([last], dev()))
+        refs = torch.autograd.grad(ref, small, g)
+        pairs = ((tail, ref), *((a[-last:], b) for a, b in zip(grads, refs)))
+    for a, b in pairs:
+        b = b.detach()
+        assert float((a.detach() - b).abs().max()) <= 1e-5 * float(b.abs().max())
+    torch.cuda.empty_cache()
