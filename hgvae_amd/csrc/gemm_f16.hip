@@ -1661,14 +1661,15 @@ __global__ __launch_bounds__(256) void k_row_range(const float* __restrict__ A1,
 }
 }  // namespace
 
+__global__ void k_clear_flag(int* flag) { *flag = 0; }
+
 extern "C" int hgv_row_range_flag(const float* A1, int64_t lda1, int K1, const float* A2, int64_t lda2, int K2, int64_t M,
                                   int log2_limit, int* flag, hipStream_t stream) {
     HGV_REQUIRE(M >= 0 && K1 > 0 && A1 && flag && log2_limit >= 1 && log2_limit <= 60, HGV_EINVAL, "row_range_flag: bad arguments");
     HGV_REQUIRE(hgv_aligned(A1, 16) && lda1 % 4 == 0 && lda1 >= (K1 + 3) / 4 * 4, HGV_EINVAL, "row_range_flag: bad/misaligned buffer (source 1)");
     if (A2) HGV_REQUIRE(K2 > 0 && hgv_aligned(A2, 16) && lda2 % 4 == 0 && lda2 >= (K2 + 3) / 4 * 4, HGV_EINVAL,
                         "row_range_flag: bad/misaligned buffer (source 2)");
-    hipError_t e = hipMemsetAsync(flag, 0, sizeof(int), stream);
-    HGV_REQUIRE(e == hipSuccess, HGV_ELAUNCH, "row_range_flag: memset failed: %s", hipGetErrorString(e));
+    hipLaunchKernelGGL(k_clear_flag, dim3(1), dim3(1), 0, stream, flag);      // a memset node has not cleared it on later replays of a graph
     if (M == 0) return HGV_OK;
     // whole 16-byte chunks are read: pad columns must be zero (they are ignored as zeros)
     hipLaunchKernelGGL(k_row_range, dim3((unsigned)hgv_cdiv(M * 16, 256)), dim3(256), 0, stream, A1, lda1, (K1 + 3) / 4,
