@@ -2471,15 +2471,15 @@ def _leaves_of(*inputs):
 def _first_order(backward):
     """Gradients that cannot be differentiated again: a second derivative through them raises (torch's own wrapper does this
     too; it is only entered when a graph of the gradients is being built).  A captured backward pass whose leaves are still
-    held by an eager graph of another stream is refused here, before any of its gradients leaves the capture's stream."""
+    held by an eager graph of the default stream, which cannot join a capture, is refused here, before any of its gradients
+    leaves the capture's stream.  (Other streams, such as that of a warm-up, join it and come back.)"""
     guarded = torch.autograd.function.once_differentiable(backward)
 
     @functools.wraps(backward)
     def run(ctx, g):
         if ctx.leaves and torch.cuda.is_current_stream_capturing():
-            here = _lib.stream()
-            if any(s.stream != here for s in ctx.leaves):
-                raise _lib.HgvError("a backward pass cannot be captured while a graph of the same parameters that was built on another "
+            if any(s.stream == 0 for s in ctx.leaves):
+                raise _lib.HgvError("a backward pass cannot be captured while a graph of the same parameters that was built on the default "
                                     "stream is alive: drop its outputs (losses, activations) before the capture")
         return guarded(ctx, g) if torch.is_grad_enabled() else backward(ctx, g)
     return run

@@ -361,3 +361,34 @@ def test_offsets_beyond_32_bits(op):
         b = b.detach()
         assert float((a.detach() - b).abs().max()) <= 1e-5 * float(b.abs().max())
     torch.cuda.empty_cache()
+
+
+def test_capture_after_a_warm_up_whose_results_live_on():
+    """The usual recipe: warm up on a side stream, keep the last loss, capture, replay."""
+    from hgvae_amd import Segments
+    torch.manual_seed(8)
+    level = Level(64, 8, 4, 2, False).to(dev())
+    seg = Segments.from_sizes([100, 40], dev())
+    static = torch.randn(140, 64, device=dev())
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            level.zero_grad(set_to_none=True)
+            loss = (level(static, seg) ** 2).mean()
+            loss.backward()
+    torch.cuda.current_stream().wait_stream(side)
+    level.zero_grad(set_to_none=True)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = (level(static, seg) ** 2).mean()
+        out.backward()
+    del loss
+    got = {n: p.grad for n, p in level.named_parameters()}
+    for _ in range(3):
+        static.normal_()
+        graph.replay()
+        torch.cuda.synchronize()
+        want = torch.autograd.grad((level(static, seg) ** 2).mean(), list(level.parameters()))
+        for (n, g), w in zip(got.items(), want):
+            assert float((g - w).abs().max()) <= 1e-6 * float(w.abs().max()), n

@@ -88,6 +88,12 @@ def test_captured_backward_is_refused_while_an_older_graph_holds_the_leaves(monk
     late = Twice.apply(w)
     state.update(stream=0)
     assert torch.autograd.grad(Twice.apply(w).sum() + late.sum(), w)[0].tolist() == [4.0] * 3
+    del late
+    state.update(stream=5)
+    warm = Twice.apply(w)                                        # a graph of a warm-up stream may live on
+    state.update(stream=7, capturing=True)
+    assert torch.autograd.grad(Twice.apply(w).sum(), w)[0].tolist() == [2.0] * 3
+    del warm
     assert Fn._leaves_of(torch.ones(2), w * 1) == []             # no leaf, or none that asks for a gradient
 
 
