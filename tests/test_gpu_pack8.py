@@ -133,6 +133,8 @@ def test_linear8_keeps_a_quarter():
 
 def test_linear8_captured_and_on_another_stream():
     from hgvae_amd import functional as Fn
+    if Fn._CHECK_PADS:
+        pytest.skip("HGVAE_CHECK_PADS synchronises")
     gen = torch.Generator(device=dev()).manual_seed(3)
     x, w, b, g = (torch.randn(*s, generator=gen, device=dev()) for s in ((4416, 138), (138, 138), (138,), (4416, 138)))
 

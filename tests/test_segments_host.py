@@ -141,3 +141,26 @@ def test_header_and_bindings_agree_on_the_number_of_arguments():
         assert found, name
         params = found.group(1).strip()
         assert (0 if params in ("", "void") else params.count(",") + 1) == len(args), name
+
+
+def test_c_abi_refusals_of_the_packing_forms():
+    from hgvae_amd import _lib
+    lib = _lib.load()
+    room = ctypes.create_string_buffer(8192)
+    at = (ctypes.addressof(room) + 255) // 256 * 256
+
+    def norm(q, ldq, scale, rows=16):
+        return lib.hgv_group_norm_fwd8(at, 16, 12, 3, 0, 1e-5, None, None, at, at, at, at, 2, 2, 0, 0, 0, 4, rows, q, ldq, scale, at, 16, at, at,
+                                       at, 16, None)
+
+    for bad in ((None, 16, at), (at, 16, None), (at, 12, at), (at, 48, at), (at + 4, 16, at)):
+        assert norm(*bad) == -1 and b"fwd8" in lib.hgv_last_error()
+    assert norm(at, 16, at, rows=0) == -1
+    assert norm(at, 16, at) == -4                                # ... and a good form reaches the check of the workspace
+
+    def product(q, ldq, scale, lda=100):
+        return lib.hgv_gemm_nt16h_keep8(at, lda, 100, at, None, 4, 40, at, 40, q, ldq, scale, None)
+
+    for bad in ((None, 112, at), (at, 112, None), (at, 100, at), (at, 144, at), (at + 8, 112, at)):
+        assert product(*bad) == -1 and b"keep8" in lib.hgv_last_error()
+    assert product(at, 112, at, lda=98) == -1 and b"source 1" in lib.hgv_last_error()
