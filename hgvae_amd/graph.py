@@ -370,7 +370,16 @@ class Segments:
         plan = self._norm_plans.get((columns, groups))
         if plan is None:
             lib = _lib.load()
-            n, listed = bisect.bisect_right(self._sorted, lib.hgv_group_norm_small_rows(columns, groups)), len(self._sorted)
+            limit = lib.hgv_group_norm_small_rows(columns, groups)
+            per = columns // groups
+            slab = per * max(1, -(-32 // per))                  # the columns that a workgroup takes
+            if slab < columns and slab % 32 and 4 * self.num_rows * columns > 64 << 20:
+                # one read of a whole graph per workgroup saves launches and passes.  Where memory is what counts and its pieces of rows
+                # are not whole lines, long graphs run faster in chunks (forward and backward, one read / chunks; 138 columns in slabs
+                # of 46: 2 048 graphs of 300 rows 819 / 617 us, 2 500 of 200 rows 676 / 572, 2 048 of 138 rows 340 / 335, 128 of 300
+                # rows 54 / 62;  256 columns in slabs of 32: 2 500 of 200 rows 778 / 1 049, 1 500 of 340 rows 920 / 948)
+                limit = min(limit, 160)
+            n, listed = bisect.bisect_right(self._sorted, limit), len(self._sorted)
             if n < listed and 8 * sum(self._sorted[:n]) < self.num_rows:
                 n = 0                   # a few small graphs beside large ones: not worth a launch of their own
             chunks = (self._first_host[n], self._first_host[-1])

@@ -378,3 +378,9 @@ def test_kept_input_is_its_8bit_form(sizes, c, groups):
         assert torch.equal(kept[0][:, :c], want.q[:, :c]) and torch.equal(kept[1], want.scale)
         assert torch.equal(Fn.group_norm_act(x, seg, groups).isnan(), out.isnan())
         assert torch.equal(Fn.group_norm_act(x, seg, groups).nan_to_num(), out.detach().nan_to_num())
+
+
+@pytest.mark.parametrize("c,groups", [(138, 6), (256, 8)])
+def test_many_graphs_of_both_kinds(c, groups):
+    """More than 64 MB of graphs of 100 and 300 rows: some read at once, some in chunks, whatever the rule picks."""
+    test_group_norm_act_matches_float64([300] * 250 + [100] * 450 + [1, 0, 161, 160], c, groups, "silu", True)
