@@ -17,7 +17,7 @@
 // reaches 5.2.  Taking the graphs in batches of 48 ... 192 MB, so that the second read meets the memory-side cache, was measured and
 // is slower (forward and backward 1.78 ... 1.37 ms against 1.23 in one piece): the ends of the many short launches cost more than the
 // cache brings.  Streaming loads in the last pass: 160 001 x 256 3 % faster, 1.28 M x 138 (rows that share lines) 1 % slower, not taken.
-// Small graphs (32 x 138 rows x 138): forward 9.4 us, backward 10.5 + 2.8, where the host takes 140.
+// Small graphs (32 x 138 rows x 138): forward 9.4 us, backward 10.5 + 2.8, where the host takes 138.
 #include "pack8.h"
 
 namespace {

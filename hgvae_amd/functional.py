@@ -2696,22 +2696,29 @@ class _GroupNormAct(torch.autograd.Function):
         n, c = x.shape
         dev = x.device
         out = new_padded(n, c, dev, zero_pad=False)
-        mean = torch.empty(seg.num_graphs, groups, dtype=torch.float64, device=dev)
-        rstd = torch.empty(seg.num_graphs, groups, dtype=torch.float32, device=dev)
         arrays, counts, nws, _ = seg._norm_plan(c, groups)
-        ws = torch.empty(nws, dtype=torch.uint8, device=dev)
+        # the statistics, [mean fp64 | rstd fp32] per (graph, group), and a small workspace in one buffer
+        at = seg.num_graphs * groups
+        own = (at + (at + 1) // 2 + 31) // 32 * 32
+        small = nws <= 1 << 16
+        stats = torch.empty(own + (nws // 8 if small else 0), dtype=torch.float64, device=dev)
+        mean = stats.data_ptr()
+        rstd, work = mean + 8 * at, mean + 8 * own
+        if not small:
+            ws = torch.empty(nws, dtype=torch.uint8, device=dev)
+            work = ws.data_ptr()
         head = (x.data_ptr(), ld_of(x), c, groups, act, eps, _lib.ptr(w), _lib.ptr(b), *arrays, *counts)
-        tail = (out.data_ptr(), out.stride(0), mean.data_ptr(), rstd.data_ptr(), ws.data_ptr(), nws, _lib.stream())
+        tail = (out.data_ptr(), out.stride(0), mean, rstd, work, nws, _lib.stream())
         ctx.seg, ctx.cfg = seg, (groups, act)
         ctx.packed = None
         if keep8 and train and any(ctx.needs_input_grad[:3]):
             p = _empty8(n, c, dev)
             _lib.call("hgv_group_norm_fwd8", *head, n, p.q.data_ptr(), p.q.stride(0), p.scale.data_ptr(), *tail)
             ctx.packed = p.shape
-            ctx.save_for_backward(w, b, mean, rstd, p.q, p.scale)
+            ctx.save_for_backward(w, b, stats, p.q, p.scale)
         else:
             _lib.call("hgv_group_norm_fwd", *head, *tail)
-            ctx.save_for_backward(w, b, mean, rstd, x)
+            ctx.save_for_backward(w, b, stats, x)
         return out
 
     @staticmethod
@@ -2722,7 +2729,7 @@ class _GroupNormAct(torch.autograd.Function):
     @staticmethod
     def _grads(ctx, g):
         seg, (groups, act) = ctx.seg, ctx.cfg
-        w, b, mean, rstd, *kept = ctx.saved_tensors
+        w, b, stats, *kept = ctx.saved_tensors
         need = ctx.needs_input_grad
         g = rowmajor(g)
         n, c = g.shape
@@ -2737,7 +2744,7 @@ class _GroupNormAct(torch.autograd.Function):
         else:
             source = (None, 0, kept[0].data_ptr(), kept[0].stride(0), kept[1].data_ptr())
         _lib.call("hgv_group_norm_bwd", g.data_ptr(), ld_of(g), *source, c, groups, act, _lib.ptr(w), _lib.ptr(b), *arrays, *counts,
-                  mean.data_ptr(), rstd.data_ptr(), _lib.ptr(gx), gx.stride(0) if gx is not None else 0, _lib.ptr(gw), _lib.ptr(gb),
+                  stats.data_ptr(), stats.data_ptr() + 8 * seg.num_graphs * groups, _lib.ptr(gx), gx.stride(0) if gx is not None else 0, _lib.ptr(gw), _lib.ptr(gb),
                   ws.data_ptr(), nws, _lib.stream())
         return gx, gw, gb, None, None, None, None, None, None
 
