@@ -12,7 +12,8 @@
 // transposing loads.  Graphs of few rows are taken from the operands as they are, larger ones from images of the pieces that a pass
 // of its own leaves.  Kept for the backward pass: the output and two numbers per row and head (the exponent that is subtracted and the
 // inverse of the sum that is left; +inf and 0 for a row without keys).  Backward: probabilities are recomputed, once by key tiles
-// (dk, dv) and once by query tiles (dq): no atomics, the same bits every time.  A masked key's rows of k and v are taken as zeros, whatever they hold.
+// (dk, dv) and once by query tiles (dq): no atomics, the same bits every time.  A query with one key has the probability 1 whatever its
+// logit is: dq and dk are then zero by definition, which two roundings of dP and of its mean would not give.  A masked key's rows of k and v are taken as zeros, whatever they hold.
 #include "common.h"
 
 namespace {
@@ -42,6 +43,8 @@ struct AtArgs {
     int max_rows;                                               // of the largest graph
     int* part;                                                  // [tile][4][Hk] exponents of the longest row
     int* exps;                                                  // [B][Hk][4]
+    int* live;                                                  // [tile] keys that take part (backward pass)
+    int* keys;                                                  // [B] keys that take part: none, one, or 2 for more
     _Float16* img[4];                                           // [heads][N][hi DP | lo DP]
     float* out;                                                 // [N, H, D]
     float2* stats;                                              // [H, N] of a row: whole M with sum_j 2^(logit_j - M) in [1, 2), and 1 / that sum
@@ -125,6 +128,11 @@ __global__ __launch_bounds__(256) void k_at_norms(const AtArgs a, const int firs
     }
     best = max_of_all(best, red);
     if (threadIdx.x == 0) a.part[((int64_t)blockIdx.x * 4 + ten) * a.Hk + hk] = best;
+    if (a.live && ten == TK && hk == 0 && threadIdx.x < 64) {   // the first wave, whole
+        const int i = threadIdx.x;
+        const uint64_t takes = __ballot(i < rows && (!a.mask || a.mask[tile.y + i]));
+        if (i == 0) a.live[blockIdx.x] = __popcll(takes);
+    }
 }
 
 // One workgroup per (tile, tensor, key head) splits its rows with the exponent of the graph.  The gradient's also takes the dot products
@@ -142,6 +150,16 @@ __global__ __launch_bounds__(256) void k_at_split(const AtArgs a, const int firs
     e = max_of_all(e, red);
     if (e == NO_EXP) e = 0;
     if (threadIdx.x == 0 && (int)blockIdx.x == tile.z) a.exps[((int64_t)tile.x * a.Hk + hk) * 4 + ten] = e;
+    if (a.live && ten == TK && hk == 0 && (int)blockIdx.x == tile.z) {                  // the same for the whole workgroup
+        int tiles = 0, most = 0;                                // that hold keys, and the keys of one of them
+        for (int i = threadIdx.x; i < tile.w; i += 256) {
+            const int n = a.live[tile.z + i];
+            tiles += n > 0; most = max(most, n);
+        }
+        const bool many = __syncthreads_or(tiles > 1 || most > 1);
+        const int holders = __syncthreads_count(tiles > 0);     // with not many: threads that saw one tile with one key
+        if (threadIdx.x == 0) a.keys[tile.x] = many ? 2 : min(holders, 2);
+    }
     const int rows = min(64, (int)(a.ptr[tile.x + 1] - tile.y));
     const int per = (ten == TQ || ten == TG) ? a.R : 1, sub = threadIdx.x & 15;
     for (int i = threadIdx.x >> 4; i < rows * per; i += 16) {
@@ -717,7 +735,7 @@ __global__ __launch_bounds__(64 * NW, at_bounds(DP, NW)) void k_at_dkv(const AtA
     for (int b = 0; b < KB; ++b) {
         const int64_t row = key0 + 16 * b + (lane & 15);
         if (row >= g1) continue;
-        const bool live = !a.mask || a.mask[row];
+        const bool live = !a.mask || a.mask[row], many = a.keys[t.x] > 1;
         float* pk = row_out(a.dk, row, a.Hk, hk, a.D);
         float* pv = row_out(a.dv, row, a.Hk, hk, a.D);
         const int ek = ex[TG] + ex[TV] + ex[TQ] - 28, ev = ex[TG] - 29;
@@ -726,7 +744,7 @@ __global__ __launch_bounds__(64 * NW, at_bounds(DP, NW)) void k_at_dkv(const AtA
             f32x4 x, y;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                x[i] = live ? ldexpf(dk[d][b][i] * a.scale, ek) : 0.f;
+                x[i] = live && many ? ldexpf(dk[d][b][i] * a.scale, ek) : 0.f;
                 y[i] = live ? ldexpf(dv[d][b][i], ev) : 0.f;
             }
             store4(pk, 16 * d + 4 * g, a.D, x);
@@ -750,6 +768,16 @@ __global__ __launch_bounds__(64 * NW, at_bounds(DP, NW)) void k_at_dq(const AtAr
     const int4 t = a.blocks[blk];
     const int64_t k0 = a.ptr[t.x], k1 = a.ptr[t.x + 1];
     const int64_t q0 = (int64_t)t.y + 16 * QB * wave;
+    if (a.keys[t.x] < 2) {                                      // the same for the whole workgroup
+#pragma unroll
+        for (int b = 0; b < QB; ++b) {
+            const int64_t row = q0 + 16 * b + (lane & 15);
+            if (row >= k1) continue;
+#pragma unroll
+            for (int d = 0; d < DB; ++d) store4(row_out(a.dq, row, a.H, h, a.D), 16 * d + 4 * g, a.D, f32x4{0.f, 0.f, 0.f, 0.f});
+        }
+        return;
+    }
     const int* ex = a.exps + ((int64_t)t.x * a.Hk + hk) * 4;
     const float c = fold_scale(a.scale, ex[TQ] + ex[TK] - 30);
     Frag q[QB][KC], go[QB][KC];
@@ -856,17 +884,19 @@ __global__ __launch_bounds__(64 * NW, at_bounds(DP, NW)) void k_at_dq(const AtAr
 // ---- host side ----------------------------------------------------------------------------------------------------------------
 int at_dp(int D) { return (D + 31) / 32 * 32; }
 
-struct AtSizes { size_t part, exps, img[4], delta, total; };
+struct AtSizes { size_t part, exps, live, keys, img[4], delta, total; };
 AtSizes at_sizes(int64_t N, int H, int Hk, int D, int64_t n_tiles, int64_t graphs, bool backward) {
     AtSizes s;
     const size_t row = (size_t)at_dp(D) * 4;
     s.part = hgv_align256((size_t)n_tiles * 4 * Hk * sizeof(int));
     s.exps = hgv_align256((size_t)graphs * Hk * 4 * sizeof(int));
+    s.live = backward ? hgv_align256((size_t)n_tiles * sizeof(int)) : 0;
+    s.keys = backward ? hgv_align256((size_t)graphs * sizeof(int)) : 0;
     s.img[TQ] = hgv_align256((size_t)N * H * row);
     s.img[TK] = s.img[TV] = hgv_align256((size_t)N * Hk * row);
     s.img[TG] = backward ? s.img[TQ] : 0;
     s.delta = backward ? hgv_align256((size_t)N * H * sizeof(float)) : 0;
-    s.total = s.part + s.exps + s.img[0] + s.img[1] + s.img[2] + s.img[3] + s.delta;
+    s.total = s.part + s.exps + s.live + s.keys + s.img[0] + s.img[1] + s.img[2] + s.img[3] + s.delta;
     return s;
 }
 
@@ -959,6 +989,10 @@ int at_fill(AtArgs& a, const char* what, int64_t N, int num_graphs, int H, int H
     char* p = (char*)ws;
     a.part = (int*)p; p += s.part;
     a.exps = (int*)p; p += s.exps;
+    if (backward) {
+        a.live = (int*)p; p += s.live;
+        a.keys = (int*)p; p += s.keys;
+    }
     for (int i = 0; i < 4; ++i) { a.img[i] = (_Float16*)p; p += s.img[i]; }
     a.delta = (float*)p;
     return HGV_OK;
