@@ -148,11 +148,6 @@ def prepare(case, seed):
     def normal(*shape, scale=1.0):
         return torch.randn(*shape, generator=gen, device=dev) * scale
 
-    def rows16(t):                    # rows padded to 16 bytes with zeros, the layout of the matrices that the levels hand on
-        buf = torch.zeros(t.size(0), (t.size(1) + 3) // 4 * 4, device=dev)
-        buf[:, :t.size(1)] = t
-        return buf[:, :t.size(1)]
-
     op, n = case["op"], _rows(case)
     st = {"case": case}
     if op in ("norm", "attention"):
@@ -164,18 +159,18 @@ def prepare(case, seed):
     if op == "norm":
         c = case["channels"]
         # pre-activations of a projection: every column with an offset and a spread of its own
-        st["x"] = rows16(normal(n, c).mul_(torch.rand(c, generator=gen, device=dev) + 0.5).add_(normal(c, scale=0.5)))
+        st["x"] = normal(n, c).mul_(torch.rand(c, generator=gen, device=dev) + 0.5).add_(normal(c, scale=0.5))
         st["weight"], st["bias"] = torch.rand(c, generator=gen, device=dev) + 0.5, normal(c, scale=0.3)
         if case["train"]:
-            st["g"] = rows16(normal(n, c, scale=1e-2))
+            st["g"] = normal(n, c, scale=1e-2)
     elif op == "pack":
-        st["x"] = rows16(normal(n, case["columns"]) * (torch.rand(case["columns"], generator=gen, device=dev) + 0.1))
+        st["x"] = normal(n, case["columns"]) * (torch.rand(case["columns"], generator=gen, device=dev) + 0.1)
     elif op == "linear8":
         k, m = case["columns"], case["outputs"]
         # activations behind a smooth rectifier: mostly small, some large
-        st["x"] = rows16(torch.nn.functional.silu(normal(n, k)))
+        st["x"] = torch.nn.functional.silu(normal(n, k))
         st["weight"], st["bias"] = normal(m, k, scale=1.0 / math.sqrt(k)), normal(m, scale=0.1)
-        st["g"] = rows16(normal(n, m, scale=1e-2))
+        st["g"] = normal(n, m, scale=1e-2)
     else:
         h, hk, d = case["heads"], case["kv_heads"], case["width"]
         st["q"], st["k"], st["v"] = normal(n, h, d, scale=1.5), normal(n, hk, d), normal(n, hk, d)
@@ -289,7 +284,7 @@ def _plain_norm(st):
     def rows_of(t):                                     # [graphs, groups] -> [n, groups, 1]
         return t.float()[batch].unsqueeze(-1)
 
-    xg = x.reshape(n, grp, per)
+    xg = x.view(n, grp, per)
     mean = rows_of(group_mean(xg))
     d = xg - mean
     rstd = rows_of(torch.rsqrt(group_mean(d * d) + 1e-5))
@@ -300,7 +295,7 @@ def _plain_norm(st):
     if case["keep8"]:
         d = _plain_values8(x).view(n, grp, per) - mean
     xh = d * rstd
-    dz = st["g"].reshape(n, grp, per) * _act(xh * w + bias, case["act"])[1]
+    dz = st["g"].view(n, grp, per) * _act(xh * w + bias, case["act"])[1]
     gw, gb = (dz * xh).sum(0, dtype=torch.float64).reshape(c).float(), dz.sum(0, dtype=torch.float64).reshape(c).float()
     dxh = dz * w
     gx = rstd * (dxh - rows_of(group_mean(dxh)) - xh * rows_of(group_mean(dxh * xh)))
@@ -400,7 +395,7 @@ def _exact_norm(st):
         if s == 0:
             continue
         x = st["x"][at:at + s].double()
-        cols = x.reshape(s, grp, per).transpose(0, 1).reshape(grp, s * per)
+        cols = x.view(s, grp, per).transpose(0, 1).reshape(grp, s * per)
         var, mean = torch.var_mean(cols, dim=1, correction=0)
         sd = torch.sqrt(var + 1e-5).repeat_interleave(per)
         mean = mean.repeat_interleave(per)
