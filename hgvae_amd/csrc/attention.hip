@@ -41,6 +41,7 @@ struct AtArgs {
     float neg;                                                  // -1, unknown to the compiler: keeps x - (float)half one instruction (v_fma_mix_f32)
 
     int max_rows;                                               // of the largest graph
+    bool wide_g;                                                // rows of do can be read in 16 bytes (backward pass)
     int* part;                                                  // [tile][4][Hk] exponents of the longest row
     int* exps;                                                  // [B][Hk][4]
     int* live;                                                  // [tile] keys that take part (backward pass)
@@ -96,6 +97,9 @@ __device__ __forceinline__ void load_vec(const AtArgs& a, int ten, int64_t n, in
     if (ten == TG) over_sum<DP / 16>(a, n, h, v);
 }
 
+// e with |row| < 2^e, from the square of the norm
+__device__ __forceinline__ int above_norm(double square) { return ((((int)(__double_as_longlong(square) >> 52) & 2047) - 1023) >> 1) + 1; }
+
 // The largest of the workgroup's values.  red: four ints of LDS.
 __device__ __forceinline__ int max_of_all(int v, int* red) {
 #pragma unroll
@@ -123,8 +127,7 @@ __global__ __launch_bounds__(256) void k_at_norms(const AtArgs a, const int firs
         for (int e = 0; e < DP / 16; ++e) s = fma((double)v[e], (double)v[e], s);
 #pragma unroll
         for (int o = 1; o < 16; o <<= 1) s += __shfl_xor(s, o, 64);
-        const int e2 = (int)((__double_as_longlong(s) >> 52) & 2047) - 1023;
-        if (s > 0.0 && s < 1e300) best = max(best, (e2 >> 1) + 1);      // rows that hold an infinity or NaN do not count
+        if (s > 0.0 && s < 1e300) best = max(best, above_norm(s));      // rows that hold an infinity or NaN do not count
     }
     best = max_of_all(best, red);
     if (threadIdx.x == 0) a.part[((int64_t)blockIdx.x * 4 + ten) * a.Hk + hk] = best;
@@ -757,6 +760,11 @@ __global__ __launch_bounds__(64 * NW, at_bounds(DP, NW)) void k_at_dkv(const AtA
 // A workgroup owns 16 * QB * NW queries of one head and walks the keys as the forward pass does; two products in, one out; the same
 // graphs 2.9 ... 3.0 ms (1.25 PFLOP/s).  One kernel for dq, dk and dv would save two of the seven products but has to add dq over key
 // tiles, by atomics whose order changes results, or through memory.
+//
+// The incoming gradient comes from the operand itself and not from its image: each query's row has a power of two of its own, by the
+// row's own norm, up to the split of the logits' gradient.  With the scale of the longest row, a row F times shorter reached that split
+// log2 F bits lower, behind probabilities of 1 / n already (one row of 5 000 with 16 384 times the others' gradient, the others' dq by row:
+// 1.6e-3 from 64 bits; so 2e-6, the formulas in fp32 2.5e-6).
 template <int DP, int QB, int NW>
 __global__ __launch_bounds__(64 * NW, at_bounds(DP, NW)) void k_at_dq(const AtArgs a) {
     constexpr int KC = DP / 32, DB = DP / 16;
@@ -782,16 +790,37 @@ __global__ __launch_bounds__(64 * NW, at_bounds(DP, NW)) void k_at_dq(const AtAr
     const float c = fold_scale(a.scale, ex[TQ] + ex[TK] - 30);
     Frag q[QB][KC], go[QB][KC];
     float ls[QB], de[QB];
+    int eg[QB];                                                 // exponent of the row's own scale
 #pragma unroll
     for (int b = 0; b < QB; ++b) {
         const int64_t row = min(q0 + 16 * b + (lane & 15), k1 - 1);
+        const float2 st = a.stats[(int64_t)h * a.N + row];
+        const float* p = a.src[TG] + row * a.row_stride[TG] + h * a.head_stride[TG];
+        f32x4 x[KC][2];
+        double sum = 0.0;
+#pragma unroll
+        for (int k = 0; k < KC; ++k)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int d = 32 * k + 8 * g + 4 * i;
+                x[k][i] = a.wide_g ? four<true>(p, d, a.D, true) : four<false>(p, d, a.D, true);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) { x[k][i][j] *= st.y; sum = fma((double)x[k][i][j], (double)x[k][i][j], sum); }
+            }
+        sum += __shfl_xor(sum, 16, 64);
+        sum += __shfl_xor(sum, 32, 64);
+        eg[b] = sum > 0.0 && sum < 1e300 ? above_norm(sum) : ex[TG];
 #pragma unroll
         for (int k = 0; k < KC; ++k) {
             q[b][k] = own_frag<DP>(a.img[TQ] + (int64_t)h * a.N * (2 * DP), row, k, lane);
-            go[b][k] = own_frag<DP>(a.img[TG] + (int64_t)h * a.N * (2 * DP), row, k, lane);
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x[k][i][j] = ldexpf(x[k][i][j], 15 - eg[b]);
+            go[b][k] = split_frag<true>(x[k][0], x[k][1], a.neg);
         }
-        ls[b] = -a.stats[(int64_t)h * a.N + row].x;
-        de[b] = ldexpf(a.delta[(int64_t)h * a.N + row], -ex[TV]);
+        ls[b] = -st.x;
+        de[b] = ldexpf(a.delta[(int64_t)h * a.N + row], ex[TG] - eg[b] - ex[TV]);
     }
     f32x4 acc[DB][QB];
 #pragma unroll
@@ -870,7 +899,7 @@ __global__ __launch_bounds__(64 * NW, at_bounds(DP, NW)) void k_at_dq(const AtAr
         const int64_t row = q0 + 16 * b + (lane & 15);
         if (row >= k1) continue;
         float* o = row_out(a.dq, row, a.H, h, a.D);
-        const int e = ex[TG] + ex[TV] + ex[TK] - 28;
+        const int e = eg[b] + ex[TV] + ex[TK] - 28;
 #pragma unroll
         for (int d = 0; d < DB; ++d) {
             f32x4 x;
@@ -922,6 +951,7 @@ int at_launch(AtArgs a, bool backward, hipStream_t stream) {
     bool vec = a.D == DP;
     for (int i = 0; i < (backward ? 4 : 3); ++i)
         vec = vec && hgv_aligned(a.src[i], 16) && a.row_stride[i] % 4 == 0 && a.head_stride[i] % 4 == 0;
+    a.wide_g = vec;
     // Without images where no graph is large: what splitting every operand once per workgroup costs stays below a pass of its own over
     // memory (four heads of 64, with and without: 32 graphs of 138 nodes 15 and 26 us, 2 000 of 250 0.70 and 1.74 ms, 200 of 512 0.26
     // and 0.37, 100 of 1 000 0.43 and 0.51, 16 of 5 000 1.44 and 1.29; six heads of 23: 200 of 512 0.24 and 0.26, 100 of 1 000 0.39

@@ -51,3 +51,31 @@ def test_gradients_through_a_single_key_are_zero(h, hk, d, sizes, keys):
             assert bool(((dv[live[0]].double() - parts.sum((0, 2))).abs() <= bound).all())
         elif live.numel() > 1:
             assert bool(dq[rows].any()) and bool(dk[live].any())
+
+
+@pytest.mark.parametrize("n,h,hk,d", [(300, 2, 1, 23), (300, 1, 1, 64), (5000, 1, 1, 64), (5000, 2, 2, 40), (2600, 1, 1, 128)])
+@pytest.mark.parametrize("factor", [2.0 ** 10, 2.0 ** 14, 2.0 ** 20])
+def test_dq_of_ordinary_rows_beside_one_with_a_large_gradient(n, h, hk, d, factor):
+    """dq of a row depends on that row's gradient alone, and is as exact as if the others' were of its size."""
+    q, k, v, g = make(n, h, hk, d, seed=n + d)
+    g[n // 3] *= factor
+    dq = run(q, k, v, [n], g)[1].double()
+    scale = d ** -0.5
+    for head in range(h):
+        Q, K, V, G = (t[:, i].double() for t, i in ((q, head), (k, head * hk // h), (v, head * hk // h), (g, head)))
+        P = torch.softmax(scale * Q @ K.t().contiguous(), 1)
+        dP = G @ V.t().contiguous()
+        D = (P * dP).sum(1, keepdim=True)
+        want = scale * (P * (dP - D)) @ K
+        # relative to sum_j p_j (|dP_j| + |D|) |k_j|: logits of about 25 at most from 22-bit pieces and fp32 (their errors times the
+        # probability), dP and D likewise, a split of the sum's terms, sums of n terms a fourth at a time;  and the two floors
+        # 2^-39 of the pieces against the row's and the graph's own norms
+        terms = scale * (P * (dP.abs() + D.abs())) @ K.abs()
+        norms = G.norm(dim=1, keepdim=True) * V.norm(dim=1).max() * K.norm(dim=1).max() * scale
+        logit = scale * (Q.norm(dim=1) * K.norm(dim=1).max()).max()
+        bound = terms * (logit * 2.0 ** -20 + 2.0 ** -20 + n / 4 * U) + norms * 2.0 ** -34 * n ** 0.5
+        err = (dq[:, head] - want).abs()
+        assert bool((err <= bound).all()), f"{float((err / bound).max()):.3g} bounds"
+        # by row: pieces of 22 bits in q, k, v and g, and fp32 sums
+        off = (dq[:, head] - want).norm(dim=1) / want.norm(dim=1)
+        assert float(off.max()) <= 2.0 ** -15, float(off.max())
