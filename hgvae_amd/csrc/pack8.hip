@@ -131,11 +131,15 @@ extern "C" int hgv_unpack8(const int8_t* q, int64_t ldq, const uint8_t* scale, i
 // bf16 pieces of G (8 bits each, cut: together all 24) make the product exact up to its fp32 accumulation: three piece products
 // where two fp32 operands take six.
 //
+// The matrix cores' sums are cut downwards, whatever their sign: over 1.28 M rows whose terms cancel that alone is 1.3e-6 of the result, and
+// 4e-6 of the column sums of a gradient with a mean.  So a tile's sum starts from zero, every other tile holds -G and is subtracted, which
+// leaves as many cuts upwards, and tiles are added in fp32 by eight and then to a second sum: 1e-7, for 5 % of the kernel's time.
+//
 // A workgroup takes 144 x 144 outputs over every sets-th tile of 32 rows: G is split and V widened on the way into LDS (row-major,
 // 288 bytes per row, which spreads the eight rows of a transposing load over all banks), two buffers.  Wave w of nine owns columns
 // 16 w .. of G and all columns of V; the column sums are a product with a tile of ones.  Six more waves load and split, so that this
 // runs beside the products.  Partial sums are added in fp64 in a fixed order by k_tn8_reduce.
-// 1.28 M rows, 138 x 138: 219 us = 4.1 TB/s (nine waves that split and multiply in turn 260, with four movers 227; the six-product
+// 1.28 M rows, 138 x 138: 237 us = 3.8 TB/s (one sum in the matrix cores 224;  before that, nine waves that split and multiply in turn 260, with four movers 227; the six-product
 // kernel over the unpacked matrix 400, and 165 for unpacking).  Three or four tiles in flight instead of two: 241 and 235.
 namespace {
 
@@ -181,15 +185,16 @@ __global__ __launch_bounds__(T8_THREADS) void k_gemm_tn8(const Tn8Args a) {
     // a tile of ones behind the two buffers, for the column sums
     for (int i = t; i < T8_ROWS * 4; i += T8_THREADS) *(uint2*)(t8_lds + 2 * T8_BUF + i * 8) = make_uint2(0x3f803f80u, 0x3f803f80u);
     if (wave < 9) {
-        f32x4 acc[9], accb = {0.f, 0.f, 0.f, 0.f};
+        f32x4 acc[9], accb = {0.f, 0.f, 0.f, 0.f}, sum[9], sumb = {0.f, 0.f, 0.f, 0.f};       // of up to eight tiles; of all before them
 #pragma unroll
-        for (int k = 0; k < 9; ++k) acc[k] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int k = 0; k < 9; ++k) acc[k] = sum[k] = f32x4{0.f, 0.f, 0.f, 0.f};
         const int i16 = lane & 15;
         const int at = (4 * (lane >> 4) + (i16 >> 2)) * T8_LINE + (i16 & 3) * 8;
         __syncthreads();
         for (int64_t it = 0; it < intervals; ++it) {
             if (it < mine && wave < nt) {
                 const unsigned char* base = t8_lds + (it & 1) * T8_BUF + at;
+                const float sign = (it & 1) ? -1.f : 1.f;
                 bf16x8 gf[3];
 #pragma unroll
                 for (int j = 0; j < 3; ++j) gf[j] = t8_read(base + j * T8_PIECE + wave * 32);
@@ -197,14 +202,25 @@ __global__ __launch_bounds__(T8_THREADS) void k_gemm_tn8(const Tn8Args a) {
                 for (int k = 0; k < 9; ++k)
                     if (k < kt) {
                         const bf16x8 v = t8_read(base + 3 * T8_PIECE + k * 32);
+                        f32x4 t = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                        for (int j = 2; j >= 0; --j) acc[k] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(gf[j], v, acc[k], 0, 0, 0);
+                        for (int j = 2; j >= 0; --j) t = __builtin_amdgcn_mfma_f32_16x16x32_bf16(gf[j], v, t, 0, 0, 0);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) acc[k][i] = fmaf(t[i], sign, acc[k][i]);
                     }
                 if (kg == 0) {
                     const bf16x8 ones = t8_read(t8_lds + 2 * T8_BUF + (4 * (lane >> 4) + (i16 >> 2)) * 32 + (i16 & 3) * 8, 32);
+                    f32x4 t = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int j = 2; j >= 0; --j) accb = __builtin_amdgcn_mfma_f32_16x16x32_bf16(gf[j], ones, accb, 0, 0, 0);
+                    for (int j = 2; j >= 0; --j) t = __builtin_amdgcn_mfma_f32_16x16x32_bf16(gf[j], ones, t, 0, 0, 0);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) accb[i] = fmaf(t[i], sign, accb[i]);
                 }
+            }
+            if ((it & 7) == 7) {
+#pragma unroll
+                for (int k = 0; k < 9; ++k) { sum[k] += acc[k]; acc[k] = f32x4{0.f, 0.f, 0.f, 0.f}; }
+                sumb += accb; accb = f32x4{0.f, 0.f, 0.f, 0.f};
             }
             __syncthreads();
         }
@@ -212,8 +228,8 @@ __global__ __launch_bounds__(T8_THREADS) void k_gemm_tn8(const Tn8Args a) {
             float* out = a.partial + ((int64_t)grp * a.sets + set) * T8_SET + lane * 4;
 #pragma unroll
             for (int k = 0; k < 9; ++k)
-                if (k < kt) *(f32x4*)(out + (wave * 9 + k) * 256) = acc[k];
-            if (kg == 0) *(f32x4*)(out + (81 + wave) * 256) = accb;
+                if (k < kt) *(f32x4*)(out + (wave * 9 + k) * 256) = sum[k] + acc[k];
+            if (kg == 0) *(f32x4*)(out + (81 + wave) * 256) = sumb + accb;
         }
     } else {
         // quads m, m + 384, m + 768 of the tile's 32 x 36.  One offset per quad; what depends on the tile is uniform; quads outside the
@@ -261,7 +277,7 @@ __global__ __launch_bounds__(T8_THREADS) void k_gemm_tn8(const Tn8Args a) {
                 uint32_t p[3][4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const float x = gi ? g[S][i][e] : 0.f;
+                    const float x = gi ? (S ? -g[S][i][e] : g[S][i][e]) : 0.f;
                     p[0][e] = __float_as_uint(x);
                     const float r = x - __uint_as_float(p[0][e] & 0xffff0000u);              // exact
                     p[1][e] = __float_as_uint(r);
