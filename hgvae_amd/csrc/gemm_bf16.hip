@@ -195,12 +195,12 @@ __device__ __forceinline__ void nt16_body(const Nt16Args& a, unsigned char* lds_
         }
         for (int e = t; e < g.chunks * 4; e += blockDim.x) {
             const int blk = e;                                     // chunk * 4 + kq
-            int second = 0, col = 0; int64_t ld = a.lda1;
+            int second = 0, col = 0;
             if (blk < g.nb1) { col = 8 * blk; }
-            else if (blk < g.nb1 + g.nb2) { second = 1; col = 8 * (blk - g.nb1); ld = a.lda2; }
+            else if (blk < g.nb1 + g.nb2) { second = 1; col = 8 * (blk - g.nb1); }
             else { col = 0; }                                      // padding block: weights are zero there
-            // both 16-byte halves stay inside the row's leading dimension (columns past K meet zero weights)
-            const int c0 = (int)min((int64_t)col, ld - 4), c1 = (int)min((int64_t)col + 4, ld - 4);
+            // both 16-byte halves stay inside the row's own quads: a slice's rows may end the buffer (columns past K meet zero weights)
+            const int quad = ((second ? g.K2 : g.K1) + 3) / 4 * 4 - 4, c0 = min(col, quad), c1 = min(col + 4, quad);
             tab[e] = make_int4(c0 * 4, c1 * 4, second, 0);
         }
         for (int e = t; e < NT * 16; e += blockDim.x) {
@@ -414,10 +414,10 @@ __global__ __launch_bounds__(768) void k_gemm_nt16s(const Nt16Args a) {
     int4* tab = reinterpret_cast<int4*>(lds_raw + 2 * CHUNK_BYTES);
     float* bias_s = reinterpret_cast<float*>(lds_raw + 2 * CHUNK_BYTES + (size_t)g.chunks * 64);
     for (int e = t; e < g.chunks * 4; e += 768) {
-        int second = 0, col = 0; int64_t ld = a.lda1;
+        int second = 0, col = 0;
         if (e < g.nb1) { col = 8 * e; }
-        else if (e < g.nb1 + g.nb2) { second = 1; col = 8 * (e - g.nb1); ld = a.lda2; }
-        const int c0 = (int)min((int64_t)col, ld - 4), c1 = (int)min((int64_t)col + 4, ld - 4);
+        else if (e < g.nb1 + g.nb2) { second = 1; col = 8 * (e - g.nb1); }
+        const int quad = ((second ? g.K2 : g.K1) + 3) / 4 * 4 - 4, c0 = min(col, quad), c1 = min(col + 4, quad);
         tab[e] = make_int4(c0 * 4, c1 * 4, second, 0);
     }
     for (int e = t; e < ROWS; e += 768) bias_s[e] = (a.bias && e < g.N) ? a.bias[e] : 0.f;

@@ -304,11 +304,11 @@ __device__ __forceinline__ void nth_body(const NtHArgs& a, unsigned char* lds_ra
                 if (e0 + u * (int)blockDim.x < npieces) dst[e0 + u * (int)blockDim.x] = v[u];
         }
         for (int e = t; e < g.chunks * 4; e += blockDim.x) {
-            int second = 0, col = 0; int64_t ld = a.lda1;
+            int second = 0, col = 0;
             if (e < g.nb1) { col = 8 * e; }
-            else if (e < g.nb1 + g.nb2) { second = 1; col = 8 * (e - g.nb1); ld = a.lda2; }
-            // both 16-byte halves stay inside the row's leading dimension (columns past K meet zero weights)
-            const int c0 = (int)min((int64_t)col, ld - 4), c1 = (int)min((int64_t)col + 4, ld - 4);
+            else if (e < g.nb1 + g.nb2) { second = 1; col = 8 * (e - g.nb1); }
+            // both 16-byte halves stay inside the row's own quads: a slice's rows may end the buffer (columns past K meet zero weights)
+            const int quad = ((second ? g.K2 : g.K1) + 3) / 4 * 4 - 4, c0 = min(col, quad), c1 = min(col + 4, quad);
             tab[e] = make_int4(c0 * 4, c1 * 4, second, 0);
         }
         const float* invw = reinterpret_cast<const float*>(reinterpret_cast<const unsigned char*>(a.Wp) + (size_t)g.parts * img);
@@ -590,10 +590,10 @@ __global__ __launch_bounds__(768) void k_gemm_nt16hs(const NtHArgs a) {
     float* bias_s = reinterpret_cast<float*>(lds_raw + 2 * CHUNK_BYTES + (size_t)g.chunks * 64);
     float* invw_s = bias_s + ROWS;
     for (int e = t; e < g.chunks * 4; e += 768) {
-        int second = 0, col = 0; int64_t ld = a.lda1;
+        int second = 0, col = 0;
         if (e < g.nb1) { col = 8 * e; }
-        else if (e < g.nb1 + g.nb2) { second = 1; col = 8 * (e - g.nb1); ld = a.lda2; }
-        const int c0 = (int)min((int64_t)col, ld - 4), c1 = (int)min((int64_t)col + 4, ld - 4);
+        else if (e < g.nb1 + g.nb2) { second = 1; col = 8 * (e - g.nb1); }
+        const int quad = ((second ? g.K2 : g.K1) + 3) / 4 * 4 - 4, c0 = min(col, quad), c1 = min(col + 4, quad);
         tab[e] = make_int4(c0 * 4, c1 * 4, second, 0);
     }
     {
