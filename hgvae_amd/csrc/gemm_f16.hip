@@ -205,6 +205,9 @@ struct NtHArgs {
     float* C2; const uint32_t* act_bits2; float* stat_partial2;
     // ACT = 6: plain store, and the 8-bit form of A1 (its values are in the movers' registers anyway): q and the byte per block of 32
     int8_t* keep_q; int64_t keep_ldq; uint8_t* keep_scale;
+    // one source whose rows may be followed by anything within their leading dimension: columns from K1 on are taken as zeros.  (Their
+    // weights are zeros, but they would enter the row's scale, and 0 * inf is not 0.)  ACT = 6, 7 and the CUT kernels
+    int cut;
 };
 
 template <int CTRL> __device__ __forceinline__ float dpp_mov(float x) {
@@ -276,7 +279,15 @@ __device__ __forceinline__ SplitH split8h(const f32x4 (&av)[2], float s) {
     return o;
 }
 
-template <int NT, int RING, int ACT = 0>
+// columns 32 c + 8 kq ... + 7 of a row of K columns
+__device__ __forceinline__ void cut_row(f32x4 (&v)[2], int K, int c, int kq) {
+    const int left = K - 32 * c - 8 * kq;
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        if (e >= left) v[e >> 2][e & 3] = 0.f;
+}
+
+template <int NT, int RING, int ACT = 0, bool CUT = false>
 __device__ __forceinline__ void nth_body(const NtHArgs& a, unsigned char* lds_raw, const int part, const int wg_rank, const int wgs) {
     const GeoH& g = a.g;
     const int t = threadIdx.x, lane = t & 63, i = lane & 15, kq = lane >> 4;
@@ -435,7 +446,8 @@ __device__ __forceinline__ void nth_body(const NtHArgs& a, unsigned char* lds_ra
     SplitH cur;
     float s_cur = 1.f, inv_cur = 1.f;          // scale of the lane's row in the tile being accumulated
     if (my_tiles > 0) {
-        const f32x4 av0[2] = {ring[0][0], ring[0][1]};
+        f32x4 av0[2] = {ring[0][0], ring[0][1]};
+        if (CUT) cut_row(av0, g.K1, 0, kq);
         s_cur = scale_for(row_amax(av0), inv_cur);
         cur = split8h(av0, s_cur);
 #pragma unroll
@@ -446,7 +458,8 @@ __device__ __forceinline__ void nth_body(const NtHArgs& a, unsigned char* lds_ra
         for (int d = 0; d < RING; ++d) {
             issue(d);
             if (u0 + d < S) {
-                const f32x4 av_next[2] = {ring[(d + 1) % RING][0], ring[(d + 1) % RING][1]};
+                f32x4 av_next[2] = {ring[(d + 1) % RING][0], ring[(d + 1) % RING][1]};
+                if (CUT) cut_row(av_next, g.K1, cq + 1 == steps ? 0 : cq + 1, kq);
                 // scale of the next step: a new tile starts from its first chunk; inside a tile the scale only ever
                 // goes down, when the chunk would leave the fp16 range with the current one
                 const bool fresh = cq + 1 == steps;
@@ -559,26 +572,26 @@ __device__ __forceinline__ void nth_body(const NtHArgs& a, unsigned char* lds_ra
     }
 }
 
-template <int NT, int ACT = 0>
+template <int NT, int ACT = 0, bool CUT = false>
 __global__ __launch_bounds__(64 * nth_waves<NT>()) void k_gemm_nt16h(const NtHArgs a, const int part) {
     extern __shared__ __attribute__((aligned(16))) unsigned char lds_raw[];
     HGV_GATE_EXIT(a);
-    nth_body<NT, nth_ring<NT>(), ACT>(a, lds_raw, part, blockIdx.x, gridDim.x);
+    nth_body<NT, nth_ring<NT>(), ACT, CUT>(a, lds_raw, part, blockIdx.x, gridDim.x);
 }
 
-template <int NT0, int NT1>
+template <int NT0, int NT1, bool CUT = false>
 __global__ __launch_bounds__(64 * nth_waves<NT0>()) void k_gemm_nt16h_pair(const NtHArgs a) {
     extern __shared__ __attribute__((aligned(16))) unsigned char lds_raw[];
     HGV_GATE_EXIT(a);
-    if ((int)blockIdx.x < a.wgs0) nth_body<NT0, nth_ring<NT0>()>(a, lds_raw, 0, blockIdx.x, a.wgs0);
-    else nth_body<NT1, nth_ring<NT1>()>(a, lds_raw, 1, (int)blockIdx.x - a.wgs0, (int)gridDim.x - a.wgs0);
+    if ((int)blockIdx.x < a.wgs0) nth_body<NT0, nth_ring<NT0>(), 0, CUT>(a, lds_raw, 0, blockIdx.x, a.wgs0);
+    else nth_body<NT1, nth_ring<NT1>(), 0, CUT>(a, lds_raw, 1, (int)blockIdx.x - a.wgs0, (int)gridDim.x - a.wgs0);
 }
 
 // ------------------------------------------------------------------------------------------
 // Weights whose image does not fit in LDS (hidden width 256): 12 waves own one row tile each and all NT n tiles of
 // it; the 32-wide k chunks of the image are copied by all threads into one of two LDS buffers while the waves
 // multiply from the other (one barrier per chunk).  The scale of a row is fixed per row block the same way as above.
-template <int NT>
+template <int NT, bool CUT = false>
 __global__ __launch_bounds__(768) void k_gemm_nt16hs(const NtHArgs a) {
     extern __shared__ __attribute__((aligned(16))) unsigned char lds_raw[];
     HGV_GATE_EXIT(a);
@@ -641,6 +654,7 @@ __global__ __launch_bounds__(768) void k_gemm_nt16hs(const NtHArgs a) {
         for (int c = 0; c < chunks; ++c) {
             const int cn = c + 1 < chunks ? c + 1 : 0;
             w_load(cn);
+            if (CUT) cut_row(a_nx, g.K1, c, kq);
             {
                 const float amax = row_amax(a_nx);
                 const bool grow = amax * s_cur > 32768.f;
@@ -767,8 +781,8 @@ __global__ __launch_bounds__(MAXT) void k_gemm_nt16r(const NtHArgs a) {
     // loads are counted ones) and hand them over here: a load inside the multipliers' loop made every interval wait for the
     // completion of the store in front of it
     uint32_t* kbits = reinterpret_cast<uint32_t*>(rowinv + 2 * R);
-    constexpr bool BWD = ACT == 3 || ACT == 4, KEEP = ACT == 1 || ACT == 2 || ACT == 5, PAIR = ACT == 5, P8 = ACT == 6;
-    static_assert(!P8 || NSRC == 1, "one source is kept");
+    constexpr bool BWD = ACT == 3 || ACT == 4, KEEP = ACT == 1 || ACT == 2 || ACT == 5, PAIR = ACT == 5, P8 = ACT == 6, CUT = P8 || ACT == 7;
+    static_assert(!CUT || (NSRC == 1 && CHUNKS >= 4 && EPT == 3), "one source is kept or cut; its last quad of columns is one of 24 ... 35");
     constexpr int KW = 16;                                           // words per row in the ring: 8 per draw
     // ACT = 3: the rows of d that belong to the last four blocks of output, [4][R][NTR_LDC], handed over by the movers likewise
     float* dring = reinterpret_cast<float*>(kbits + 4 * R * KW);
@@ -947,6 +961,7 @@ __global__ __launch_bounds__(MAXT) void k_gemm_nt16r(const NtHArgs a) {
         const int tl = t - mwaves * 64, mr = tl >> 4, mj = P8 ? tl & 15 : min(tl & 15, 11);
         int qoff[EPT], soff[EPT];                     // P8: byte offsets of this lane's words and blocks from the block's first row
         int qlive[EPT];                               // ... and how many of a word's four columns there are (the others are zeros)
+        int flive[EPT];                               // CUT: how many of the loaded quad's four columns
         int eoff[NSRC][EPT], ewr[NSRC][EPT];          // element offset (floats) from the block's first row; byte offset of its h halves in a stage buffer
 #pragma unroll
         for (int sidx = 0; sidx < NSRC; ++sidx) {
@@ -962,6 +977,7 @@ __global__ __launch_bounds__(MAXT) void k_gemm_nt16r(const NtHArgs a) {
                     qlive[u] = g.K1 - 4 * word;
                     f = min(word, nf4 - 1);
                 }
+                flive[u] = g.K1 - 4 * f;
                 eoff[sidx][u] = mr * (int)(sidx ? a.lda2 : a.lda1) + 4 * f;
                 const int kc = (sidx ? 8 * g.nb1 : 0) + 4 * f;            // column of the concatenation
                 const int c = kc >> 5, c4 = (kc >> 2) & 7;          // piece c4 >> 1 of the chunk (its columns 8 q ... 8 q + 7), half c4 & 1
@@ -1033,6 +1049,13 @@ __global__ __launch_bounds__(MAXT) void k_gemm_nt16r(const NtHArgs a) {
                     for (int u = 0; u < EPT; ++u) asm volatile("" : "+v"(aadd[S][u]));
                 }
             } else if (KEEP) asm volatile("" : "+v"(kb[S]));
+            if (CUT) {                                // quads 0 ... 23 are whole
+#pragma unroll
+                for (int u = P8 ? 1 : 2; u < EPT; ++u)
+#pragma unroll
+                    for (int e = 1; e < 4; ++e)
+                        if (e >= flive[u]) raw[S][0][u][e] = 0.f;
+            }
             float m = 0.f;
 #pragma unroll
             for (int sidx = 0; sidx < NSRC; ++sidx)
@@ -1187,7 +1210,7 @@ void nth_grid(int64_t ntiles, int64_t* wpb_out, int64_t* blocks_out) {
 
 template <int NT, int ACT = 0>
 int launch_nth(const NtHArgs& a, int part, size_t lds, hipStream_t st) {
-    auto kern = k_gemm_nt16h<NT, ACT>;
+    auto kern = ACT == 0 && a.cut ? k_gemm_nt16h<NT, 0, true> : k_gemm_nt16h<NT, ACT>;
     const int rc = raise_lds_h(kern);
     if (rc != HGV_OK) return rc;
     int64_t wpb, blocks;
@@ -1284,6 +1307,7 @@ int launch_ntr(const NtHArgs& a, const NtrPlan& p, hipStream_t st) {
         if (a.A2) return stats ? launch_ntr_k<9, 2, 2>(a, p, st) : launch_ntr_k<9, 2, 1>(a, p, st);
         return stats ? launch_ntr_k<5, 1, 2>(a, p, st) : launch_ntr_k<5, 1, 1>(a, p, st);
     }
+    if (a.cut && !p.wide && a.g.K1 % 4) return a.g.chunks == 4 ? launch_ntr_k<4, 1, 7>(a, p, st) : launch_ntr_k<5, 1, 7>(a, p, st);
     if (p.wide) return a.A2 ? launch_ntr_k<16, 2, 0, 6, 768>(a, p, st) : launch_ntr_k<8, 1, 0, 6, 768>(a, p, st);
     if (a.A2) {
         switch (a.g.chunks) {
@@ -1300,7 +1324,7 @@ int launch_ntr(const NtHArgs& a, const NtrPlan& p, hipStream_t st) {
 
 template <int NT>
 int launch_nths_nt(const NtHArgs& a, hipStream_t st) {
-    auto kern = k_gemm_nt16hs<NT>;
+    auto kern = a.cut ? k_gemm_nt16hs<NT, true> : k_gemm_nt16hs<NT>;
     const int rc = raise_lds_h(kern);
     if (rc != HGV_OK) return rc;
     const size_t lds = (size_t)2 * 2 * NT * 1024 + side_bytes_h(a.g.chunks, NT);
@@ -1327,7 +1351,7 @@ int launch_nths(const NtHArgs& a, hipStream_t st) {
 // bf16 kernel: the cost of a row tile grows slowly with the part's width).
 template <int NT0, int NT1>
 int launch_nth_pair(NtHArgs a, size_t lds, hipStream_t st) {
-    auto kern = k_gemm_nt16h_pair<NT0, NT1>;
+    auto kern = a.cut ? k_gemm_nt16h_pair<NT0, NT1, true> : k_gemm_nt16h_pair<NT0, NT1>;
     const int rc = raise_lds_h(kern);
     if (rc != HGV_OK) return rc;
     const int cus = cu_count_h();
@@ -1446,7 +1470,7 @@ static int gemm_nt16h_any(const float* A1, int64_t lda1, int K1, const float* A2
                           const float* bias, int64_t M, int N, float* C, int64_t ldc, const int* gate, int gate_run_if,
                           hipStream_t stream, const uint32_t* act_bits = nullptr, int64_t act_ldb = 0, int act_relu = 0,
                           float act_scale = 1.f, float* stat_partial = nullptr, const NtHBwd* bwd = nullptr, const NtHPair* pair = nullptr,
-                          const NtHKeep* keep = nullptr) {
+                          const NtHKeep* keep = nullptr, bool cut = false) {
     HGV_REQUIRE(M >= 0 && N > 0 && K1 > 0, HGV_EINVAL, "gemm_nt16h: bad sizes");
     if (M == 0) return HGV_OK;
     NtHArgs a{};
@@ -1484,6 +1508,7 @@ static int gemm_nt16h_any(const float* A1, int64_t lda1, int K1, const float* A2
             a.bwd_add = bwd->add; a.bwd_ldadd = bwd->ldadd;
         }
     }
+    a.cut = cut && K1 % 8;                     // blocks of 8 columns are read whole
     if (keep) {
         if (ntr_keep_shape(a.g, plan)) {
             a.keep_q = keep->q; a.keep_ldq = keep->ldq; a.keep_scale = keep->scale;
@@ -1517,13 +1542,19 @@ extern "C" int hgv_gemm_nt16h(const float* A1, int64_t lda1, int K1, const float
 }
 
 // hgv_gemm_nt16h of one source that also leaves the source's 8-bit form (hgv_pack8): from the same launch where the kernel with the
-// weights in registers runs unsplit (97 ... 144 columns, 33 ... 144 outputs), else by a pass of its own.
+// weights in registers runs unsplit (97 ... 144 columns, 33 ... 144 outputs), else by a pass of its own.  The rows may be followed by anything.
 extern "C" int hgv_gemm_nt16h_keep8(const float* A, int64_t lda, int K, const void* Wp, const float* bias, int64_t M, int N, float* C,
                                     int64_t ldc, int8_t* q, int64_t ldq, uint8_t* scale, hipStream_t stream) {
     HGV_REQUIRE(K > 0 && q && scale && ldq >= K && ldq % 16 == 0 && ldq <= 32 * (int64_t)((K + 31) / 32) && hgv_aligned(q, 16), HGV_EINVAL,
                 "gemm_nt16h_keep8: null / misaligned buffer or bad leading dimension");
     const NtHKeep keep{q, ldq, scale};
-    return gemm_nt16h_any(A, lda, K, nullptr, 0, 0, Wp, bias, M, N, C, ldc, nullptr, 0, stream, nullptr, 0, 0, 1.f, nullptr, nullptr, nullptr, &keep);
+    return gemm_nt16h_any(A, lda, K, nullptr, 0, 0, Wp, bias, M, N, C, ldc, nullptr, 0, stream, nullptr, 0, 0, 1.f, nullptr, nullptr, nullptr, &keep, true);
+}
+
+// hgv_gemm_nt16h of one source whose rows may be followed by anything
+extern "C" int hgv_gemm_nt16h_cut(const float* A, int64_t lda, int K, const void* Wp, const float* bias, int64_t M, int N, float* C,
+                                  int64_t ldc, hipStream_t stream) {
+    return gemm_nt16h_any(A, lda, K, nullptr, 0, 0, Wp, bias, M, N, C, ldc, nullptr, 0, stream, nullptr, 0, 0, 1.f, nullptr, nullptr, nullptr, nullptr, true);
 }
 
 // 1 when hgv_gemm_nt16h_act can run this shape

@@ -2555,13 +2555,33 @@ def _pack8(x: torch.Tensor) -> Packed8:
     return p
 
 
-def _own_rows(t: torch.Tensor) -> torch.Tensor:
-    """``as_padded``, but a column slice of a wider matrix is copied where its rows' last 16 bytes hold foreign columns."""
+def _rows16(t: torch.Tensor) -> torch.Tensor:
+    """``as_padded``; rows so far apart that sixteen of them pass 31 bits are copied too."""
     p = as_padded(t)
-    if p is t and t.size(1) % 4 and ld_of(t) > pad4(t.size(1)):
+    if ld_of(p) > 1 << 26:
         p = new_padded(t.size(0), t.size(1), t.device)
         p.copy_(t)
     return p
+
+
+def _clean_rows(t: torch.Tensor) -> torch.Tensor:
+    """``_rows16``, but a matrix whose rows are followed by columns that may be another's is copied."""
+    p = _rows16(t)
+    if p is t and ld_of(t) > t.size(1):
+        p = new_padded(t.size(0), t.size(1), t.device)
+        p.copy_(t)
+    return p
+
+
+def _product8(x: torch.Tensor, img: "_Image", bias, n_out: int) -> torch.Tensor:
+    """x W^T + bias where nobody controls what lies behind the last column of x: a slice of a wider matrix, or the gradient that
+    the backward pass of a concatenation hands on."""
+    if img.kind != "f16x3" or _probe is not None:
+        return _gemm_nt(_clean_rows(x), img, None, bias, n_out)
+    y = new_padded(x.size(0), n_out, x.device, zero_pad=False)
+    _lib.call("hgv_gemm_nt16h_cut", x.data_ptr(), ld_of(x), x.size(1), img.a.data_ptr(), _lib.ptr(bias), x.size(0), n_out, y.data_ptr(),
+              ld_of(y), _lib.stream())
+    return y
 
 
 class _Piece:
@@ -2612,20 +2632,20 @@ class _Linear8(torch.autograd.Function):
     def forward(ctx, x, w, bias, train):
         need = ctx.needs_input_grad if train else (False, False, False)      # a parameter asks for its gradient under no_grad too
         ctx.leaves = _leaves_of(x, w, bias) if train else ()
-        x = _own_rows(x)
+        x = _rows16(x)
         fwd, ctx.image = _image_pair(w, need[0])
         ctx.packed = None
         if not need[1]:
             ctx.save_for_backward(w)
-            return _gemm_nt(x, fwd, None, bias, w.size(0))
-        if fwd.kind == "f16x3" and _probe is None and not _CHECK_PADS:
+            return _product8(x, fwd, bias, w.size(0))
+        if fwd.kind == "f16x3" and _probe is None:
             n, k = x.shape
             y = new_padded(n, w.size(0), x.device, zero_pad=False)
             p = _empty8(n, k, x.device)
             _lib.call("hgv_gemm_nt16h_keep8", x.data_ptr(), ld_of(x), k, fwd.a.data_ptr(), _lib.ptr(bias), n, w.size(0), y.data_ptr(), ld_of(y),
                       p.q.data_ptr(), p.q.stride(0), p.scale.data_ptr(), _lib.stream())
         else:
-            y, p = _gemm_nt(x, fwd, None, bias, w.size(0)), _pack8(x)
+            y, p = _product8(x, fwd, bias, w.size(0)), _pack8(x)
         ctx.packed = p.shape
         ctx.save_for_backward(w, p.q, p.scale)
         return y
@@ -2640,13 +2660,14 @@ class _Linear8(torch.autograd.Function):
         need = ctx.needs_input_grad
         w, *kept = ctx.saved_tensors
         gx = gw = gb = None
-        g = _own_rows(g)
+        g = _rows16(g)
         if need[1]:
             gw, gb = _weight_grad8(g, Packed8(*kept, ctx.packed), need[2])
         elif need[2]:
-            gb = _gemm_tn(g, g[:, :1], True)[1]                 # a frozen weight: the column sums of a product one column wide
+            c = _clean_rows(g) if _tn_f16 else g                # (that kernel scales by its whole operand)
+            gb = _gemm_tn(c, c[:, :1], True)[1]                 # a frozen weight: the column sums of a product one column wide
         if need[0]:
-            gx = _gemm_nt(g, ctx.image, None, None, w.size(1))
+            gx = _product8(g, ctx.image, None, w.size(1))
         return gx, gw, gb, None
 
 
@@ -2666,8 +2687,8 @@ def linear8(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = Non
     """``x @ w.T + bias`` with fp32 results, as :func:`dual_linear`, that keeps ``x`` in 8 bits (:func:`pack8`) for the
     backward pass: a quarter of the memory.  The gradients with respect to ``x`` and ``bias`` are those of the exact
     product; the weight gradient is ``g.T @ v`` with ``v`` the 8-bit values of ``x``.  Gradients cannot be differentiated
-    again.  As for every projection, a matrix whose rows are ``K`` rounded up to a multiple of 4 apart holds zeros behind its
-    last column, as all matrices of this package do; other layouts are copied."""
+    again.  ``x`` may be a slice of a wider matrix, whatever that holds beside it; rows that are not a multiple of 16 bytes
+    apart are copied."""
     x = plain(x)
     _check_matrix("x", x)
     _check_matrix("w", w, x.device, x.size(1))

@@ -578,10 +578,12 @@ size_t hgv_gemm_tn8_ws(int64_t M, int N, int K);
 int hgv_gemm_tn8(const float* G, int64_t ldg, int N, const int8_t* q, int64_t ldq, const uint8_t* scale, int K, int64_t M, float* GW,
                  int64_t ldgw, float* gbias, void* ws, size_t ws_bytes, hgv_stream_t stream);
 
-/* The projection that leaves its input in 8 bits: C = A W^T (+ bias) as hgv_gemm_nt16h (Wp: hgv_pack16h_weights_multi, one source;
- * pad columns of A are zero) and (q, scale) = hgv_pack8 of A. */
+/* The projection that leaves its input in 8 bits: C = A W^T (+ bias) as hgv_gemm_nt16h (Wp: hgv_pack16h_weights_multi, one source)
+ * and (q, scale) = hgv_pack8 of A;  and the projection alone.  Columns of A from K on, within lda, may hold anything. */
 int hgv_gemm_nt16h_keep8(const float* A, int64_t lda, int K, const void* Wp, const float* bias, int64_t M, int N, float* C, int64_t ldc,
                          int8_t* q, int64_t ldq, uint8_t* scale, hgv_stream_t stream);
+int hgv_gemm_nt16h_cut(const float* A, int64_t lda, int K, const void* Wp, const float* bias, int64_t M, int N, float* C, int64_t ldc,
+                       hgv_stream_t stream);
 
 /* ---- group norm with an activation over the rows of each graph, channels last (no reference counterpart: its levels
  *      normalise over the whole batch, nn.BatchNorm1d at gvae/gvae_skipcon.py:63) --------------------------------------
