@@ -2556,20 +2556,22 @@ def _pack8(x: torch.Tensor) -> Packed8:
 
 
 def _rows16(t: torch.Tensor) -> torch.Tensor:
-    """``as_padded``; rows so far apart that sixteen of them pass 31 bits are copied too."""
-    p = as_padded(t)
-    if ld_of(p) > 1 << 26:
-        p = new_padded(t.size(0), t.size(1), t.device)
-        p.copy_(t)
+    """Rows that start at multiples of 16 bytes, a copy where they do not (or are so far apart that sixteen of them pass 31 bits).
+    What the copy's rows hold behind the last column is left open."""
+    if (t.size(1) <= 1 or t.stride(1) == 1) and (t.size(0) <= 1 or t.size(1) <= t.stride(0) <= 1 << 26) and is_vec4(t):
+        return t
+    p = new_padded(t.size(0), t.size(1), t.device, zero_pad=False)
+    p.copy_(t)
     return p
 
 
 def _clean_rows(t: torch.Tensor) -> torch.Tensor:
-    """``_rows16``, but a matrix whose rows are followed by columns that may be another's is copied."""
-    p = _rows16(t)
-    if p is t and ld_of(t) > t.size(1):
-        p = new_padded(t.size(0), t.size(1), t.device)
-        p.copy_(t)
+    """``_rows16``, with zeros behind the last column."""
+    t = _rows16(t)
+    if ld_of(t) == t.size(1):
+        return t
+    p = new_padded(t.size(0), t.size(1), t.device)
+    p.copy_(t)
     return p
 
 
