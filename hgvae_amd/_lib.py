@@ -145,6 +145,7 @@ SIGNATURES = {
     "hgv_mse_fwd_grad": (C.c_int, [_vp, _i64, _vp, _i64, _i64, _i32, _vp, _vp, _i64, _vp, _sz, _vp]),
     "hgv_mse_bwd_unless_unit": (C.c_int, [_vp, _i64, _vp, _i64, _i64, _i32, _vp, _vp, _i64, _vp]),
     "hgv_graph_attention_ws": (_sz, [_i64, _i32, _i32, _i32, _i32, _i64, _i32]),
+    "hgv_graph_attention_fwd_ws": (_sz, [_i64, _i32, _i32, _i32, _i32, _i64, _i32]),
     "hgv_graph_attention_fwd": (C.c_int, [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _i32, _i32, _i32, _i32, _f32, _vp, _vp,
                                           _i32, _vp, _i32, _vp, _i32, _i32, _vp, _vp, _vp, _sz, _vp]),
     "hgv_graph_attention_bwd": (C.c_int, [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _i32, _i32,

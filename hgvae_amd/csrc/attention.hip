@@ -913,6 +913,9 @@ __global__ __launch_bounds__(64 * NW, at_bounds(DP, NW)) void k_at_dq(const AtAr
 // ---- host side ----------------------------------------------------------------------------------------------------------------
 int at_dp(int D) { return (D + 31) / 32 * 32; }
 
+constexpr int SMALL_ROWS = 512;                                 // forward: no images where no graph is larger
+bool at_no_images(bool backward, int max_rows) { return !backward && max_rows <= SMALL_ROWS; }
+
 struct AtSizes { size_t part, exps, live, keys, img[4], delta, total; };
 AtSizes at_sizes(int64_t N, int H, int Hk, int D, int64_t n_tiles, int64_t graphs, bool backward) {
     AtSizes s;
@@ -956,7 +959,7 @@ int at_launch(AtArgs a, bool backward, hipStream_t stream) {
     // memory (four heads of 64, with and without: 32 graphs of 138 nodes 15 and 26 us, 2 000 of 250 0.70 and 1.74 ms, 200 of 512 0.26
     // and 0.37, 100 of 1 000 0.43 and 0.51, 16 of 5 000 1.44 and 1.29; six heads of 23: 200 of 512 0.24 and 0.26, 100 of 1 000 0.39
     // and 0.35).
-    if (!backward && a.max_rows <= 512) {
+    if (at_no_images(backward, a.max_rows)) {
         constexpr int QB = DP <= 64 ? 2 : 1;
         at_rows(a, a.H, [&](int i, dim3 grid) {
             if (i && vec) hipLaunchKernelGGL((k_at_fwd_small<DP, QB, 8 / QB, true>), grid, dim3(512 / QB), 0, stream, a);
@@ -1010,12 +1013,14 @@ int at_fill(AtArgs& a, const char* what, int64_t N, int num_graphs, int H, int H
     HGV_REQUIRE(ptr && tiles && blocks && n_tiles > 0 && n64 > 0 && n128 > 0 && max_rows > 0, HGV_EINVAL, "%s: null plan", what);
     HGV_REQUIRE((int64_t)n64 * H <= 0x3fffffff, HGV_EUNSUPPORTED, "%s: too many tiles", what);
     const AtSizes s = at_sizes(N, H, Hk, D, n_tiles, num_graphs, backward);
-    HGV_REQUIRE(ws && ws_bytes >= s.total && hgv_aligned(ws, 256), HGV_EWORKSPACE, "%s: workspace too small or misaligned", what);
+    const size_t need = at_no_images(backward, max_rows) ? 256 : s.total;
+    HGV_REQUIRE(ws && ws_bytes >= need && hgv_aligned(ws, 256), HGV_EWORKSPACE, "%s: workspace too small or misaligned", what);
     a.neg = -1.f;
     a.N = N; a.H = H; a.Hk = Hk; a.R = H / Hk; a.D = D; a.scale = scale; a.mask = mask; a.ptr = ptr;
     a.tiles = (const int4*)tiles; a.n_tiles = n_tiles; a.max_rows = max_rows;
     a.n_blocks[0] = n64; a.n_blocks[1] = n128;
     a.block_list[0] = (const int4*)blocks; a.block_list[1] = a.block_list[0] + n64;
+    if (at_no_images(backward, max_rows)) return HGV_OK;
     char* p = (char*)ws;
     a.part = (int*)p; p += s.part;
     a.exps = (int*)p; p += s.exps;
@@ -1033,6 +1038,11 @@ int at_fill(AtArgs& a, const char* what, int64_t N, int num_graphs, int H, int H
 extern "C" size_t hgv_graph_attention_ws(int64_t N, int num_graphs, int H, int Hk, int D, int64_t n_tiles, int backward) {
     if (N <= 0 || num_graphs <= 0 || H <= 0 || Hk <= 0 || D <= 0 || n_tiles <= 0) return 0;
     return at_sizes(N, H, Hk, D, n_tiles, num_graphs, backward != 0).total;
+}
+
+extern "C" size_t hgv_graph_attention_fwd_ws(int64_t N, int num_graphs, int H, int Hk, int D, int64_t n_tiles, int max_rows) {
+    const size_t all = hgv_graph_attention_ws(N, num_graphs, H, Hk, D, n_tiles, 0);
+    return all && at_no_images(false, max_rows) ? 256 : all;
 }
 
 extern "C" int hgv_graph_attention_fwd(const float* q, int64_t q_row, int64_t q_head, const float* k, int64_t k_row, int64_t k_head,

@@ -2834,7 +2834,7 @@ class _GraphAttention(torch.autograd.Function):
         out = torch.empty(n, h, d, dtype=torch.float32, device=q.device)
         train = train and any(ctx.needs_input_grad[:3])
         stats = torch.empty(h, n, 2, dtype=torch.float32, device=q.device) if train else None
-        nws = _lib.load().hgv_graph_attention_ws(n, seg.num_graphs, h, hk, d, seg._n_tiles, 0)
+        nws = _lib.load().hgv_graph_attention_fwd_ws(n, seg.num_graphs, h, hk, d, seg._n_tiles, seg._attention_plan[1])
         ws = torch.empty(nws, dtype=torch.uint8, device=q.device)
         _lib.call("hgv_graph_attention_fwd", *_strided(q), *_strided(k), *_strided(v), n, seg.num_graphs, h, hk, d, scale, _lib.ptr(mask),
                   *seg._attention_plan, out.data_ptr(), _lib.ptr(stats), ws.data_ptr(), nws, _lib.stream())

@@ -624,6 +624,8 @@ int hgv_group_norm_bwd(const float* g, int64_t ldg, const float* x, int64_t ldx,
  * inverse of that sum; +inf and 0 for a row without keys) may be NULL in the forward pass; the backward pass
  * reads it and out.  dq, or dk and dv together, may be NULL. */
 size_t hgv_graph_attention_ws(int64_t N, int num_graphs, int H, int Hk, int D, int64_t n_tiles, int backward);
+/* ... of the forward pass over graphs of at most max_rows rows: next to nothing where all are small. */
+size_t hgv_graph_attention_fwd_ws(int64_t N, int num_graphs, int H, int Hk, int D, int64_t n_tiles, int max_rows);
 int hgv_graph_attention_fwd(const float* q, int64_t q_row, int64_t q_head, const float* k, int64_t k_row, int64_t k_head, const float* v,
                             int64_t v_row, int64_t v_head, int64_t N, int num_graphs, int H, int Hk, int D, float scale,
                             const uint8_t* mask, const int32_t* ptr, int max_rows, const int32_t* tiles, int n_tiles, const int32_t* blocks,
