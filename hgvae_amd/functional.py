@@ -2476,12 +2476,12 @@ def _first_order(backward):
     guarded = torch.autograd.function.once_differentiable(backward)
 
     @functools.wraps(backward)
-    def run(ctx, g):
+    def run(ctx, *g):
         if ctx.leaves and torch.cuda.is_current_stream_capturing():
             if any(s.stream == 0 for s in ctx.leaves):
                 raise _lib.HgvError("a backward pass cannot be captured while a graph of the same parameters that was built on the default "
                                     "stream is alive: drop its outputs (losses, activations) before the capture")
-        return guarded(ctx, g) if torch.is_grad_enabled() else backward(ctx, g)
+        return guarded(ctx, *g) if torch.is_grad_enabled() else backward(ctx, *g)
     return run
 
 
@@ -2586,6 +2586,18 @@ def _product8(x: torch.Tensor, img: "_Image", bias, n_out: int) -> torch.Tensor:
     return y
 
 
+def _product_keep8(x: torch.Tensor, img: "_Image", bias, n_out: int):
+    """:func:`_product8`, and x in 8 bits."""
+    if img.kind != "f16x3" or _probe is not None:
+        return _product8(x, img, bias, n_out), _pack8(x)
+    n, k = x.shape
+    y = new_padded(n, n_out, x.device, zero_pad=False)
+    p = _empty8(n, k, x.device)
+    _lib.call("hgv_gemm_nt16h_keep8", x.data_ptr(), ld_of(x), k, img.a.data_ptr(), _lib.ptr(bias), n, n_out, y.data_ptr(), ld_of(y),
+              p.q.data_ptr(), p.q.stride(0), p.scale.data_ptr(), _lib.stream())
+    return y, p
+
+
 class _Piece:
     """Part of a buffer that only kernels look at: its address, and the buffer that keeps it."""
     __slots__ = ("buf", "address")
@@ -2640,14 +2652,7 @@ class _Linear8(torch.autograd.Function):
         if not need[1]:
             ctx.save_for_backward(w)
             return _product8(x, fwd, bias, w.size(0))
-        if fwd.kind == "f16x3" and _probe is None:
-            n, k = x.shape
-            y = new_padded(n, w.size(0), x.device, zero_pad=False)
-            p = _empty8(n, k, x.device)
-            _lib.call("hgv_gemm_nt16h_keep8", x.data_ptr(), ld_of(x), k, fwd.a.data_ptr(), _lib.ptr(bias), n, w.size(0), y.data_ptr(), ld_of(y),
-                      p.q.data_ptr(), p.q.stride(0), p.scale.data_ptr(), _lib.stream())
-        else:
-            y, p = _product8(x, fwd, bias, w.size(0)), _pack8(x)
+        y, p = _product_keep8(x, fwd, bias, w.size(0))
         ctx.packed = p.shape
         ctx.save_for_backward(w, p.q, p.scale)
         return y
@@ -2685,6 +2690,68 @@ def _weight_grad8(g: torch.Tensor, x8: Packed8, want_bias: bool):
     return gw, gb
 
 
+class _Linear8Each(torch.autograd.Function):
+    """y_i = x W_i^T of several weights, with x kept in 8 bits once."""
+
+    @staticmethod
+    def forward(ctx, x, train, *ws):
+        need = ctx.needs_input_grad if train else (False,) * (2 + len(ws))
+        ctx.leaves = _leaves_of(x, *ws) if train else ()
+        x = _rows16(x)
+        pairs = [_image_pair(w, need[0]) for w in ws]
+        ctx.images = [back for _, back in pairs]
+        ctx.packed, kept, ys = None, (), []
+        for w, (fwd, _) in zip(ws, pairs):
+            if any(need[2:]) and ctx.packed is None:
+                y, p = _product_keep8(x, fwd, None, w.size(0))
+                ctx.packed, kept = p.shape, (p.q, p.scale)
+            else:
+                y = _product8(x, fwd, None, w.size(0))
+            ys.append(y)
+        ctx.save_for_backward(*kept, *ws)
+        return tuple(ys)
+
+    @staticmethod
+    @_first_order
+    def backward(ctx, *gs):
+        return _on_device(gs[0], _Linear8Each._grads, ctx, gs)
+
+    @staticmethod
+    def _grads(ctx, gs):
+        need = ctx.needs_input_grad
+        saved = ctx.saved_tensors
+        ws = saved[len(saved) - len(gs):]
+        gs = [_rows16(g) for g in gs]
+        gw = [None] * len(gs)
+        for i, g in enumerate(gs):
+            if need[2 + i]:
+                gw[i] = _weight_grad8(g, Packed8(*saved[:2], ctx.packed), False)[0]
+        gx = None
+        if need[0]:
+            whole = lambda t: t.as_strided((t.size(0), t.stride(0)), (t.stride(0), 1))          # with the pad columns: one run of memory
+            for g, w, image in zip(gs, ws, ctx.images):
+                part = _product8(g, image, None, w.size(1))
+                gx = part if gx is None else (whole(gx).add_(whole(part)), gx)[1]
+        return (gx, None, *gw)
+
+
+def _linear8_each(x: torch.Tensor, weights):
+    """:func:`linear8` of one matrix with several weights, without biases: what it keeps of ``x`` serves all of them."""
+    x = plain(x)
+    for w in weights:
+        _check_linear8(x, w)
+    if x.size(0) == 0:
+        return tuple(torch.nn.functional.linear(x, w) for w in weights)
+    return _on_device(x, _Linear8Each.apply, x, torch.is_grad_enabled(), *weights)
+
+
+def _check_linear8(x, w):
+    _check_matrix("x", x)
+    _check_matrix("w", w, x.device, x.size(1))
+    if not 1 <= w.size(0) <= MAX_GEMM_N or not 1 <= w.size(1) <= MAX_GEMM_N:
+        raise _lib.HgvError(f"projection widths above {MAX_GEMM_N} are not supported (got {tuple(w.shape)})")
+
+
 def linear8(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``x @ w.T + bias`` with fp32 results, as :func:`dual_linear`, that keeps ``x`` in 8 bits (:func:`pack8`) for the
     backward pass: a quarter of the memory.  The gradients with respect to ``x`` and ``bias`` are those of the exact
@@ -2692,10 +2759,7 @@ def linear8(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = Non
     again.  ``x`` may be a slice of a wider matrix, whatever that holds beside it; rows that are not a multiple of 16 bytes
     apart are copied."""
     x = plain(x)
-    _check_matrix("x", x)
-    _check_matrix("w", w, x.device, x.size(1))
-    if not 1 <= w.size(0) <= MAX_GEMM_N or not 1 <= w.size(1) <= MAX_GEMM_N:
-        raise _lib.HgvError(f"projection widths above {MAX_GEMM_N} are not supported (got {tuple(w.shape)})")
+    _check_linear8(x, w)
     bias = _check_vector("bias", bias, w.size(0), x.device)
     if x.size(0) == 0:
         return torch.nn.functional.linear(x, w, bias)           # no rows: an empty matrix, zero gradients

@@ -151,7 +151,7 @@ class Linear8(nn.Linear):
 class GraphAttention(nn.Module):
     """Multi-head attention among the nodes of each graph: projections to ``heads`` queries and ``kv_heads`` keys and
     values, :func:`~hgvae_amd.functional.graph_attention`, output projection.  ``forward(x, segments, mask=None)``.  With
-    ``keep8`` the projections keep their input in 8 bits for the backward pass."""
+    ``keep8`` the projections keep their input in 8 bits for the backward pass, the first three one form of it."""
 
     def __init__(self, channels: int, heads: int = 1, kv_heads: int = None, head_dim: int = None, keep8: bool = False):
         super().__init__()
@@ -173,7 +173,9 @@ class GraphAttention(nn.Module):
     def forward(self, x: torch.Tensor, segments, mask=None) -> torch.Tensor:
         project = Fn.linear8 if self.keep8 else (lambda x, w, b=None: Fn.dual_linear(x, w, bias=b))
         n, d = x.size(0), self.head_dim
-        q, k, v = (project(x, lin.weight).unflatten(1, (-1, d)) for lin in (self.lin_q, self.lin_k, self.lin_v))
+        weights = [lin.weight for lin in (self.lin_q, self.lin_k, self.lin_v)]
+        qkv = Fn._linear8_each(x, weights) if self.keep8 else [project(x, w) for w in weights]
+        q, k, v = (t.unflatten(1, (-1, d)) for t in qkv)
         out = Fn.graph_attention(q, k, v, segments, mask=mask)
         return project(out.reshape(n, self.heads * d), self.lin_out.weight, self.lin_out.bias)
 
