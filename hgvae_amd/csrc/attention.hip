@@ -357,7 +357,9 @@ __device__ __forceinline__ void fwd_tile(const unsigned char* ldsK, const unsign
         if (biased) {
             const f32x4 o = *(const f32x4*)(bias + 16 * b + 4 * g);
 #pragma unroll
-            for (int j = 0; j < QB; ++j) s[b][j] += o;
+            for (int j = 0; j < QB; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[b][j][i] = o[i] < 0.f ? -INFINITY : s[b][j][i];        // a sum would keep a NaN
         }
     }
 #pragma unroll

@@ -79,3 +79,18 @@ def test_dq_of_ordinary_rows_beside_one_with_a_large_gradient(n, h, hk, d, facto
         # by row: pieces of 22 bits in q, k, v and g, and fp32 sums
         off = (dq[:, head] - want).norm(dim=1) / want.norm(dim=1)
         assert float(off.max()) <= 2.0 ** -15, float(off.max())
+
+
+@pytest.mark.parametrize("sizes", [[40, 70], [600, 90]])
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+def test_bad_queries_of_a_graph_without_keys_give_zeros(sizes, value):
+    """A graph without keys gives zeros and zero gradients, whatever its rows of q, k, v and g hold; the other keeps its bits."""
+    n, first = sum(sizes), sizes[0]
+    q, k, v, g = make(n, 4, 2, 24, seed=n)
+    mask = torch.arange(n, device=dev()) >= first
+    want = run(q, k, v, sizes, g, mask)
+    for t in (q, k, v, g):
+        t[3], t[first - 1, 0, 5] = value, value
+    got = run(q, k, v, sizes, g, mask)
+    for name, a, b in zip(("out", "dq", "dk", "dv"), got, want):
+        assert not bool(a[:first].any()) and torch.equal(a[first:], b[first:]), name
