@@ -2783,7 +2783,7 @@ class _GroupNormAct(torch.autograd.Function):
         n, c = x.shape
         dev = x.device
         out = new_padded(n, c, dev, zero_pad=False)
-        arrays, counts, nws, _ = seg._norm_plan(c, groups)
+        arrays, counts, nws, _ = seg._norm_plan(c, groups, is_vec4(x))
         # the statistics, [mean fp64 | rstd fp32] per (graph, group), and a small workspace in one buffer
         at = seg.num_graphs * groups
         own = (at + (at + 1) // 2 + 31) // 32 * 32
@@ -2824,7 +2824,8 @@ class _GroupNormAct(torch.autograd.Function):
         gx = new_padded(n, c, dev, zero_pad=False) if need[0] else None
         gw = torch.empty(c, dtype=torch.float32, device=dev) if need[1] else None
         gb = torch.empty(c, dtype=torch.float32, device=dev) if need[2] else None
-        arrays, counts, _, nws = seg._norm_plan(c, groups)
+        wide = is_vec4(g) and (ctx.packed is not None or is_vec4(kept[0]))
+        arrays, counts, _, nws = seg._norm_plan(c, groups, wide)
         ws = torch.empty(nws, dtype=torch.uint8, device=dev)
         if ctx.packed is None:
             source = (kept[0].data_ptr(), ld_of(kept[0]), None, 0, None)

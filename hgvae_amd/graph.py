@@ -364,20 +364,22 @@ class Segments:
             raise _lib.HgvError(f"Segments: {count} graphs")
         return cls(np.bincount(host, minlength=count) if host.size else np.zeros(count, dtype=np.int64), batch.device)
 
-    def _norm_plan(self, columns: int, groups: int):
+    def _norm_plan(self, columns: int, groups: int, wide: bool):
         """What a call of the norm passes on: (device arrays), (graphs, graphs with rows, how many of them one workgroup reads at
-        once, rows of the largest of those, first chunk of the others, end of the chunks), workspace bytes forward and backward."""
-        plan = self._norm_plans.get((columns, groups))
+        once, rows of the largest of those, first chunk of the others, end of the chunks), workspace bytes forward and backward.
+        ``wide``: the matrices' rows are multiples of 16 bytes apart."""
+        plan = self._norm_plans.get((columns, groups, wide))
         if plan is None:
             lib = _lib.load()
             limit = lib.hgv_group_norm_small_rows(columns, groups)
             per = columns // groups
             slab = per * max(1, -(-32 // per))                  # the columns that a workgroup takes
-            if slab < columns and slab % 32 and 4 * self.num_rows * columns > 64 << 20:
+            if wide and slab < columns and slab % 32 and 4 * self.num_rows * columns > 64 << 20:
                 # one read of a whole graph per workgroup saves launches and passes.  Where memory is what counts and its pieces of rows
-                # are not whole lines, long graphs run faster in chunks (forward and backward, one read / chunks; 138 columns in slabs
-                # of 46: 2 048 graphs of 300 rows 819 / 617 us, 2 500 of 200 rows 676 / 572, 2 048 of 138 rows 340 / 335, 128 of 300
-                # rows 54 / 62;  256 columns in slabs of 32: 2 500 of 200 rows 778 / 1 049, 1 500 of 340 rows 920 / 948)
+                # are not whole lines, long graphs run faster in chunks of 16-byte reads (forward and backward, one read / chunks, 50 M values:
+                # slabs of 33 columns, graphs of 130 rows 477 / 473 us, of 200 466 / 435, of 300 516 / 362;  of 46 columns 430 / 439, 512 / 413,
+                # 460 / 353;  of 60 columns 485 / 380, 419 / 382;  256 columns in slabs of 32: 2 500 of 200 rows 778 / 1 049).  Chunks in
+                # 4-byte reads are slower (138 columns without pads: 130 rows 432 / 587, 200 rows 514 / 595, 300 rows 461 / 493)
                 limit = min(limit, 160)
             n, listed = bisect.bisect_right(self._sorted, limit), len(self._sorted)
             if n < listed and 8 * sum(self._sorted[:n]) < self.num_rows:
@@ -386,7 +388,7 @@ class Segments:
             ws = [lib.hgv_group_norm_ws(chunks[1] - chunks[0], self.num_graphs, listed, n, columns, groups, b) for b in (0, 1)]
             plan = (tuple(t.data_ptr() for t in (self._ptr, self._order, self._chunks, self._first)),
                     (self.num_graphs, listed, n, self._sorted[n - 1] if n else 0, *chunks), *ws)
-            self._norm_plans[columns, groups] = plan
+            self._norm_plans[columns, groups, wide] = plan
         return plan
 
     def __repr__(self):
