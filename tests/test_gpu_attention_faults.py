@@ -94,3 +94,18 @@ def test_bad_queries_of_a_graph_without_keys_give_zeros(sizes, value):
     got = run(q, k, v, sizes, g, mask)
     for name, a, b in zip(("out", "dq", "dk", "dv"), got, want):
         assert not bool(a[:first].any()) and torch.equal(a[first:], b[first:]), name
+
+
+@pytest.mark.parametrize("h,hk,d", [(2, 1, 23), (1, 1, 64)])
+@pytest.mark.parametrize("sizes", [[8] * 40 + [513, 512], [512, 511, 1, 64], [600] + [3] * 30])
+def test_graphs_on_both_sides_of_the_limit_of_the_small_kernel(sizes, h, hk, d):
+    """Batches whose largest graph takes images of the operands, with graphs of a few rows beside it, and batches that do without."""
+    from test_gpu_graph_attention import check, reference
+    n = sum(sizes)
+    q, k, v, g = make(n, h, hk, d, seed=n + d)
+    mask = torch.rand(n, generator=torch.Generator(device=dev()).manual_seed(d), device=dev()) < 0.7
+    for m in (None, mask):
+        got = run(q, k, v, sizes, g, m)
+        want, bound = reference(q, k, v, sizes, m, d ** -0.5, g)
+        for name, a, e, b in zip(("out", "dq", "dk", "dv"), got, want, bound):
+            check(a, e, b, name)
