@@ -327,6 +327,36 @@ __device__ __forceinline__ void store4(float* p, int d, int D, f32x4 v) {
     }
 }
 
+// Long sums in two steps: what the matrix cores have added over PART tiles of 64 rows goes to a second sum in LDS.  One sum alone is rounded
+// six times per tile at its own size, and what out is off by enters all terms of a row of dq.  13 000 nodes, two key heads of 4, values and
+// gradients with a mean, from 64 bits with one sum / two: out 1.5e-6 / 1.7e-7, dq 4.1e-5 / 3.9e-6, dk 4.7e-6 / 2.6e-7, dv 4.9e-6 / 1.8e-7;  no
+// difference in time (second sums in the output's rows instead: 5 to 12 % of the kernels').  Kept where the workgroups that share a compute
+// unit still fit into its LDS: everywhere but for dv of 64- and 128-wide heads and out of 96-wide ones in blocks of 128 rows.  A thread
+// has SLOTS values of four columns there, `held` once there is something in them.
+constexpr int PART = 16;
+constexpr bool two_fit(int DP, int slots, int NW, int waves) {      // waves per SIMD that are to stay
+    return (waves * 4 / NW) * (2 * 64 * (4 * DP + 16) + slots * NW * 1024 + 1024) <= 160 * 1024;
+}
+template <int SLOTS, int NW, bool TWO>
+struct Second {
+    static constexpr int FLOATS = TWO ? NW * SLOTS * 256 : 4;
+    f32x4* lds;
+    bool held;                                                  // the same for the whole workgroup
+    __device__ __forceinline__ explicit Second(float* p) : lds((f32x4*)p), held(false) {}
+    __device__ __forceinline__ f32x4& at(int slot) const { return lds[(threadIdx.x >> 6) * (SLOTS * 64) + (threadIdx.x & 63) + slot * 64]; }
+    __device__ __forceinline__ void take(int slot, f32x4& v) const {                // v joins the second sum and starts again
+        at(slot) = held ? at(slot) + v : v;
+        v = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    __device__ __forceinline__ void scale(int first, int step, float f) const {
+        if (TWO && held) {
+#pragma unroll 1
+            for (int slot = first; slot < SLOTS; slot += step) at(slot) *= f;
+        }
+    }
+    __device__ __forceinline__ f32x4 total(int slot, f32x4 v) const { return TWO && held ? at(slot) + v : v; }
+};
+
 constexpr float P_BITS = 8.f;                                   // probabilities start at 2^8 and may grow to 2^15 before a rescale
 constexpr float P_GROW = 7.f;
 
@@ -337,10 +367,10 @@ constexpr int at_bounds(int DP, int NW) { return DP == 128 && NW == 4 ? 1 : 2; }
 // One tile of 64 keys (pieces in LDS) against a wave's queries.  c: what a product of the pieces is multiplied by, base 2.  RN: the
 // probabilities' pieces to nearest, which shows in the sums over a few keys (graphs of two rows: 1.0e-7 -> 6.5e-8 of the result) and
 // would take 3 (64 columns) to 7 % (23) of the time of large graphs.
-template <int DP, int QB, bool RN>
+template <int DP, int QB, bool RN, typename S2>
 __device__ __forceinline__ void fwd_tile(const unsigned char* ldsK, const unsigned char* ldsV, const float* bias, bool biased, int lane,
                                          const float (&c)[QB], const Frag (&q)[QB][DP / 32], float (&m)[QB], float (&l)[QB],
-                                         f32x4 (&acc)[DP / 16][QB], float neg) {
+                                         f32x4 (&acc)[DP / 16][QB], float neg, const S2& second) {
     constexpr int KC = DP / 32, DB = DP / 16;
     const int g = lane >> 4;
     f32x4 s[4][QB];
@@ -377,6 +407,7 @@ __device__ __forceinline__ void fwd_tile(const unsigned char* ldsK, const unsign
             l[b] *= f;
 #pragma unroll
             for (int d = 0; d < DB; ++d) acc[d][b] *= f;
+            second.scale(b, QB, f);
         }
         const float off = m[b] == -INFINITY ? 0.f : P_BITS - m[b];
         float sum[4] = {0.f, 0.f, 0.f, 0.f};
@@ -405,9 +436,9 @@ __device__ __forceinline__ void fwd_tile(const unsigned char* ldsK, const unsign
 }
 
 // The rows of a wave's queries, and their stats; ev: exponent of the values' scale.
-template <int DP, int QB>
+template <int DP, int QB, typename S2>
 __device__ __forceinline__ void fwd_rows(const AtArgs& a, int64_t q0, int64_t k1, int h, int lane, int ev, const float (&m)[QB], float (&l)[QB],
-                                         const f32x4 (&acc)[DP / 16][QB]) {
+                                         const f32x4 (&acc)[DP / 16][QB], const S2& second) {
     constexpr int DB = DP / 16;
     const int g = lane >> 4;
 #pragma unroll
@@ -420,7 +451,7 @@ __device__ __forceinline__ void fwd_rows(const AtArgs& a, int64_t q0, int64_t k1
         const float f = none ? 0.f : ldexpf(1.f / l[b], ev - 15);
         float* o = row_out(a.out, row, a.H, h, a.D);
 #pragma unroll
-        for (int d = 0; d < DB; ++d) store4(o, 16 * d + 4 * g, a.D, none ? f32x4{0.f, 0.f, 0.f, 0.f} : acc[d][b] * f);
+        for (int d = 0; d < DB; ++d) store4(o, 16 * d + 4 * g, a.D, none ? f32x4{0.f, 0.f, 0.f, 0.f} : second.total(d * QB + b, acc[d][b]) * f);
         if (g == 0 && a.stats) {
             const int e = (int)(__float_as_uint(l[b]) >> 23) - 127;         // l = 2^e * (1 ... 2)
             a.stats[(int64_t)h * a.N + row] = none ? make_float2(INFINITY, 0.f) : make_float2(m[b] - P_BITS + (float)e, ldexpf(1.f / l[b], e));
@@ -440,6 +471,10 @@ __global__ __launch_bounds__(64 * NW, DP == 32 ? 4 : at_bounds(DP, NW)) void k_a
     __shared__ __align__(16) unsigned char ldsK[64 * line_bytes<DP>()];
     __shared__ __align__(16) unsigned char ldsV[64 * line_bytes<DP>()];
     __shared__ __align__(16) float bias[64];
+    constexpr bool TWO = two_fit(DP, DB * QB, NW, DP == 32 ? 4 : at_bounds(DP, NW));
+    typedef Second<DB * QB, NW, TWO> S2;
+    __shared__ __align__(16) float ldsS[S2::FLOATS];
+    S2 second(ldsS);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int blk = blockIdx.x / a.H, h = blockIdx.x - blk * a.H, hk = h / a.R;
     const int4 t = a.blocks[blk];
@@ -469,23 +504,33 @@ __global__ __launch_bounds__(64 * NW, DP == 32 ? 4 : at_bounds(DP, NW)) void k_a
     sk.load(ki, min(64, n));
     sv.load(vi, min(64, n));
     float nb = threadIdx.x < 64 && (int)threadIdx.x < n && (!a.mask || a.mask[k0 + threadIdx.x]) ? 0.f : -INFINITY;
-    for (int kt = 0; kt < n; kt += 64) {
-        __syncthreads();
-        sk.store(ldsK);
-        sv.store(ldsV);
-        if (threadIdx.x < 64) bias[threadIdx.x] = nb;
-        __syncthreads();
-        const int next = kt + 64;
-        if (next < n) {
-            sk.load(ki + (int64_t)next * (2 * DP), min(64, n - next));
-            sv.load(vi + (int64_t)next * (2 * DP), min(64, n - next));
-            const int j = next + (int)threadIdx.x;
-            nb = threadIdx.x < 64 && j < n && (!a.mask || a.mask[k0 + j]) ? 0.f : -INFINITY;
+    for (int kt0 = 0; kt0 < n; kt0 += 64 * PART) {
+        const int kt1 = min(n, kt0 + 64 * PART);
+        for (int kt = kt0; kt < kt1; kt += 64) {
+            __syncthreads();
+            sk.store(ldsK);
+            sv.store(ldsV);
+            if (threadIdx.x < 64) bias[threadIdx.x] = nb;
+            __syncthreads();
+            const int next = kt + 64;
+            if (next < n) {
+                sk.load(ki + (int64_t)next * (2 * DP), min(64, n - next));
+                sv.load(vi + (int64_t)next * (2 * DP), min(64, n - next));
+                const int j = next + (int)threadIdx.x;
+                nb = threadIdx.x < 64 && j < n && (!a.mask || a.mask[k0 + j]) ? 0.f : -INFINITY;
+            }
+            const bool biased = a.mask != nullptr || kt + 64 > n;
+            fwd_tile<DP, QB, false>(ldsK, ldsV, bias, biased, lane, c, q, m, l, acc, a.neg, second);
         }
-        const bool biased = a.mask != nullptr || kt + 64 > n;
-        fwd_tile<DP, QB, false>(ldsK, ldsV, bias, biased, lane, c, q, m, l, acc, a.neg);
+        if (TWO && kt1 < n) {
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int b = 0; b < QB; ++b) second.take(d * QB + b, acc[d][b]);
+            second.held = true;
+        }
     }
-    fwd_rows<DP, QB>(a, q0, k1, h, lane, ex[TV], m, l, acc);
+    fwd_rows<DP, QB>(a, q0, k1, h, lane, ex[TV], m, l, acc, second);
 }
 
 // Graphs of few rows: the operands as they are, without images.  Every workgroup splits what it multiplies on the way into the
@@ -574,6 +619,7 @@ __global__ __launch_bounds__(64 * NW, DP == 32 ? 3 : at_bounds(DP, NW)) void k_a
     for (int d = 0; d < DB; ++d)
 #pragma unroll
         for (int b = 0; b < QB; ++b) acc[d][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const Second<1, 1, false> none(nullptr);
     int ev = -126;
     for (int kt = 0; kt < n; kt += 64) {
         uint32_t uk = 0, uv = 0;
@@ -623,21 +669,26 @@ __global__ __launch_bounds__(64 * NW, DP == 32 ? 3 : at_bounds(DP, NW)) void k_a
         float c[QB];
 #pragma unroll
         for (int b = 0; b < QB; ++b) c[b] = fold_scale(a.scale, eq[b] + ek - 30);
-        fwd_tile<DP, QB, true>(ldsK, ldsV, bias, biased, lane, c, q, m, l, acc, a.neg);
+        fwd_tile<DP, QB, true>(ldsK, ldsV, bias, biased, lane, c, q, m, l, acc, a.neg, none);
     }
-    fwd_rows<DP, QB>(a, q0, k1, h, lane, ev, m, l, acc);
+    fwd_rows<DP, QB>(a, q0, k1, h, lane, ev, m, l, acc, none);
 }
 
 // ---- backward: dk and dv ---------------------------------------------------------------------------------------------------
 // A workgroup owns 16 * KB * NW keys of one key head (a wave 16 * KB), walks the queries of the graph, head by head, in tiles of 64 rows.
 // Two products in, two out; the same graphs 3.8 ... 4.0 ms (1.25 PFLOP/s of piece products).
 template <int DP, int KB, int NW>
-__global__ __launch_bounds__(64 * NW, at_bounds(DP, NW)) void k_at_dkv(const AtArgs a) {
+__global__ __launch_bounds__(64 * NW, DP == 32 ? 3 : at_bounds(DP, NW)) void k_at_dkv(const AtArgs a) {
     constexpr int KC = DP / 32, DB = DP / 16;
     __shared__ __align__(16) unsigned char ldsQ[64 * line_bytes<DP>()];
     __shared__ __align__(16) unsigned char ldsG[64 * line_bytes<DP>()];
     __shared__ __align__(16) float ldsL[64];
     __shared__ __align__(16) float ldsD[64];
+    constexpr int WAVES = DP == 32 ? 3 : at_bounds(DP, NW);
+    constexpr bool BOTH = two_fit(DP, 2 * DB * KB, NW, WAVES), TWO = BOTH || two_fit(DP, DB * KB, NW, WAVES);       // dk and dv, or dk alone
+    typedef Second<(BOTH ? 2 : 1) * DB * KB, NW, TWO> S2;
+    __shared__ __align__(16) float ldsS[S2::FLOATS];
+    S2 second(ldsS);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
     const int blk = blockIdx.x / a.Hk, hk = blockIdx.x - blk * a.Hk;
     const int4 t = a.blocks[blk];
@@ -674,66 +725,79 @@ __global__ __launch_bounds__(64 * NW, at_bounds(DP, NW)) void k_at_dkv(const AtA
         }
     };
     fetch(0);
-    for (int step = 0; step < steps; ++step) {
-        __syncthreads();
-        sq.store(ldsQ);
-        sg.store(ldsG);
-        if (threadIdx.x < 64) {
-            ldsL[threadIdx.x] = -nl;
-            ldsD[threadIdx.x] = ldexpf(nd, -ex[TV]);
-        }
-        __syncthreads();
-        if (step + 1 < steps) fetch(step + 1);
+    for (int step0 = 0; step0 < steps; step0 += PART) {
+        const int step1 = min(steps, step0 + PART);
+        for (int step = step0; step < step1; ++step) {
+            __syncthreads();
+            sq.store(ldsQ);
+            sg.store(ldsG);
+            if (threadIdx.x < 64) {
+                ldsL[threadIdx.x] = -nl;
+                ldsD[threadIdx.x] = ldexpf(nd, -ex[TV]);
+            }
+            __syncthreads();
+            if (step + 1 < steps) fetch(step + 1);
 #pragma unroll
-        for (int qc = 0; qc < 2; ++qc) {                        // 32 queries at a time
-            Frag pf[KB], df[KB];
-            {
-                f32x4 p[2][KB], s[2][KB];
+            for (int qc = 0; qc < 2; ++qc) {                        // 32 queries at a time
+                Frag pf[KB], df[KB];
+                {
+                    f32x4 p[2][KB], s[2][KB];
 #pragma unroll
-                for (int b = 0; b < 2; ++b) {
-                    const int r0 = 32 * qc + 16 * b;
+                    for (int b = 0; b < 2; ++b) {
+                        const int r0 = 32 * qc + 16 * b;
 #pragma unroll
-                    for (int j = 0; j < KB; ++j) p[b][j] = s[b][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+                        for (int j = 0; j < KB; ++j) p[b][j] = s[b][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int k = 0; k < KC; ++k) {
-                        const Frag f = row_frag<DP>(ldsQ, r0, k, lane);
+                        for (int k = 0; k < KC; ++k) {
+                            const Frag f = row_frag<DP>(ldsQ, r0, k, lane);
 #pragma unroll
-                        for (int j = 0; j < KB; ++j) p[b][j] = mma3(f, kf[j][k], p[b][j]);
-                    }
-#pragma unroll
-                    for (int k = 0; k < KC; ++k) {
-                        const Frag f = row_frag<DP>(ldsG, r0, k, lane);
-#pragma unroll
-                        for (int j = 0; j < KB; ++j) s[b][j] = mma3(f, vf[j][k], s[b][j]);
-                    }
-                    const f32x4 ls = *(const f32x4*)(ldsL + r0 + 4 * g), de = *(const f32x4*)(ldsD + r0 + 4 * g);
-#pragma unroll
-                    for (int j = 0; j < KB; ++j)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            p[b][j][i] = exp2_fast(fmaf(p[b][j][i], c, ls[i]));
-                            s[b][j][i] = p[b][j][i] * fmaf(s[b][j][i], 0x1p-17f, -de[i]);
-                            p[b][j][i] *= 0x1p14f;
+                            for (int j = 0; j < KB; ++j) p[b][j] = mma3(f, kf[j][k], p[b][j]);
                         }
+#pragma unroll
+                        for (int k = 0; k < KC; ++k) {
+                            const Frag f = row_frag<DP>(ldsG, r0, k, lane);
+#pragma unroll
+                            for (int j = 0; j < KB; ++j) s[b][j] = mma3(f, vf[j][k], s[b][j]);
+                        }
+                        const f32x4 ls = *(const f32x4*)(ldsL + r0 + 4 * g), de = *(const f32x4*)(ldsD + r0 + 4 * g);
+#pragma unroll
+                        for (int j = 0; j < KB; ++j)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                p[b][j][i] = exp2_fast(fmaf(p[b][j][i], c, ls[i]));
+                                s[b][j][i] = p[b][j][i] * fmaf(s[b][j][i], 0x1p-17f, -de[i]);
+                                p[b][j][i] *= 0x1p14f;
+                            }
+                    }
+#pragma unroll
+                    for (int j = 0; j < KB; ++j) {
+                        pf[j] = split_frag(p[0][j], p[1][j], a.neg);
+                        df[j] = split_frag(s[0][j], s[1][j], a.neg);
+                    }
                 }
 #pragma unroll
-                for (int j = 0; j < KB; ++j) {
-                    pf[j] = split_frag(p[0][j], p[1][j], a.neg);
-                    df[j] = split_frag(s[0][j], s[1][j], a.neg);
+                for (int d = 0; d < DB; ++d) {
+                    const Frag f = col_frag<DP>(ldsG, 32 * qc, d, lane);
+#pragma unroll
+                    for (int j = 0; j < KB; ++j) dv[d][j] = mma3(f, pf[j], dv[d][j]);
+                }
+#pragma unroll
+                for (int d = 0; d < DB; ++d) {
+                    const Frag f = col_frag<DP>(ldsQ, 32 * qc, d, lane);
+#pragma unroll
+                    for (int j = 0; j < KB; ++j) dk[d][j] = mma3(f, df[j], dk[d][j]);
                 }
             }
+        }
+        if (TWO && step1 < steps) {
 #pragma unroll
-            for (int d = 0; d < DB; ++d) {
-                const Frag f = col_frag<DP>(ldsG, 32 * qc, d, lane);
+            for (int d = 0; d < DB; ++d)
 #pragma unroll
-                for (int j = 0; j < KB; ++j) dv[d][j] = mma3(f, pf[j], dv[d][j]);
-            }
-#pragma unroll
-            for (int d = 0; d < DB; ++d) {
-                const Frag f = col_frag<DP>(ldsQ, 32 * qc, d, lane);
-#pragma unroll
-                for (int j = 0; j < KB; ++j) dk[d][j] = mma3(f, df[j], dk[d][j]);
-            }
+                for (int b = 0; b < KB; ++b) {
+                    second.take(d * KB + b, dk[d][b]);
+                    if (BOTH) second.take((DB + d) * KB + b, dv[d][b]);
+                }
+            second.held = true;
         }
     }
 #pragma unroll
@@ -746,11 +810,11 @@ __global__ __launch_bounds__(64 * NW, at_bounds(DP, NW)) void k_at_dkv(const AtA
         const int ek = ex[TG] + ex[TV] + ex[TQ] - 28, ev = ex[TG] - 29;
 #pragma unroll
         for (int d = 0; d < DB; ++d) {
-            f32x4 x, y;
+            f32x4 x = second.total(d * KB + b, dk[d][b]), y = BOTH ? second.total((DB + d) * KB + b, dv[d][b]) : dv[d][b];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                x[i] = live && many ? ldexpf(dk[d][b][i] * a.scale, ek) : 0.f;
-                y[i] = live ? ldexpf(dv[d][b][i], ev) : 0.f;
+                x[i] = live && many ? ldexpf(x[i] * a.scale, ek) : 0.f;
+                y[i] = live ? ldexpf(y[i], ev) : 0.f;
             }
             store4(pk, 16 * d + 4 * g, a.D, x);
             store4(pv, 16 * d + 4 * g, a.D, y);
@@ -768,11 +832,15 @@ __global__ __launch_bounds__(64 * NW, at_bounds(DP, NW)) void k_at_dkv(const AtA
 // log2 F bits lower, behind probabilities of 1 / n already (one row of 5 000 with 16 384 times the others' gradient, the others' dq by row:
 // 1.6e-3 from 64 bits; so 2e-6, the formulas in fp32 2.5e-6).
 template <int DP, int QB, int NW>
-__global__ __launch_bounds__(64 * NW, at_bounds(DP, NW)) void k_at_dq(const AtArgs a) {
+__global__ __launch_bounds__(64 * NW, DP == 32 ? 3 : at_bounds(DP, NW)) void k_at_dq(const AtArgs a) {
     constexpr int KC = DP / 32, DB = DP / 16;
     __shared__ __align__(16) unsigned char ldsK[64 * line_bytes<DP>()];
     __shared__ __align__(16) unsigned char ldsV[64 * line_bytes<DP>()];
     __shared__ __align__(16) float bias[64];
+    constexpr bool TWO = two_fit(DP, DB * QB, NW, DP == 32 ? 3 : at_bounds(DP, NW));
+    typedef Second<DB * QB, NW, TWO> S2;
+    __shared__ __align__(16) float ldsS[S2::FLOATS];
+    S2 second(ldsS);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
     const int blk = blockIdx.x / a.H, h = blockIdx.x - blk * a.H, hk = h / a.R;
     const int4 t = a.blocks[blk];
@@ -836,64 +904,74 @@ __global__ __launch_bounds__(64 * NW, at_bounds(DP, NW)) void k_at_dq(const AtAr
     sk.load(ki, min(64, n));
     sv.load(vi, min(64, n));
     float nb = threadIdx.x < 64 && (int)threadIdx.x < n && (!a.mask || a.mask[k0 + threadIdx.x]) ? 0.f : -INFINITY;
-    for (int kt = 0; kt < n; kt += 64) {
-        __syncthreads();
-        sk.store(ldsK);
-        sv.store(ldsV);
-        if (threadIdx.x < 64) bias[threadIdx.x] = nb;
-        __syncthreads();
-        const int next = kt + 64;
-        if (next < n) {
-            sk.load(ki + (int64_t)next * (2 * DP), min(64, n - next));
-            sv.load(vi + (int64_t)next * (2 * DP), min(64, n - next));
-            const int j = next + (int)threadIdx.x;
-            nb = threadIdx.x < 64 && j < n && (!a.mask || a.mask[k0 + j]) ? 0.f : -INFINITY;
-        }
-        const bool biased = a.mask != nullptr || kt + 64 > n;
+    for (int kt0 = 0; kt0 < n; kt0 += 64 * PART) {
+        const int kt1 = min(n, kt0 + 64 * PART);
+        for (int kt = kt0; kt < kt1; kt += 64) {
+            __syncthreads();
+            sk.store(ldsK);
+            sv.store(ldsV);
+            if (threadIdx.x < 64) bias[threadIdx.x] = nb;
+            __syncthreads();
+            const int next = kt + 64;
+            if (next < n) {
+                sk.load(ki + (int64_t)next * (2 * DP), min(64, n - next));
+                sv.load(vi + (int64_t)next * (2 * DP), min(64, n - next));
+                const int j = next + (int)threadIdx.x;
+                nb = threadIdx.x < 64 && j < n && (!a.mask || a.mask[k0 + j]) ? 0.f : -INFINITY;
+            }
+            const bool biased = a.mask != nullptr || kt + 64 > n;
 #pragma unroll
-        for (int kc = 0; kc < 2; ++kc) {
-            Frag df[QB];
-            {
-                f32x4 p[2][QB], s[2][QB];
+            for (int kc = 0; kc < 2; ++kc) {
+                Frag df[QB];
+                {
+                    f32x4 p[2][QB], s[2][QB];
 #pragma unroll
-                for (int b = 0; b < 2; ++b) {
-                    const int r0 = 32 * kc + 16 * b;
+                    for (int b = 0; b < 2; ++b) {
+                        const int r0 = 32 * kc + 16 * b;
 #pragma unroll
-                    for (int j = 0; j < QB; ++j) p[b][j] = s[b][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+                        for (int j = 0; j < QB; ++j) p[b][j] = s[b][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int k = 0; k < KC; ++k) {
-                        const Frag f = row_frag<DP>(ldsK, r0, k, lane);
+                        for (int k = 0; k < KC; ++k) {
+                            const Frag f = row_frag<DP>(ldsK, r0, k, lane);
 #pragma unroll
-                        for (int j = 0; j < QB; ++j) p[b][j] = mma3(f, q[j][k], p[b][j]);
-                    }
-#pragma unroll
-                    for (int k = 0; k < KC; ++k) {
-                        const Frag f = row_frag<DP>(ldsV, r0, k, lane);
-#pragma unroll
-                        for (int j = 0; j < QB; ++j) s[b][j] = mma3(f, go[j][k], s[b][j]);
-                    }
-                    if (biased) {
-                        const f32x4 o = *(const f32x4*)(bias + r0 + 4 * g);
-#pragma unroll
-                        for (int j = 0; j < QB; ++j) p[b][j] += o;
-                    }
-#pragma unroll
-                    for (int j = 0; j < QB; ++j)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const float e = exp2_fast(fmaf(p[b][j][i], c, ls[j]));
-                            s[b][j][i] = e * fmaf(s[b][j][i], 0x1p-17f, -de[j]);
+                            for (int j = 0; j < QB; ++j) p[b][j] = mma3(f, q[j][k], p[b][j]);
                         }
+#pragma unroll
+                        for (int k = 0; k < KC; ++k) {
+                            const Frag f = row_frag<DP>(ldsV, r0, k, lane);
+#pragma unroll
+                            for (int j = 0; j < QB; ++j) s[b][j] = mma3(f, go[j][k], s[b][j]);
+                        }
+                        if (biased) {
+                            const f32x4 o = *(const f32x4*)(bias + r0 + 4 * g);
+#pragma unroll
+                            for (int j = 0; j < QB; ++j) p[b][j] += o;
+                        }
+#pragma unroll
+                        for (int j = 0; j < QB; ++j)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const float e = exp2_fast(fmaf(p[b][j][i], c, ls[j]));
+                                s[b][j][i] = e * fmaf(s[b][j][i], 0x1p-17f, -de[j]);
+                            }
+                    }
+#pragma unroll
+                    for (int j = 0; j < QB; ++j) df[j] = split_frag(s[0][j], s[1][j], a.neg);
                 }
 #pragma unroll
-                for (int j = 0; j < QB; ++j) df[j] = split_frag(s[0][j], s[1][j], a.neg);
-            }
+                for (int d = 0; d < DB; ++d) {
+                    const Frag f = col_frag<DP>(ldsK, 32 * kc, d, lane);
 #pragma unroll
-            for (int d = 0; d < DB; ++d) {
-                const Frag f = col_frag<DP>(ldsK, 32 * kc, d, lane);
-#pragma unroll
-                for (int j = 0; j < QB; ++j) acc[d][j] = mma3(f, df[j], acc[d][j]);
+                    for (int j = 0; j < QB; ++j) acc[d][j] = mma3(f, df[j], acc[d][j]);
+                }
             }
+        }
+        if (TWO && kt1 < n) {
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int b = 0; b < QB; ++b) second.take(d * QB + b, acc[d][b]);
+            second.held = true;
         }
     }
 #pragma unroll
@@ -904,9 +982,9 @@ __global__ __launch_bounds__(64 * NW, at_bounds(DP, NW)) void k_at_dq(const AtAr
         const int e = eg[b] + ex[TV] + ex[TK] - 28;
 #pragma unroll
         for (int d = 0; d < DB; ++d) {
-            f32x4 x;
+            f32x4 x = second.total(d * QB + b, acc[d][b]);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] = ldexpf(acc[d][b][i] * a.scale, e);
+            for (int i = 0; i < 4; ++i) x[i] = ldexpf(x[i] * a.scale, e);
             store4(o, 16 * d + 4 * g, a.D, x);
         }
     }

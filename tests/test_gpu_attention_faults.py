@@ -109,3 +109,50 @@ def test_graphs_on_both_sides_of_the_limit_of_the_small_kernel(sizes, h, hk, d):
         want, bound = reference(q, k, v, sizes, m, d ** -0.5, g)
         for name, a, e, b in zip(("out", "dq", "dk", "dv"), got, want, bound):
             check(a, e, b, name)
+
+
+@pytest.mark.parametrize("mean", [0.0, 1.0])
+@pytest.mark.parametrize("h,hk,d", [(2, 1, 4), (1, 1, 23), (1, 1, 64), (1, 1, 128)])
+def test_long_sums(h, hk, d, mean):
+    """Sums over the 9 000 nodes of a graph, of values and gradients with and without a mean, against float64 by their norms.
+
+    The sums: parts of 1 024 rows in the matrix cores, six roundings per 64 rows, nine parts.  Where the terms do not cancel a part
+    grows to a ninth of the whole: sqrt(9 * 96 / 3) / 9 = 1.9, and nine additions sqrt(9 / 3) = 1.7;  where they cancel to a third:
+    sqrt(9 * 96 / 2) / 3 = 6.9, and sqrt(9 / 2) = 2.1;  10 in units of 2^-24 of the result holds both.  dv of heads of 33 ... 64 and 97 ...
+    128 columns has no second sum: sqrt(850 / 2) = 20.6 by the same count, and the cuts of one sign beside it: 40.
+    The terms: a probability is off by ln 2 times its logit's error (the exponent's rounding, |logit - M| < 32: 2^-20; three
+    sums of |logit| < 16: 3 * 2^-21; three times the pieces' 2^-24 of the products, below 16: 3 * 2^-23), exp2's 2^-23, its split's 2^-22: 5 * 2^-21
+    together, which also holds the relative error of dP and D in units of |dP| + |D| + the root of the products' squares.  Errors of
+    single terms are independent and add in squares.
+    dq: what D = sum_j p_j dP_j has from out's sum moves all terms of the row alike."""
+    n = 9000
+    q, k, v, g = make(n, h, hk, d, seed=d)
+    q *= 1.5
+    v += mean
+    g += mean
+    got = run(q, k, v, [n], g)
+    want, single = ([torch.zeros_like(t, dtype=torch.float64) for t in (q, q, k, v)] for _ in range(2))
+    common = torch.zeros_like(q, dtype=torch.float64)
+    scale = d ** -0.5
+    for i in range(h):
+        j = i * hk // h
+        Q, K, V, G = (t[:, x].double().contiguous() for t, x in ((q, i), (k, j), (v, j), (g, i)))
+        P = torch.softmax(scale * Q @ K.t().contiguous(), 1)
+        O = P @ V
+        D = (G * O).sum(1, keepdim=True)
+        dP = G @ V.t().contiguous()
+        T = scale * P * (dP - D)
+        M = (scale * P * (dP.abs() + D.abs() + ((G * G) @ (V * V).t().contiguous()).sqrt())) ** 2
+        want[0][:, i], want[1][:, i], common[:, i] = O, T @ K, scale * D * (P @ K)
+        want[2][:, j] += T.t().contiguous() @ Q
+        want[3][:, j] += P.t().contiguous() @ G
+        single[0][:, i], single[1][:, i] = (P * P) @ (V * V), M @ (K * K)
+        single[2][:, j] += M.t().contiguous() @ (Q * Q)
+        single[3][:, j] += (P * P).t().contiguous() @ (G * G)
+    for name, a, e, s in zip(("out", "dq", "dk", "dv"), got, want, single):
+        second = name != "dv" or d <= 32 or 64 < d <= 96
+        allowed = (10 if second else 40) * U * e.norm() + 5 * 2.0 ** -21 * s.sum().sqrt()
+        if name == "dq":
+            allowed = allowed + 10 * U * common.norm()
+        off = (a.double() - e).norm()
+        assert float(off) <= float(allowed), f"{name}: {float(off / allowed):.3g} of what is allowed"
