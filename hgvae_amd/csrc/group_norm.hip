@@ -60,7 +60,7 @@ struct GnArgs {
     int64_t rows;                     // of x, where its 8-bit form is kept
     double2* part;                    // [chunk][C] sums over a chunk's rows, from the first chunk of a larger graph on
     double2* colsum;                  // [rows of colsum][C] column sums (dz * xh, dz): one row per small workgroup, then per large graph
-    float4* gsum;                     // [B, groups] mean(a) in two pieces, mean(a * xh)
+    float2* gsum;                     // [B, groups] mean(a), mean(a * xh)
     int8_t* keep; uint8_t* keep_scale;                              // forward: where the 8-bit form of x goes (leading dimension ldq)
     int n_small, slab, nslabs, pad;   // pad: columns behind the last one that rows of out have for 16-byte access (zeroed)
 };
@@ -74,9 +74,10 @@ __device__ __forceinline__ Mean2 mean2(double m) {
     if (!(fabsf(r.hi) < 3.0e38f)) r.lo = 0.f;
     return r;
 }
-// a - mean(a) - xh * mean(a * xh), a = dz * w.  With mean(a) in two pieces and one rounding the first difference is exact where a is its
-// own mean: the gradient of a single value is zero by definition, and rstd would make 316 times the rounding of one piece of it.
-__device__ __forceinline__ float centred(float dz, float w, float xh, Mean2 m1, float m2) { return fmaf(dz, w, -m1.hi) - fmaf(xh, m2, m1.lo); }
+// a - mean(a) - xh * mean(a * xh), a = dz * w rounded by itself: where a is its own mean, the mean is the same rounding of the same product,
+// and the gradient of a single value is zero, as it is by definition (one rounding of a - mean(a) would leave that of the mean, times
+// rstd, which is 316 there).
+__device__ __forceinline__ float centred(float dz, float w, float xh, float m1, float m2) { return fmaf(-xh, m2, dz * w - m1); }
 __device__ __forceinline__ float normed(float x, Mean2 m, float rs) { return ((x - m.hi) - m.lo) * rs; }
 
 __device__ __forceinline__ float value8(const GnArgs& a, int64_t n, int c) {
@@ -209,8 +210,7 @@ __global__ __launch_bounds__(NT) void k_gn_small(const GnArgs a) {
                 red[ty * sc + tx] = make_double2(s1 * (double)w, s2 * (double)w);
             }
             reduce_slab(red, grp, sc, ty_n, a.per, NT, active, tx, ty);
-            const Mean2 m1 = mean2(grp[j].x / count);
-            const float m2 = (float)(grp[j].y / count);
+            const float m1 = (float)(grp[j].x / count), m2 = (float)(grp[j].y / count);
             if (active && a.out) {
 #pragma unroll
                 for (int i = 0; i < R; ++i) {
@@ -410,12 +410,8 @@ __global__ __launch_bounds__(1024) void k_gn_join(const GnArgs a, const int chun
     const int j = threadIdx.x;
     if (j < sc / a.per) {
         const int64_t at = (int64_t)graph * a.groups + c0 / a.per + j;
-        if (BWD) {
-            const Mean2 m1 = mean2(total.x / count);
-            a.gsum[at] = make_float4(m1.hi, m1.lo, (float)(total.y / count), 0.f);
-        } else {
-            stats_of(total, pivot_of(a, graph, c0 / a.per + j), count, a.eps, a.mean + at, a.rstd + at);
-        }
+        if (BWD) a.gsum[at] = make_float2((float)(total.x / count), (float)(total.y / count));
+        else stats_of(total, pivot_of(a, graph, c0 / a.per + j), count, a.eps, a.mean + at, a.rstd + at);
     }
 }
 
@@ -430,13 +426,12 @@ __global__ __launch_bounds__(256) void k_gn_apply(const GnArgs a, const int chun
     const int4 ch = a.chunks[chunk0 + (int)(gridDim.x - 1 - blockIdx.x)];
     GnCols<VEC> k;
     gn_cols<VEC>(a, ch.x, l.c, k);
-    Mean2 m1[VEC];
-    float m2[VEC];
+    float m1[VEC], m2[VEC];
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
         if (BWD) {
-            const float4 t = a.gsum[(int64_t)ch.x * a.groups + k.j[i]];
-            m1[i].hi = t.x; m1[i].lo = t.y; m2[i] = t.z;
+            const float2 t = a.gsum[(int64_t)ch.x * a.groups + k.j[i]];
+            m1[i] = t.x; m2[i] = t.y;
         }
     }
     const bool stored = !PACK || l.c < a.C;
@@ -590,7 +585,7 @@ extern "C" size_t hgv_group_norm_ws(int64_t n_chunks, int num_graphs, int listed
     size_t n = hgv_align256((size_t)n_chunks * C * sizeof(double2));
     if (backward) {
         n += hgv_align256((size_t)(min(n_small, SMALL_WGS) + listed - n_small) * C * sizeof(double2));
-        n += hgv_align256((size_t)num_graphs * groups * sizeof(float4));
+        n += hgv_align256((size_t)num_graphs * groups * sizeof(float2));
     }
     return n + 256;
 }
@@ -681,7 +676,7 @@ extern "C" int hgv_group_norm_bwd(const float* g, int64_t ldg, const float* x, i
     p += hgv_align256((size_t)(chunk1 - chunk0) * C * sizeof(double2));
     if (gw || gb) a.colsum = (double2*)p;
     p += hgv_align256((size_t)(min(n_small, SMALL_WGS) + listed - n_small) * C * sizeof(double2));
-    a.gsum = (float4*)p;
+    a.gsum = (float2*)p;
     return q ? gn_bwd<true>(act, a, listed, small_rows, chunk0, chunk1, gw, gb, stream)
              : gn_bwd<false>(act, a, listed, small_rows, chunk0, chunk1, gw, gb, stream);
 }
