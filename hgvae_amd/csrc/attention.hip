@@ -42,13 +42,13 @@ struct AtArgs {
 
     int max_rows;                                               // of the largest graph
     bool wide_g;                                                // rows of do can be read in 16 bytes (backward pass)
-    int* part;                                                  // [tile][4][Hk] exponents of the longest row
+    int* part;                                                  // [tile][5][Hk] exponents of the longest row;  [4]: of do where rows count 2^-lift
     int* exps;                                                  // [B][Hk][4]
     int* live;                                                  // [tile] keys that take part (backward pass)
-    int* keys;                                                  // [B] keys that take part: none, one, or 2 for more
+    int2* keys;                                                 // [B] keys that take part (none, one, or 2 for more), first tile of the graph
     _Float16* img[4];                                           // [heads][N][hi DP | lo DP]
     float* out;                                                 // [N, H, D]
-    float2* stats;                                              // [H, N] of a row: whole M with sum_j 2^(logit_j - M) in [1, 2), and 1 / that sum
+    float2* stats;                                              // [H, N] of a row: M + lift / 64 (see row_top), and 1 / sum_j 2^(logit_j - M)
     float* delta;                                               // [H, N] sum_d do * o over the row's sum, times 2^(13 - exponent of do)
     float* dq; float* dk; float* dv;                            // [N, H or Hk, D]
 };
@@ -100,6 +100,15 @@ __device__ __forceinline__ void load_vec(const AtArgs& a, int ten, int64_t n, in
 // e with |row| < 2^e, from the square of the norm
 __device__ __forceinline__ int above_norm(double square) { return ((((int)(__double_as_longlong(square) >> 52) & 2047) - 1023) >> 1) + 1; }
 
+// A row keeps a whole M with sum_j 2^(logit_j - M) in [1, 2), and beside it, as 64ths, by how many powers of two its probabilities may be
+// raised and stay below 2 (none where M needs the bits): the split of the logits' gradient has an absolute floor, and behind
+// probabilities of 1 / n it would be met by every term.
+__device__ __forceinline__ float with_lift(float M, float top) {
+    return fabsf(M) < 131072.f ? fmaf(fminf(fmaxf(floorf(M - top), 0.f), 31.f), 0.015625f, M) : M;
+}
+__device__ __forceinline__ float row_top(float x) { return floorf(x); }
+__device__ __forceinline__ int row_lift(float x) { return x < 1e30f ? (int)((x - floorf(x)) * 64.f) : 0; }
+
 // The largest of the workgroup's values.  red: four ints of LDS.
 __device__ __forceinline__ int max_of_all(int v, int* red) {
 #pragma unroll
@@ -113,11 +122,11 @@ __device__ __forceinline__ int max_of_all(int v, int* red) {
 // finite and not zero).
 template <int DP, bool VEC>
 __global__ __launch_bounds__(256) void k_at_norms(const AtArgs a, const int first) {
-    __shared__ int red[4];
+    __shared__ int red[2][4];
     const int ten = first + blockIdx.y, hk = blockIdx.z;
     const int4 tile = a.tiles[blockIdx.x];
     const int rows = min(64, (int)(a.ptr[tile.x + 1] - tile.y)), per = (ten == TQ || ten == TG) ? a.R : 1;
-    int best = NO_EXP;
+    int best = NO_EXP, lifted = NO_EXP;
     for (int i = threadIdx.x >> 4; i < rows * per; i += 16) {
         const int r = i / per;
         float v[DP / 16];
@@ -127,10 +136,19 @@ __global__ __launch_bounds__(256) void k_at_norms(const AtArgs a, const int firs
         for (int e = 0; e < DP / 16; ++e) s = fma((double)v[e], (double)v[e], s);
 #pragma unroll
         for (int o = 1; o < 16; o <<= 1) s += __shfl_xor(s, o, 64);
-        if (s > 0.0 && s < 1e300) best = max(best, above_norm(s));      // rows that hold an infinity or NaN do not count
+        if (s > 0.0 && s < 1e300) {                             // rows that hold an infinity or NaN do not count
+            const int e = above_norm(s);
+            best = max(best, e);
+            if (ten == TG) lifted = max(lifted, e - row_lift(a.stats[(int64_t)(hk * per + i - r * per) * a.N + tile.y + r].x));
+        }
     }
-    best = max_of_all(best, red);
-    if (threadIdx.x == 0) a.part[((int64_t)blockIdx.x * 4 + ten) * a.Hk + hk] = best;
+    best = max_of_all(best, red[0]);
+    if (ten == TG) lifted = max_of_all(lifted, red[1]);
+    if (threadIdx.x == 0) {
+        int* p = a.part + (int64_t)blockIdx.x * 5 * a.Hk + hk;
+        p[ten * a.Hk] = best;
+        if (ten == TG) p[4 * a.Hk] = lifted;
+    }
     if (a.live && ten == TK && hk == 0 && threadIdx.x < 64) {   // the first wave, whole
         const int i = threadIdx.x;
         const uint64_t takes = __ballot(i < rows && (!a.mask || a.mask[tile.y + i]));
@@ -149,7 +167,7 @@ __global__ __launch_bounds__(256) void k_at_split(const AtArgs a, const int firs
     const int ten = first + blockIdx.y, hk = blockIdx.z;
     const int4 tile = a.tiles[blockIdx.x];
     int e = NO_EXP;
-    for (int i = threadIdx.x; i < tile.w; i += 256) e = max(e, a.part[((int64_t)(tile.z + i) * 4 + ten) * a.Hk + hk]);
+    for (int i = threadIdx.x; i < tile.w; i += 256) e = max(e, a.part[((int64_t)(tile.z + i) * 5 + ten) * a.Hk + hk]);
     e = max_of_all(e, red);
     if (e == NO_EXP) e = 0;
     if (threadIdx.x == 0 && (int)blockIdx.x == tile.z) a.exps[((int64_t)tile.x * a.Hk + hk) * 4 + ten] = e;
@@ -161,7 +179,7 @@ __global__ __launch_bounds__(256) void k_at_split(const AtArgs a, const int firs
         }
         const bool many = __syncthreads_or(tiles > 1 || most > 1);
         const int holders = __syncthreads_count(tiles > 0);     // with not many: threads that saw one tile with one key
-        if (threadIdx.x == 0) a.keys[tile.x] = many ? 2 : min(holders, 2);
+        if (threadIdx.x == 0) a.keys[tile.x] = make_int2(many ? 2 : min(holders, 2), tile.z);
     }
     const int rows = min(64, (int)(a.ptr[tile.x + 1] - tile.y));
     const int per = (ten == TQ || ten == TG) ? a.R : 1, sub = threadIdx.x & 15;
@@ -370,7 +388,7 @@ constexpr int at_bounds(int DP, int NW) { return DP == 128 && NW == 4 ? 1 : 2; }
 template <int DP, int QB, bool RN, typename S2>
 __device__ __forceinline__ void fwd_tile(const unsigned char* ldsK, const unsigned char* ldsV, const float* bias, bool biased, int lane,
                                          const float (&c)[QB], const Frag (&q)[QB][DP / 32], float (&m)[QB], float (&l)[QB],
-                                         f32x4 (&acc)[DP / 16][QB], float neg, const S2& second) {
+                                         f32x4 (&acc)[DP / 16][QB], float neg, const S2& second, float (&most)[QB]) {
     constexpr int KC = DP / 32, DB = DP / 16;
     const int g = lane >> 4;
     f32x4 s[4][QB];
@@ -399,6 +417,7 @@ __device__ __forceinline__ void fwd_tile(const unsigned char* ldsK, const unsign
         for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i >> 2][b][i & 3]);
         top = fmaxf(top, __shfl_xor(top, 16, 64));
         top = fmaxf(top, __shfl_xor(top, 32, 64)) * c[b];
+        most[b] = fmaxf(most[b], top);
         // rescale only when a probability would leave its range
         if (__any(top > m[b] + P_GROW || (m[b] == -INFINITY && top > -INFINITY))) {
             const float mn = ceilf(fmaxf(m[b], top));      // whole: what is subtracted is then exact, and so are the rescales
@@ -438,7 +457,7 @@ __device__ __forceinline__ void fwd_tile(const unsigned char* ldsK, const unsign
 // The rows of a wave's queries, and their stats; ev: exponent of the values' scale.
 template <int DP, int QB, typename S2>
 __device__ __forceinline__ void fwd_rows(const AtArgs& a, int64_t q0, int64_t k1, int h, int lane, int ev, const float (&m)[QB], float (&l)[QB],
-                                         const f32x4 (&acc)[DP / 16][QB], const S2& second) {
+                                         const f32x4 (&acc)[DP / 16][QB], const S2& second, const float (&most)[QB]) {
     constexpr int DB = DP / 16;
     const int g = lane >> 4;
 #pragma unroll
@@ -454,7 +473,7 @@ __device__ __forceinline__ void fwd_rows(const AtArgs& a, int64_t q0, int64_t k1
         for (int d = 0; d < DB; ++d) store4(o, 16 * d + 4 * g, a.D, none ? f32x4{0.f, 0.f, 0.f, 0.f} : second.total(d * QB + b, acc[d][b]) * f);
         if (g == 0 && a.stats) {
             const int e = (int)(__float_as_uint(l[b]) >> 23) - 127;         // l = 2^e * (1 ... 2)
-            a.stats[(int64_t)h * a.N + row] = none ? make_float2(INFINITY, 0.f) : make_float2(m[b] - P_BITS + (float)e, ldexpf(1.f / l[b], e));
+            a.stats[(int64_t)h * a.N + row] = none ? make_float2(INFINITY, 0.f) : make_float2(with_lift(m[b] - P_BITS + (float)e, most[b]), ldexpf(1.f / l[b], e));
         }
     }
 }
@@ -490,9 +509,9 @@ __global__ __launch_bounds__(64 * NW, DP == 32 ? 4 : at_bounds(DP, NW)) void k_a
 #pragma unroll
         for (int k = 0; k < KC; ++k) q[b][k] = own_frag<DP>(a.img[TQ] + (int64_t)h * a.N * (2 * DP), min(q0 + 16 * b + (lane & 15), k1 - 1), k, lane);
     f32x4 acc[DB][QB];
-    float m[QB], l[QB];                                         // m: the exponent that is subtracted, base 2
+    float m[QB], l[QB], most[QB];                               // the exponent that is subtracted, base 2;  the sum;  the largest logit
 #pragma unroll
-    for (int b = 0; b < QB; ++b) { m[b] = -INFINITY; l[b] = 0.f; }
+    for (int b = 0; b < QB; ++b) { m[b] = most[b] = -INFINITY; l[b] = 0.f; }
 #pragma unroll
     for (int d = 0; d < DB; ++d)
 #pragma unroll
@@ -520,7 +539,7 @@ __global__ __launch_bounds__(64 * NW, DP == 32 ? 4 : at_bounds(DP, NW)) void k_a
                 nb = threadIdx.x < 64 && j < n && (!a.mask || a.mask[k0 + j]) ? 0.f : -INFINITY;
             }
             const bool biased = a.mask != nullptr || kt + 64 > n;
-            fwd_tile<DP, QB, false>(ldsK, ldsV, bias, biased, lane, c, q, m, l, acc, a.neg, second);
+            fwd_tile<DP, QB, false>(ldsK, ldsV, bias, biased, lane, c, q, m, l, acc, a.neg, second, most);
         }
         if (TWO && kt1 < n) {
 #pragma unroll
@@ -530,7 +549,7 @@ __global__ __launch_bounds__(64 * NW, DP == 32 ? 4 : at_bounds(DP, NW)) void k_a
             second.held = true;
         }
     }
-    fwd_rows<DP, QB>(a, q0, k1, h, lane, ex[TV], m, l, acc, second);
+    fwd_rows<DP, QB>(a, q0, k1, h, lane, ex[TV], m, l, acc, second, most);
 }
 
 // Graphs of few rows: the operands as they are, without images.  Every workgroup splits what it multiplies on the way into the
@@ -612,9 +631,9 @@ __global__ __launch_bounds__(64 * NW, DP == 32 ? 3 : at_bounds(DP, NW)) void k_a
         }
     }
     f32x4 acc[DB][QB];
-    float m[QB], l[QB];
+    float m[QB], l[QB], most[QB];
 #pragma unroll
-    for (int b = 0; b < QB; ++b) { m[b] = -INFINITY; l[b] = 0.f; }
+    for (int b = 0; b < QB; ++b) { m[b] = most[b] = -INFINITY; l[b] = 0.f; }
 #pragma unroll
     for (int d = 0; d < DB; ++d)
 #pragma unroll
@@ -669,9 +688,9 @@ __global__ __launch_bounds__(64 * NW, DP == 32 ? 3 : at_bounds(DP, NW)) void k_a
         float c[QB];
 #pragma unroll
         for (int b = 0; b < QB; ++b) c[b] = fold_scale(a.scale, eq[b] + ek - 30);
-        fwd_tile<DP, QB, true>(ldsK, ldsV, bias, biased, lane, c, q, m, l, acc, a.neg, none);
+        fwd_tile<DP, QB, true>(ldsK, ldsV, bias, biased, lane, c, q, m, l, acc, a.neg, none, most);
     }
-    fwd_rows<DP, QB>(a, q0, k1, h, lane, ev, m, l, acc, none);
+    fwd_rows<DP, QB>(a, q0, k1, h, lane, ev, m, l, acc, none, most);
 }
 
 // ---- backward: dk and dv ---------------------------------------------------------------------------------------------------
@@ -711,8 +730,15 @@ __global__ __launch_bounds__(64 * NW, DP == 32 ? 3 : at_bounds(DP, NW)) void k_a
 #pragma unroll
         for (int b = 0; b < KB; ++b) dk[d][b] = dv[d][b] = f32x4{0.f, 0.f, 0.f, 0.f};
     const int n = (int)(g1 - g0), tiles = (n + 63) / 64, steps = tiles * a.R;
+    // What the logits' gradient of a part's queries is multiplied by before it is split: 2^up, as far as their longest gradients and largest
+    // probabilities allow (not the graph's).  The part's exponents are loaded one part ahead, a tile per lane.  15 200 nodes, dk from 64
+    // bits with one scale / scales per part: all rows alike 7.8e-7 / 5.0e-7, one row with 1 024 times the gradient 3.8e-5 / 6.7e-7, one with
+    // 1 024 times the value 7.5e-5 / 1.3e-6;  1 to 1.5 % of this kernel's time.  (A scale per tile of 64 rows: 2 to 3.5 %.)
+    static_assert(TWO, "parts of dk have scales of their own");
+    const int2 keys = a.keys[t.x];
     Stage<DP, 64 * NW> sq, sg;
     float nl = INFINITY, nd = 0.f;
+    int up = 0;
     auto fetch = [&](int step) __attribute__((always_inline)) {
         const int hh = hk * a.R + step / tiles, r0 = (step % tiles) * 64, rows = min(64, n - r0);
         const int64_t at = (int64_t)hh * a.N + g0 + r0;
@@ -724,16 +750,28 @@ __global__ __launch_bounds__(64 * NW, DP == 32 ? 3 : at_bounds(DP, NW)) void k_a
             nd = a.delta[at + threadIdx.x];
         }
     };
+    static_assert(PART == 16, "sixteen lanes");
+    auto limits = [&](int from) __attribute__((always_inline)) {
+        const int step = min(from + (lane & 15), steps - 1);
+        return a.part[((int64_t)(keys.y + step % tiles) * 5 + 4) * a.Hk + hk];
+    };
+    int ahead = limits(0);
     fetch(0);
     for (int step0 = 0; step0 < steps; step0 += PART) {
         const int step1 = min(steps, step0 + PART);
+        int top = ahead;
+#pragma unroll
+        for (int o = 1; o < 16; o <<= 1) top = max(top, __shfl_xor(top, o, 64));
+        up = min(__builtin_amdgcn_readfirstlane(ex[TG] - top), 60);
+        if (step1 < steps) ahead = limits(step1);
+        const float unit = __uint_as_float((uint32_t)(127 - 17 + up) << 23);
         for (int step = step0; step < step1; ++step) {
             __syncthreads();
             sq.store(ldsQ);
             sg.store(ldsG);
             if (threadIdx.x < 64) {
-                ldsL[threadIdx.x] = -nl;
-                ldsD[threadIdx.x] = ldexpf(nd, -ex[TV]);
+                ldsL[threadIdx.x] = -row_top(nl);
+                ldsD[threadIdx.x] = ldexpf(nd, up - ex[TV]);
             }
             __syncthreads();
             if (step + 1 < steps) fetch(step + 1);
@@ -765,7 +803,7 @@ __global__ __launch_bounds__(64 * NW, DP == 32 ? 3 : at_bounds(DP, NW)) void k_a
 #pragma unroll
                             for (int i = 0; i < 4; ++i) {
                                 p[b][j][i] = exp2_fast(fmaf(p[b][j][i], c, ls[i]));
-                                s[b][j][i] = p[b][j][i] * fmaf(s[b][j][i], 0x1p-17f, -de[i]);
+                                s[b][j][i] = p[b][j][i] * fmaf(s[b][j][i], unit, -de[i]);
                                 p[b][j][i] *= 0x1p14f;
                             }
                     }
@@ -790,10 +828,12 @@ __global__ __launch_bounds__(64 * NW, DP == 32 ? 3 : at_bounds(DP, NW)) void k_a
             }
         }
         if (TWO && step1 < steps) {
+            const float down = ldexpf(1.f, -up);
 #pragma unroll
             for (int d = 0; d < DB; ++d)
 #pragma unroll
                 for (int b = 0; b < KB; ++b) {
+                    dk[d][b] *= down;
                     second.take(d * KB + b, dk[d][b]);
                     if (BOTH) second.take((DB + d) * KB + b, dv[d][b]);
                 }
@@ -804,13 +844,14 @@ __global__ __launch_bounds__(64 * NW, DP == 32 ? 3 : at_bounds(DP, NW)) void k_a
     for (int b = 0; b < KB; ++b) {
         const int64_t row = key0 + 16 * b + (lane & 15);
         if (row >= g1) continue;
-        const bool live = !a.mask || a.mask[row], many = a.keys[t.x] > 1;
+        const bool live = !a.mask || a.mask[row], many = keys.x > 1;
         float* pk = row_out(a.dk, row, a.Hk, hk, a.D);
         float* pv = row_out(a.dv, row, a.Hk, hk, a.D);
+        const float down = ldexpf(1.f, -up);
         const int ek = ex[TG] + ex[TV] + ex[TQ] - 28, ev = ex[TG] - 29;
 #pragma unroll
         for (int d = 0; d < DB; ++d) {
-            f32x4 x = second.total(d * KB + b, dk[d][b]), y = BOTH ? second.total((DB + d) * KB + b, dv[d][b]) : dv[d][b];
+            f32x4 x = second.total(d * KB + b, dk[d][b] * down), y = BOTH ? second.total((DB + d) * KB + b, dv[d][b]) : dv[d][b];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 x[i] = live && many ? ldexpf(x[i] * a.scale, ek) : 0.f;
@@ -830,7 +871,8 @@ __global__ __launch_bounds__(64 * NW, DP == 32 ? 3 : at_bounds(DP, NW)) void k_a
 // The incoming gradient comes from the operand itself and not from its image: each query's row has a power of two of its own, by the
 // row's own norm, up to the split of the logits' gradient.  With the scale of the longest row, a row F times shorter reached that split
 // log2 F bits lower, behind probabilities of 1 / n already (one row of 5 000 with 16 384 times the others' gradient, the others' dq by row:
-// 1.6e-3 from 64 bits; so 2e-6, the formulas in fp32 2.5e-6).
+// 1.6e-3 from 64 bits; so 8e-7, the formulas in fp32 2.5e-6).  A row's probabilities are raised by its lift on the way (one value of 15 200
+// 1 024 times the others: dq 4.6e-5 without, 6.3e-7 with).
 template <int DP, int QB, int NW>
 __global__ __launch_bounds__(64 * NW, DP == 32 ? 3 : at_bounds(DP, NW)) void k_at_dq(const AtArgs a) {
     constexpr int KC = DP / 32, DB = DP / 16;
@@ -846,7 +888,7 @@ __global__ __launch_bounds__(64 * NW, DP == 32 ? 3 : at_bounds(DP, NW)) void k_a
     const int4 t = a.blocks[blk];
     const int64_t k0 = a.ptr[t.x], k1 = a.ptr[t.x + 1];
     const int64_t q0 = (int64_t)t.y + 16 * QB * wave;
-    if (a.keys[t.x] < 2) {                                      // the same for the whole workgroup
+    if (a.keys[t.x].x < 2) {                                      // the same for the whole workgroup
 #pragma unroll
         for (int b = 0; b < QB; ++b) {
             const int64_t row = q0 + 16 * b + (lane & 15);
@@ -860,7 +902,7 @@ __global__ __launch_bounds__(64 * NW, DP == 32 ? 3 : at_bounds(DP, NW)) void k_a
     const float c = fold_scale(a.scale, ex[TQ] + ex[TK] - 30);
     Frag q[QB][KC], go[QB][KC];
     float ls[QB], de[QB];
-    int eg[QB];                                                 // exponent of the row's own scale
+    int eg[QB], lift[QB];                                       // exponent of the row's own scale
 #pragma unroll
     for (int b = 0; b < QB; ++b) {
         const int64_t row = min(q0 + 16 * b + (lane & 15), k1 - 1);
@@ -889,7 +931,8 @@ __global__ __launch_bounds__(64 * NW, DP == 32 ? 3 : at_bounds(DP, NW)) void k_a
                 for (int j = 0; j < 4; ++j) x[k][i][j] = ldexpf(x[k][i][j], 15 - eg[b]);
             go[b][k] = split_frag<true>(x[k][0], x[k][1], a.neg);
         }
-        ls[b] = -st.x;
+        lift[b] = row_lift(st.x);
+        ls[b] = (float)lift[b] - row_top(st.x);                 // probabilities of up to 1 ... 2
         de[b] = ldexpf(a.delta[(int64_t)h * a.N + row], ex[TG] - eg[b] - ex[TV]);
     }
     f32x4 acc[DB][QB];
@@ -979,7 +1022,7 @@ __global__ __launch_bounds__(64 * NW, DP == 32 ? 3 : at_bounds(DP, NW)) void k_a
         const int64_t row = q0 + 16 * b + (lane & 15);
         if (row >= k1) continue;
         float* o = row_out(a.dq, row, a.H, h, a.D);
-        const int e = eg[b] + ex[TV] + ex[TK] - 28;
+        const int e = eg[b] - lift[b] + ex[TV] + ex[TK] - 28;
 #pragma unroll
         for (int d = 0; d < DB; ++d) {
             f32x4 x = second.total(d * QB + b, acc[d][b]);
@@ -1000,10 +1043,10 @@ struct AtSizes { size_t part, exps, live, keys, img[4], delta, total; };
 AtSizes at_sizes(int64_t N, int H, int Hk, int D, int64_t n_tiles, int64_t graphs, bool backward) {
     AtSizes s;
     const size_t row = (size_t)at_dp(D) * 4;
-    s.part = hgv_align256((size_t)n_tiles * 4 * Hk * sizeof(int));
+    s.part = hgv_align256((size_t)n_tiles * 5 * Hk * sizeof(int));
     s.exps = hgv_align256((size_t)graphs * Hk * 4 * sizeof(int));
     s.live = backward ? hgv_align256((size_t)n_tiles * sizeof(int)) : 0;
-    s.keys = backward ? hgv_align256((size_t)graphs * sizeof(int)) : 0;
+    s.keys = backward ? hgv_align256((size_t)graphs * sizeof(int2)) : 0;
     s.img[TQ] = hgv_align256((size_t)N * H * row);
     s.img[TK] = s.img[TV] = hgv_align256((size_t)N * Hk * row);
     s.img[TG] = backward ? s.img[TQ] : 0;
@@ -1106,7 +1149,7 @@ int at_fill(AtArgs& a, const char* what, int64_t N, int num_graphs, int H, int H
     a.exps = (int*)p; p += s.exps;
     if (backward) {
         a.live = (int*)p; p += s.live;
-        a.keys = (int*)p; p += s.keys;
+        a.keys = (int2*)p; p += s.keys;
     }
     for (int i = 0; i < 4; ++i) { a.img[i] = (_Float16*)p; p += s.img[i]; }
     a.delta = (float*)p;

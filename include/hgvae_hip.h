@@ -620,8 +620,8 @@ int hgv_group_norm_bwd(const float* g, int64_t ldg, const float* x, int64_t ldx,
  * A masked row of k or v may hold anything; its dk and dv are zeros.  scale > 0.
  * Graphs: ptr [num_graphs + 1], the largest has max_rows rows; tiles [n_tiles][4] (graph, first row, first tile of the graph, tiles of the graph) of 64 rows;
  * blocks [n64 + n128][4] (graph, first row, -, -): all tiles of 64 rows, then those of 128, in the order in which they are to run.
- * stats [H, N, 2] (8-byte aligned; per row a whole M with sum_j 2^(logit_j - M) in [1, 2), base 2 of the scaled logits, and the
- * inverse of that sum; +inf and 0 for a row without keys) may be NULL in the forward pass; the backward pass
+ * stats [H, N, 2] (8-byte aligned; per row a whole M with sum_j 2^(logit_j - M) in [1, 2), base 2 of the scaled logits, plus k / 64, where
+ * 2^k times the largest of these powers is below 2 (0 <= k < 32; 0 for |M| >= 2^17), and the inverse of that sum; +inf and 0 for a row without keys) may be NULL in the forward pass; the backward pass
  * reads it and out.  dq, or dk and dv together, may be NULL. */
 size_t hgv_graph_attention_ws(int64_t N, int num_graphs, int H, int Hk, int D, int64_t n_tiles, int backward);
 /* ... of the forward pass over graphs of at most max_rows rows: next to nothing where all are small. */

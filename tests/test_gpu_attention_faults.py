@@ -156,3 +156,33 @@ def test_long_sums(h, hk, d, mean):
             allowed = allowed + 10 * U * common.norm()
         off = (a.double() - e).norm()
         assert float(off) <= float(allowed), f"{name}: {float(off / allowed):.3g} of what is allowed"
+
+
+@pytest.mark.parametrize("h,hk,d", [(1, 1, 64), (2, 1, 23), (1, 1, 96)])
+@pytest.mark.parametrize("which", ["g", "v"])
+@pytest.mark.parametrize("factor", [2.0 ** 6, 2.0 ** 10, 2.0 ** 16])
+def test_dq_and_dk_beside_one_large_row(h, hk, d, which, factor):
+    """One row of g or of v far larger than the others of its graph: dq and dk as a whole stay as exact as fp32 is.
+
+    The logits' gradient is split with an absolute floor 2^-25 under a bound of 2^14 that holds for the largest gradient and the largest
+    probability of 1 024 rows (dk) or of the row (dq).  A term of ordinary size, |dP| about |do| |v| / 8, next to its bound: 2^11.  With a large row of v
+    the bound is F times too high for all others: 2^11 / F, at F = 2^10 2^1 with errors of 2^-26, and the large row's own
+    terms, p F |do| |v|, of which n are summed, are as many times larger: 6 000 errors of 2^-26 against 2^11, 2^-31 of the whole.
+    So the bound is that of the long sums, 10 * 2^-24 of the norm, and of single terms' errors, 5 * 2^-21 in squares, where they cancel in
+    full: 50 * 2^-24 at most."""
+    n = 6000
+    q, k, v, g = make(n, h, hk, d, seed=d)
+    (g if which == "g" else v)[n // 3] *= factor
+    _, dq, dk, _ = run(q, k, v, [n], g)
+    want = [torch.zeros_like(t, dtype=torch.float64) for t in (q, k)]
+    scale = d ** -0.5
+    for i in range(h):
+        j = i * hk // h
+        Q, K, V, G = (t[:, x].double().contiguous() for t, x in ((q, i), (k, j), (v, j), (g, i)))
+        P = torch.softmax(scale * Q @ K.t().contiguous(), 1)
+        T = scale * P * (G @ V.t().contiguous() - (G * (P @ V)).sum(1, keepdim=True))
+        want[0][:, i] = T @ K
+        want[1][:, j] += T.t().contiguous() @ Q
+    for name, a, e in zip(("dq", "dk"), (dq, dk), want):
+        off = float((a.double() - e).norm() / e.norm())
+        assert off <= 50 * U, f"{name}: {off:.3g}"
